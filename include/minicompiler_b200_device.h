@@ -268,6 +268,81 @@ MCD_API int mcd_tensor_core_supported(int device, int arith);
 MCD_API int mcd_gemm_f32_split_no_alloc(const float* a, const float* b, float* c, int m, int n, int k, int splits,
                                         void* stream);
 
+/* ------------------------------------------- microscaled 4-bit floating point
+ * No counterpart in the reference, whose narrowest multiplicands are 16 bits wide
+ * (src/cuda/matmul_tensor_core.cu:45-57). A matrix is held as e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives) that share a scale per block of consecutive columns of a row:
+ *   MCD_FP4_E8M0_32  blocks of 32, the scale a power of two (e8m0: byte b stands for 2^(b-127), 255 for NaN);
+ *   MCD_FP4_E4M3_16  blocks of 16, the scale an e4m3 number without its sign (0 .. 448, 0x7F is NaN), and one
+ *                    f32 number per matrix (`tensor_scale`) on top.
+ * The value of an element is code * block scale (* tensor scale).
+ *
+ * Layout in device memory, for each of `batch` matrices [rows, cols] one behind the other:
+ *   codes   row-major, two per byte, the even column in the low four bits. A row takes mcd_fp4_code_pitch(cols)
+ *           bytes (16 for every 32 columns begun); the codes behind the last column are 0.
+ *   scales  tiles of 512 bytes, each 128 rows x 4 blocks, the tiles of the same 128 rows one behind the other:
+ *           row r, block b at tile (r/128) * ceil(blocks/4) + b/4, byte (r%32)*16 + (r/32%4)*4 + b%4, which is the
+ *           order the tensor cores take scales in. Bytes that belong to no block are 0.
+ * mcd_fp4_quantize writes both in full, the padding included; who fills them otherwise must do the same. */
+#define MCD_FP4_E8M0_32 1
+#define MCD_FP4_E4M3_16 2
+
+/* Types of dense values in the calls below; the 16-bit ones are MCD_HALF_*. */
+#define MCD_TYPE_F32 0
+
+typedef struct mcd_fp4_tensor {
+    int format;       /* MCD_FP4_* */
+    int batch;        /* matrices, 1 for a single one */
+    long long rows;   /* of one matrix, at most 2^31 - 1 */
+    long long cols;
+    void* codes;      /* device, 16-byte aligned */
+    void* scales;     /* device, 16-byte aligned */
+    const float* tensor_scale; /* device, `batch` floats > 0; NULL = 1. E8M0_32 has none (must be NULL) */
+} mcd_fp4_tensor;
+
+MCD_API long long mcd_fp4_code_pitch(long long cols);               /* bytes per row of codes */
+MCD_API size_t mcd_fp4_codes_bytes(long long rows, long long cols, int batch);
+MCD_API size_t mcd_fp4_scales_bytes(int format, long long rows, long long cols, int batch); /* 0: unknown format */
+
+/* out[i] = max(largest finite magnitude of matrix i / 2688, 2^-120): the tensor scale that takes the largest value to
+ * 6 * 448, the end of E4M3_16's range. `src` holds [batch, rows, cols] of `type`, `pitch` elements from row to row,
+ * rows * pitch from matrix to matrix. NaN and infinities are passed over. An empty or zero matrix gets 1. */
+MCD_API int mcd_fp4_tensor_scale(int type, const void* src, long long rows, long long cols, long long pitch, int batch,
+                                 float* out, void* stream);
+/* Rounds [batch, rows, cols] values of `type` (same layout rule) into `dst`. With amax the largest magnitude of a block:
+ *   E8M0_32: scale 2^e, e = max(floor(log2 amax) - 2, -127); codes are x / 2^e to nearest, ties to even, at most 6.
+ *   E4M3_16: scale s = amax / (6 g) in f32, rounded to e4m3 (nearest even, at most 448), g the tensor scale; codes are
+ *            x * (1 / (s g)), each step in f32, to nearest even, at most 6. A block with s g = 0 has codes 0.
+ * A block that holds a NaN or an infinity gets the NaN scale and codes 0, so that every product with it is NaN; so do
+ * all blocks when g is not a positive finite number. Works on `stream`; one launch. */
+MCD_API int mcd_fp4_quantize(int type, const void* src, long long pitch, const mcd_fp4_tensor* dst, void* stream);
+/* The values `src` stands for, rounded once to `type` (f32: E8M0_32 exactly unless the value is below f32's range). */
+MCD_API int mcd_fp4_dequantize(const mcd_fp4_tensor* src, int type, void* dst, long long pitch, void* stream);
+
+/* C[m,n] = A * B^T with A [m,k] and B [n,k] held in the same 4-bit format (batch 1), on the tensor cores' block-scaled
+ * multiply, accumulated in f32; A's and B's tensor scales multiply the finished sum. k is cols of both.
+ *  c          [m,n] of c_type (MCD_TYPE_F32 or MCD_HALF_*), ldc elements from row to row. Only the m x n elements are
+ *             written.
+ *  workspace  mcd_fp4_gemm_workspace(args) bytes of device memory, 16-byte aligned, or NULL where that is 0. Calls that
+ *             may run at the same time (two streams, two captured graphs) need one each.
+ *  status     device word, may be NULL: a kernel that gives up a bounded wait ORs an error code in (as in mcd_gemm).
+ * Results do not depend on scheduling: K slices are added in a fixed order. */
+typedef struct mcd_fp4_gemm_args {
+    mcd_fp4_tensor a;
+    mcd_fp4_tensor b;
+    void* c;
+    int c_type;
+    long long ldc;
+    void* workspace;
+    size_t workspace_bytes;
+    unsigned int* status;
+} mcd_fp4_gemm_args;
+
+/* Bytes of workspace for a problem of this size (c, workspace and operand pointers are not looked at). */
+MCD_API size_t mcd_fp4_gemm_workspace(const mcd_fp4_gemm_args* args);
+MCD_API int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream);
+MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
+
 #ifdef __cplusplus
 }
 #endif

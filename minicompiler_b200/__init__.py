@@ -24,13 +24,29 @@ from .api import (  # noqa: F401
     tensor_core_tile_n,
     uniform_values,
 )
+from .fp4 import (  # noqa: F401
+    Fp4Gemm,
+    Fp4Matrix,
+    fp4_dequantize,
+    fp4_gemm_workspace_bytes,
+    fp4_quantize,
+    fp4_sizes,
+    fp4_tensor_scale,
+)
 
 __all__ = [
     "Communicator",
     "CompiledGraph",
+    "Fp4Gemm",
+    "Fp4Matrix",
     "HostGraph",
     "McError",
     "compile_graph",
+    "fp4_dequantize",
+    "fp4_gemm_workspace_bytes",
+    "fp4_quantize",
+    "fp4_sizes",
+    "fp4_tensor_scale",
     "graph_path",
     "lib",
     "resolve_matmul_kernel",

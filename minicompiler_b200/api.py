@@ -114,6 +114,15 @@ def lib() -> C.CDLL:
         "mcb_tensor_core_tile_n": (i32, [i32, i32, i32, i32, i32]),
         "mcb_resolve_matmul_kernel": (cp, [cp, i32, i32, i32, i32]),
         "mcd_launch_count": (C.c_ulonglong, []),
+        "mcd_fp4_code_pitch": (i64, [i64]),
+        "mcd_fp4_codes_bytes": (C.c_size_t, [i64, i64, i32]),
+        "mcd_fp4_scales_bytes": (C.c_size_t, [i32, i64, i64, i32]),
+        "mcd_fp4_tensor_scale": (i32, [i32, vp, i64, i64, i64, i32, vp, vp]),
+        "mcd_fp4_quantize": (i32, [i32, vp, i64, vp, vp]),
+        "mcd_fp4_dequantize": (i32, [vp, i32, vp, i64, vp]),
+        "mcd_fp4_gemm_workspace": (C.c_size_t, [vp]),
+        "mcd_fp4_gemm": (i32, [vp, vp]),
+        "mcd_fp4_gemm_launches": (i32, [vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

@@ -80,6 +80,7 @@ const DriverApi* driver_api() {
         ok = resolve("cuFuncSetAttribute", api.FuncSetAttribute) && ok;
         ok = resolve("cuOccupancyMaxActiveBlocksPerMultiprocessor", api.OccupancyMaxActiveBlocksPerMultiprocessor) && ok;
         ok = resolve("cuTensorMapEncodeTiled", api.TensorMapEncodeTiled) && ok;
+        ok = resolve("cuPointerGetAttribute", api.PointerGetAttribute) && ok;
         usable = ok;
     });
     return usable ? &api : nullptr;

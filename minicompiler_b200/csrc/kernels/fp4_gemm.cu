@@ -1,0 +1,504 @@
+// mcd_fp4_gemm: C[m,n] = A[m,k] * B[n,k]^T with both operands in a microscaled 4-bit format, on the tensor cores'
+// block-scaled multiply (tcgen05.mma kind::mxf4 / kind::mxf4nvf4). The products code * code and the scales are exact in
+// the multiplier; sums are f32.
+//
+//   sum over k of (a b) = sum over blocks of s_a s_b * (sum over the block of code_a code_b)
+//
+// An instruction covers 64 columns of k; the scales it needs lie in TMEM, brought there from shared memory by
+// tcgen05.cp, which the tensor core executes in order with the multiplies behind it.
+
+#include "minicompiler_b200_device.h"
+
+#include "device/driver_api.hpp"
+#include "device/per_device.hpp"
+#include "kernels/fp4_host.hpp"
+#include "kernels/fp4_mma.cuh"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+using namespace mcd;
+
+namespace {
+
+#define MC_FP4_ERR_PRODUCER 0x100u
+#define MC_FP4_ERR_MMA 0x200u
+#define MC_FP4_ERR_EPILOGUE 0x400u
+#define MC_FP4_ERR_DRAIN 0x800u
+
+constexpr int kTileRows = 128;   // TMEM lanes
+constexpr int kRaster = 16;      // row tiles per band of work items
+
+struct Fp4GemmParams {
+    // "rows" is the operand on the 128 TMEM lanes, "columns" the one whose rows are accumulator columns
+    const unsigned char* row_scales;
+    const unsigned char* col_scales;
+    long long k_tiles;  // scale tiles per 128 rows
+    const float* row_scale;  // tensor scales, may be null
+    const float* col_scale;
+    void* c;
+    float* workspace;
+    unsigned* status;
+    long long ldc;
+    int c_type;
+    int rows, cols, k;
+    int k_blocks, k_blocks_per_split, splits;
+    int swapped;  // 0: rows are C's rows; 1: rows are C's columns
+};
+
+__device__ __forceinline__ void store_c(void* c, int type, long long at, float v) {
+    if (type == MCD_TYPE_F32) {
+        static_cast<float*>(c)[at] = v;
+    } else {
+        unsigned short h;
+        if (type == MCD_HALF_BF16) {
+            asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(h) : "f"(v));
+        } else {
+            asm("cvt.rn.f16.f32 %0, %1;" : "=h"(h) : "f"(v));
+        }
+        static_cast<unsigned short*>(c)[at] = h;
+    }
+}
+
+__device__ __forceinline__ unsigned pack_half2(float lo, float hi, int type) {
+    unsigned d;
+    if (type == MCD_HALF_BF16) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    } else {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    }
+    return d;
+}
+
+__device__ __forceinline__ float product_scale(const float* a, const float* b) {
+    return (a != nullptr ? *a : 1.0f) * (b != nullptr ? *b : 1.0f);
+}
+
+// ------------------------------------------------------------------------------------------------ one CTA per tile
+//
+// 128 rows x kCols columns, K in blocks of 256 codes (128 bytes per tile row). Warp 0 brings tiles and scales into a ring
+// of stages, warp 1 issues copies of scales and multiplies, warps 2-5 drain one of two accumulators while the other is
+// being filled.
+
+template <int kFormat, int kCols>
+struct Fp4Tile {
+    static constexpr int kScaleTiles = kFormat == MCD_FP4_E8M0_32 ? 2 : 4;  // per K block
+    static constexpr int kRowBytes = kTileRows * 128;
+    static constexpr int kColBytes = kCols * 128;
+    static constexpr int kScaleBytes = kScaleTiles * kFp4TileBytes;
+    static constexpr int kStageBytes = kRowBytes + kColBytes + 2 * kScaleBytes;
+    static constexpr int kStages = std::min(10, 222000 / kStageBytes);
+    static constexpr int kBarrierBytes = 512;
+    static constexpr int kSmem = kStages * kStageBytes + 1024 + kBarrierBytes;
+    static constexpr int kAccColumns = kCols < 32 ? 32 : kCols;
+    static constexpr int kScaleColumns = kScaleTiles * 4;
+    static constexpr int kScaleBase = 2 * kAccColumns;
+    static_assert(kScaleBase + kStages * 2 * kScaleColumns <= 512, "TMEM columns");
+    static_assert(kStages * 16 + 32 <= kBarrierBytes, "barriers");
+};
+
+constexpr int kOneCtaThreads = 64 + 128;
+
+__device__ __forceinline__ void fp4_decode_item(int item, int tiles_r, int tiles_c, int splits, int& rb, int& cb, int& split) {
+    split = item % splits;
+    const int tile = item / splits;
+    const int band_tiles = kRaster * tiles_c;
+    const int band = tile / band_tiles;
+    const int first = band * kRaster;
+    const int band_rows = min(kRaster, tiles_r - first);
+    const int within = tile - band * band_tiles;
+    rb = first + within % band_rows;
+    cb = within / band_rows;
+}
+
+template <int kFormat, int kCols>
+__global__ void __launch_bounds__(kOneCtaThreads, 1)
+mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant__ McTensorMap map_cols, const Fp4GemmParams p) {
+    using Tile = Fp4Tile<kFormat, kCols>;
+    constexpr int stages = Tile::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    const unsigned tiles_base = (mc_smem_addr(smem_raw) + 1023u) & ~1023u;
+    const unsigned bars = tiles_base + stages * Tile::kStageBytes;
+    const unsigned bar_full = bars, bar_empty = bars + 8 * stages, bar_acc_full = bars + 16 * stages, bar_acc_empty = bar_acc_full + 16;
+    __shared__ unsigned tmem_slot;
+    __shared__ int abort_storage;
+    volatile int* abort_flag = &abort_storage;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tiles_r = (p.rows + kTileRows - 1) / kTileRows;
+    const int tiles_c = (p.cols + kCols - 1) / kCols;
+    const int items = tiles_r * tiles_c * p.splits;
+
+    if (threadIdx.x == 0) {
+        abort_storage = 0;
+        for (int s = 0; s < stages; ++s) {
+            mc_mbar_init(bar_full + 8 * s, 1);
+            mc_mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mc_mbar_init(bar_acc_full + 8 * a, 1);
+            mc_mbar_init(bar_acc_empty + 8 * a, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mc_smem_addr(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = tmem_slot;
+    // A programmatic dependent of the launch before it: global memory is touched only once that launch is complete.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0, issued = 0;
+            unsigned phase = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+                int rb, cb, split;
+                fp4_decode_item(item, tiles_r, tiles_c, p.splits, rb, cb, split);
+                const int kb_begin = split * p.k_blocks_per_split;
+                const int kb_end = min(p.k_blocks, kb_begin + p.k_blocks_per_split);
+                const unsigned char* row_scales = p.row_scales + rb * p.k_tiles * kFp4TileBytes;
+                const unsigned char* col_scales = p.col_scales + (cb * kCols >> 7) * p.k_tiles * kFp4TileBytes;
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
+                    ok = mc_mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, MC_FP4_ERR_PRODUCER);
+                    if (!ok) break;
+                    const unsigned full = bar_full + 8 * stage;
+                    const unsigned rows_dst = tiles_base + stage * Tile::kStageBytes;
+                    const unsigned cols_dst = rows_dst + Tile::kRowBytes;
+                    const unsigned scales_dst = cols_dst + Tile::kColBytes;
+                    const int kt = kb * Tile::kScaleTiles;
+                    const unsigned scale_bytes = static_cast<unsigned>(min(static_cast<long long>(Tile::kScaleTiles), p.k_tiles - kt)) * kFp4TileBytes;
+                    mc_mbar_expect_tx(full, Tile::kRowBytes + Tile::kColBytes + 2 * scale_bytes);
+                    mc_tma_load_2d(rows_dst, &map_rows, full, kb * 128, rb * kTileRows);
+                    mc_tma_load_2d(cols_dst, &map_cols, full, kb * 128, cb * kCols);
+                    fp4_bulk_load(scales_dst, row_scales + static_cast<long long>(kt) * kFp4TileBytes, scale_bytes, full);
+                    fp4_bulk_load(scales_dst + Tile::kScaleBytes, col_scales + static_cast<long long>(kt) * kFp4TileBytes, scale_bytes, full);
+                    ++issued;
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                // copies in flight land before shared memory is given up
+                const int pending = min(issued, stages);
+                for (int i = 0; i < pending; ++i) {
+                    if (stage == 0) {
+                        stage = stages;
+                        phase ^= 1u;
+                    }
+                    --stage;
+                    const unsigned long long t0 = mc_globaltimer();
+                    while (!mc_mbar_try_wait(bar_full + 8 * stage, phase)) {
+                        if (mc_globaltimer() - t0 > MC_WAIT_NS / 4) {
+                            if (p.status != nullptr) atomicOr(p.status, MC_FP4_ERR_DRAIN);
+                            break;
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr unsigned idesc = fp4_instruction<kFormat>(kTileRows, kCols);
+            int stage = 0, acc = 0;
+            unsigned phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+                int rb, cb, split;
+                fp4_decode_item(item, tiles_r, tiles_c, p.splits, rb, cb, split);
+                const int kb_begin = split * p.k_blocks_per_split;
+                const int kb_end = min(p.k_blocks, kb_begin + p.k_blocks_per_split);
+                ok = mc_mbar_wait(bar_acc_empty + 8 * acc, acc_phase ^ 1u, abort_flag, p.status, MC_FP4_ERR_MMA);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned tmem_d = tmem + static_cast<unsigned>(acc * Tile::kAccColumns);
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
+                    ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned rows_src = tiles_base + stage * Tile::kStageBytes;
+                    const unsigned cols_src = rows_src + Tile::kRowBytes;
+                    const unsigned scales_src = cols_src + Tile::kColBytes;
+                    const unsigned scale_r = tmem + Tile::kScaleBase + static_cast<unsigned>(stage * 2 * Tile::kScaleColumns);
+                    const unsigned scale_c = scale_r + Tile::kScaleColumns;
+                    const int left = p.k - kb * kFp4BlockK;
+                    // Behind the last column there are no scale tiles: those instructions are left out (the codes there are
+                    // 0, but what lies in the scales' place could be a NaN).
+                    const int steps = min(kFp4BlockK / kFp4MmaK, (left + kFp4MmaK - 1) / kFp4MmaK);
+#pragma unroll
+                    for (int t = 0; t < Tile::kScaleTiles; ++t) {
+                        if (t * (kFp4BlockK / kFp4MmaK / Tile::kScaleTiles) < steps) {
+                            fp4_scales_to_tmem<1>(scale_r + 4 * t, fp4_scale_desc(scales_src + t * kFp4TileBytes));
+                            fp4_scales_to_tmem<1>(scale_c + 4 * t, fp4_scale_desc(scales_src + Tile::kScaleBytes + t * kFp4TileBytes));
+                        }
+                    }
+                    const unsigned long long desc_r = fp4_tile_desc(rows_src);
+                    const unsigned long long desc_c = fp4_tile_desc(cols_src);
+#pragma unroll
+                    for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
+                        if (ks < steps) {
+                            const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
+                            const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
+                            fp4_mma<kFormat, 1>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 4 * t,
+                                                (kb > kb_begin || ks > 0) ? 1u : 0u);
+                        }
+                    }
+                    fp4_commit(bar_empty + 8 * stage);
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                fp4_commit(bar_acc_full + 8 * acc);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        constexpr int kChunk = 16;
+        const float alpha = product_scale(p.row_scale, p.col_scale);
+        int acc = 0;
+        unsigned acc_phase = 0;
+        bool ok = true;
+        const long long m = p.swapped ? p.cols : p.rows;
+        const long long n = p.swapped ? p.rows : p.cols;
+        for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            int rb, cb, split;
+            fp4_decode_item(item, tiles_r, tiles_c, p.splits, rb, cb, split);
+            ok = mc_mbar_wait(bar_acc_full + 8 * acc, acc_phase, abort_flag, p.status, MC_FP4_ERR_EPILOGUE);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int row = rb * kTileRows + quarter * 32 + lane;
+            const bool partial = p.splits > 1;
+            void* dst = partial ? static_cast<void*>(p.workspace + split * m * n) : p.c;
+            const long long ld = partial ? n : p.ldc;
+            const int type = partial ? MCD_TYPE_F32 : p.c_type;
+            const float scale = partial ? 1.0f : alpha;
+            for (int chunk = 0; chunk < kCols / kChunk; ++chunk) {
+                const int col0 = cb * kCols + chunk * kChunk;
+                if (col0 >= p.cols) break;
+                unsigned v[kChunk];
+                tmem_load16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + static_cast<unsigned>(acc * Tile::kAccColumns + chunk * kChunk), v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (row < p.rows) {
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        if (col0 + j < p.cols) {
+                            const long long at = p.swapped ? static_cast<long long>(col0 + j) * ld + row : static_cast<long long>(row) * ld + col0 + j;
+                            store_c(dst, type, at, __uint_as_float(v[j]) * scale);
+                        }
+                    }
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mc_mbar_arrive(bar_acc_empty + 8 * acc);
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1u;
+        }
+    }
+
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// The K slices of every element in slice order, times the tensor scales.
+__global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ parts, int splits, long long m, long long n, const float* scale_a,
+                                                   const float* scale_b, void* c, int c_type, long long ldc) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float alpha = product_scale(scale_a, scale_b);
+    const long long count = m * n;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * 256) {
+        float sum = parts[i];
+        for (int z = 1; z < splits; ++z) sum += parts[z * count + i];
+        const long long r = i / n;
+        store_c(c, c_type, r * ldc + (i - r * n), sum * alpha);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+
+struct Plan {
+    bool swapped = false;
+    int tile_cols = 128;
+    int splits = 1;
+    int k_blocks = 1;
+    int per_split = 1;
+};
+
+Plan plan_for(long long m, long long n, long long k) {
+    Plan plan;
+    plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
+    plan.swapped = m <= 128;
+    const long long rows = plan.swapped ? n : m;
+    const long long cols = plan.swapped ? m : n;
+    plan.tile_cols = !plan.swapped ? 128 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    const long long tiles = ((rows + 127) / 128) * ((cols + plan.tile_cols - 1) / plan.tile_cols);
+    const int sms = 148;
+    int splits = 1;
+    if (tiles * 2 <= sms) splits = static_cast<int>(std::max<long long>(1, std::min<long long>(sms / tiles, plan.k_blocks / 4)));
+    plan.per_split = (plan.k_blocks + splits - 1) / splits;
+    plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
+    return plan;
+}
+
+int encode_codes(McTensorMap* map, const mcd_fp4_tensor& t, unsigned box_rows) {
+    static_assert(sizeof(McTensorMap) == sizeof(CUtensorMap), "tensor map size");
+    const DriverApi* drv = driver_api();
+    if (drv == nullptr) return fail("the CUDA driver API is unavailable");
+    const auto pitch = static_cast<cuuint64_t>(mcd_fp4_code_pitch(t.cols));
+    const cuuint64_t dims[2] = {pitch, static_cast<cuuint64_t>(t.rows)};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t elem_strides[2] = {1, 1};
+    return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.codes, dims, strides,
+                                               box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled");
+}
+
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, Args... args) {
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid, 1, 1);
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return check_rt(cudaLaunchKernelEx(&config, kernel, args...), what);
+}
+
+template <int kFormat, int kCols>
+int launch_one_cta(const McTensorMap& rows, const McTensorMap& cols, const Fp4GemmParams& p, unsigned grid, cudaStream_t s) {
+    using Tile = Fp4Tile<kFormat, kCols>;
+    static_assert(Tile::kSmem + 64 <= 227 * 1024, "shared memory");
+    static PerDeviceOnce configured;
+    int device = 0;
+    if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+    if (configured.first_use(device)) {
+        if (int rc = check_rt(cudaFuncSetAttribute(mc_fp4_gemm<kFormat, kCols>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem),
+                              "cudaFuncSetAttribute(max dynamic shared memory)")) {
+            configured.forget(device);
+            return rc;
+        }
+    }
+    return launch_dependent(mc_fp4_gemm<kFormat, kCols>, grid, kOneCtaThreads, Tile::kSmem, s, "mc_fp4_gemm", rows, cols, p);
+}
+
+template <int kFormat>
+int launch_format(int tile_cols, const McTensorMap& rows, const McTensorMap& cols, const Fp4GemmParams& p, unsigned grid, cudaStream_t s) {
+    switch (tile_cols) {
+        case 16: return launch_one_cta<kFormat, 16>(rows, cols, p, grid, s);
+        case 32: return launch_one_cta<kFormat, 32>(rows, cols, p, grid, s);
+        case 64: return launch_one_cta<kFormat, 64>(rows, cols, p, grid, s);
+        default: return launch_one_cta<kFormat, 128>(rows, cols, p, grid, s);
+    }
+}
+
+size_t plan_workspace(const Plan& plan, long long m, long long n) {
+    return plan.splits > 1 ? static_cast<size_t>(plan.splits) * static_cast<size_t>(m) * static_cast<size_t>(n) * sizeof(float) : 0;
+}
+
+bool sized(const mcd_fp4_gemm_args* a) { return a != nullptr && a->a.rows > 0 && a->b.rows > 0 && a->a.cols > 0; }
+
+}  // namespace
+
+extern "C" size_t mcd_fp4_gemm_workspace(const mcd_fp4_gemm_args* args) {
+    if (!sized(args)) return 0;
+    return plan_workspace(plan_for(args->a.rows, args->b.rows, args->a.cols), args->a.rows, args->b.rows);
+}
+
+extern "C" int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args) {
+    if (!sized(args)) return 0;
+    return plan_for(args->a.rows, args->b.rows, args->a.cols).splits > 1 ? 2 : 1;
+}
+
+extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
+    const char* who = "mcd_fp4_gemm";
+    if (args == nullptr) return fail("mcd_fp4_gemm: null arguments");
+    if (int rc = check_fp4(who, &args->a)) return rc;
+    if (int rc = check_fp4(who, &args->b)) return rc;
+    if (args->a.batch != 1 || args->b.batch != 1) return fail("mcd_fp4_gemm: operands are single matrices (batch 1)");
+    if (args->a.format != args->b.format) return fail("mcd_fp4_gemm: the operands' formats differ");
+    if (args->a.cols != args->b.cols) return fail("mcd_fp4_gemm: the operands' columns (k) differ");
+    const int type = args->c_type;
+    if (type != MCD_TYPE_F32 && type != MCD_HALF_BF16 && type != MCD_HALF_F16) return fail("mcd_fp4_gemm: unknown type of c");
+    if (args->c == nullptr) return fail("mcd_fp4_gemm: no output buffer");
+    if (!is_aligned(args->c, type == MCD_TYPE_F32 ? 4 : 2)) return fail("mcd_fp4_gemm: c is not aligned to its type");
+    const long long m = args->a.rows, n = args->b.rows, k = args->a.cols;
+    if (args->ldc < n) return fail("mcd_fp4_gemm: ldc is less than a row of c");
+    if (!fits(1, m, args->ldc, 1LL << 46)) return fail("mcd_fp4_gemm: c is too large");
+    if (!is_aligned(args->status, 4)) return fail("mcd_fp4_gemm: unaligned status word");
+    const Plan plan = plan_for(m, n, k);
+    const long long rows = plan.swapped ? n : m, cols = plan.swapped ? m : n;
+    const long long items = ((rows + 127) / 128) * ((cols + plan.tile_cols - 1) / plan.tile_cols) * plan.splits;
+    if (items > 2000000000LL) return fail("mcd_fp4_gemm: too many tiles");
+    const size_t need = plan_workspace(plan, m, n);
+    if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) {
+        return fail("mcd_fp4_gemm: this problem needs " + std::to_string(need) + " bytes of workspace");
+    }
+    if (need > 0 && !is_aligned(args->workspace, 16)) return fail("mcd_fp4_gemm: the workspace needs 16-byte alignment");
+    if (int rc = check_device_pointers(who, {args->a.codes, args->a.scales, args->a.tensor_scale, args->b.codes, args->b.scales, args->b.tensor_scale,
+                                             args->c, need > 0 ? args->workspace : nullptr, args->status})) {
+        return rc;
+    }
+    const mcd_fp4_tensor& on_rows = plan.swapped ? args->b : args->a;
+    const mcd_fp4_tensor& on_cols = plan.swapped ? args->a : args->b;
+    McTensorMap map_rows, map_cols;
+    if (int rc = encode_codes(&map_rows, on_rows, kTileRows)) return rc;
+    if (int rc = encode_codes(&map_cols, on_cols, static_cast<unsigned>(plan.tile_cols))) return rc;
+    Fp4GemmParams p;
+    p.row_scales = static_cast<const unsigned char*>(on_rows.scales);
+    p.col_scales = static_cast<const unsigned char*>(on_cols.scales);
+    p.k_tiles = fp4_geometry(args->a.format, 1, k).k_tiles;
+    p.row_scale = on_rows.tensor_scale;
+    p.col_scale = on_cols.tensor_scale;
+    p.c = args->c;
+    p.workspace = static_cast<float*>(args->workspace);
+    p.status = args->status;
+    p.ldc = args->ldc;
+    p.c_type = type;
+    p.rows = static_cast<int>(rows);
+    p.cols = static_cast<int>(cols);
+    p.k = static_cast<int>(k);
+    p.k_blocks = plan.k_blocks;
+    p.k_blocks_per_split = plan.per_split;
+    p.splits = plan.splits;
+    p.swapped = plan.swapped ? 1 : 0;
+    auto s = static_cast<cudaStream_t>(stream);
+    const auto grid = static_cast<unsigned>(std::min<long long>(items, sm_count()));
+    if (int rc = args->a.format == MCD_FP4_E8M0_32 ? launch_format<MCD_FP4_E8M0_32>(plan.tile_cols, map_rows, map_cols, p, grid, s)
+                                                   : launch_format<MCD_FP4_E4M3_16>(plan.tile_cols, map_rows, map_cols, p, grid, s)) {
+        return rc;
+    }
+    if (plan.splits == 1) return 0;
+    const long long blocks = std::max<long long>(1, std::min<long long>((m * n + 255) / 256, 8LL * sm_count()));
+    return launch_dependent(mc_fp4_join, static_cast<unsigned>(blocks), 256, 0, s, "mc_fp4_join", static_cast<const float*>(p.workspace), plan.splits, m, n,
+                            args->a.tensor_scale, args->b.tensor_scale, p.c, p.c_type, p.ldc);
+}
