@@ -343,6 +343,50 @@ MCD_API size_t mcd_fp4_gemm_workspace(const mcd_fp4_gemm_args* args);
 MCD_API int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream);
 MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
 
+/* ------------------------------------------------- mixture of experts, few tokens
+ * A whole layer: for each of 1 .. MCD_MOE_MAX_TOKENS tokens
+ *   l = R x (64-bit sums of the 16-bit products), p = softmax(l) over all experts,
+ *   the top_k experts by l, ties and NaN to the lowest index (a NaN counts as lower than every number),
+ *   w_j = p of the j-th one (renormalize != 0: divided by their sum),
+ *   y = sum_j w_j * D_j (silu(G_j x) * (U_j x)),   silu(v) = v / (1 + exp(-v)).
+ *  type       MCD_HALF_*: x, router and y
+ *  x          [tokens, d], ldx elements from row to row
+ *  router     [experts, d], ld_router
+ *  gate_up    batch = experts, rows = 2f: f rows of G, then f rows of U; cols = d
+ *  down       batch = experts, rows = d, cols = f, same format
+ *  y          [tokens, d], ldy; only these elements are written
+ *  chosen     [tokens, top_k] int32, best first, and weights [tokens, top_k] f32: device, either may be NULL
+ *  workspace  mcd_moe_workspace(...) bytes, 16-byte aligned; calls that may run at the same time need one each
+ * The products accumulate in f32. x and silu(..) * (..) enter them with 11 significant bits after a power of two per token,
+ * or per token and expert, that takes their largest magnitude below 2^15: nothing of a bf16 or f16 x is lost above 2^-29 of
+ * the token's largest value. The experts' results are added in an order that the routing alone fixes: results do not
+ * depend on scheduling. No wait, no status word; three launches. */
+#define MCD_MOE_MAX_TOKENS 64
+#define MCD_MOE_MAX_EXPERTS 512
+#define MCD_MOE_MAX_TOP_K 16
+
+typedef struct mcd_moe_args {
+    int type;
+    int tokens;
+    int top_k;
+    int renormalize;
+    const void* x;
+    long long ldx;
+    const void* router;
+    long long ld_router;
+    mcd_fp4_tensor gate_up;
+    mcd_fp4_tensor down;
+    void* y;
+    long long ldy;
+    int* chosen;
+    float* weights;
+    void* workspace;
+    size_t workspace_bytes;
+} mcd_moe_args;
+
+MCD_API size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f);
+MCD_API int mcd_moe_layer(const mcd_moe_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,7 @@ from .fp4 import (  # noqa: F401
     fp4_sizes,
     fp4_tensor_scale,
 )
+from .moe import MoeLayer, moe_workspace_bytes  # noqa: F401
 
 __all__ = [
     "Communicator",
@@ -41,6 +42,7 @@ __all__ = [
     "Fp4Matrix",
     "HostGraph",
     "McError",
+    "MoeLayer",
     "compile_graph",
     "fp4_dequantize",
     "fp4_gemm_workspace_bytes",
@@ -49,6 +51,7 @@ __all__ = [
     "fp4_tensor_scale",
     "graph_path",
     "lib",
+    "moe_workspace_bytes",
     "resolve_matmul_kernel",
     "shard_dims",
     "split_k_splits",

@@ -123,6 +123,8 @@ def lib() -> C.CDLL:
         "mcd_fp4_gemm_workspace": (C.c_size_t, [vp]),
         "mcd_fp4_gemm": (i32, [vp, vp]),
         "mcd_fp4_gemm_launches": (i32, [vp]),
+        "mcd_moe_workspace": (C.c_size_t, [i32, i32, i32, i64, i64]),
+        "mcd_moe_layer": (i32, [vp, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

@@ -46,7 +46,7 @@ HOST_SOURCES = [
     "device/nccl_layer.cpp",
     "capi/capi.cpp",
 ]
-CUDA_SOURCES = ["kernels/gemm_launch.cu", "kernels/no_alloc.cu", "kernels/fp4_quantize.cu", "kernels/fp4_gemm.cu"]
+CUDA_SOURCES = ["kernels/gemm_launch.cu", "kernels/no_alloc.cu", "kernels/fp4_quantize.cu", "kernels/fp4_gemm.cu", "kernels/moe_layer.cu"]
 EMBEDDED = {
     "kSourceEpilogue": "kernels/epilogue.cuh",
     "kSourceAsyncCopy": "kernels/async_copy.cuh",
