@@ -293,7 +293,7 @@ MCD_API int mcd_gemm_f32_split_no_alloc(const float* a, const float* b, float* c
 typedef struct mcd_fp4_tensor {
     int format;       /* MCD_FP4_* */
     int batch;        /* matrices, 1 for a single one */
-    long long rows;   /* of one matrix, at most 2^31 - 1 */
+    long long rows;   /* of one matrix, at most 2^31 - 256 */
     long long cols;
     void* codes;      /* device, 16-byte aligned */
     void* scales;     /* device, 16-byte aligned */

@@ -323,6 +323,319 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
     }
 }
 
+// --------------------------------------------------------------------------------------------- an SM pair per tile
+//
+// A cluster of two CTAs owns 256 x 256 of C: each stages its own 128 rows of A, its own 128 of the 256 rows of B, the
+// scales of its rows of A and of all 256 rows of B; the leader's cta_group::2 instructions read both CTAs' shared memory
+// and leave each CTA's 128 rows in its TMEM.
+//
+// TMEM: two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap. The second
+// one begins kOverlap columns before the first one ends, which leaves kOverlap columns for two K blocks' scales (24 columns
+// each for E8M0_32, 48 for E4M3_16). The epilogue takes the shared columns of a tile into registers first and gives them
+// back before it does anything else, so the multiplies of the next tile wait for a few TMEM reads only.
+// A K block's scales go to the half of that space whose last user, the K block two before, has been committed.
+
+template <int kFormat>
+struct Fp4Pair {
+    static constexpr int kScaleTiles = kFormat == MCD_FP4_E8M0_32 ? 2 : 4;
+    static constexpr int kRowBytes = 128 * 128;
+    static constexpr int kColBytes = 128 * 128;
+    static constexpr int kRowScaleBytes = kScaleTiles * kFp4TileBytes;
+    static constexpr int kColScaleBytes = 2 * kRowScaleBytes;
+    static constexpr int kStageBytes = kRowBytes + kColBytes + kRowScaleBytes + kColScaleBytes;
+    static constexpr int kStages = 5;
+    static constexpr int kStagingPerWarp = 4096;
+    static constexpr int kBarrierBytes = 1024;
+    static constexpr int kSmem = kStages * kStageBytes + 1024 + kBarrierBytes + 8 * kStagingPerWarp;
+    static constexpr int kOverlapChunks = kFormat == MCD_FP4_E8M0_32 ? 2 : 3;  // of 32 columns
+    static constexpr int kOverlap = 32 * kOverlapChunks;
+    static constexpr int kScaleBase = 512 - kOverlap;
+    static constexpr int kRowScaleColumns = kScaleTiles * 4;
+    static constexpr int kScaleColumns = 3 * kRowScaleColumns;  // rows, then columns: 8 per scale tile
+    static_assert(2 * kScaleColumns <= kOverlap, "TMEM columns");
+};
+
+constexpr int kPairThreads = 64 + 8 * 32;
+constexpr int kPairTile = 256;
+
+struct Fp4PairParams {
+    const float* row_scale;
+    const float* col_scale;
+    void* c;
+    unsigned* status;
+    long long ldc;
+    int c_type;
+    int m, n, k, k_blocks;
+    int by_tma;  // C leaves as TMA boxes; otherwise (alignment) straight from registers
+};
+
+template <int kFormat>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_constant__ McTensorMap map_cols,
+                 const __grid_constant__ McTensorMap map_row_scales, const __grid_constant__ McTensorMap map_col_scales,
+                 const __grid_constant__ McTensorMap map_c, const Fp4PairParams p) {
+    using Pair = Fp4Pair<kFormat>;
+    constexpr int stages = Pair::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    const unsigned tiles_base = (mc_smem_addr(smem_raw) + 1023u) & ~1023u;
+    const unsigned staging = tiles_base + stages * Pair::kStageBytes;
+    const unsigned bars = staging + 8 * Pair::kStagingPerWarp;
+    // full: the leader's, counts both CTAs' bytes. empty: one in each CTA. acc_full: one in each; acc_empty: the leader's.
+    const unsigned bar_full = bars, bar_empty = bars + 8 * stages, bar_acc_full = bars + 16 * stages, bar_acc_empty = bar_acc_full + 8;
+    __shared__ unsigned tmem_slot;
+    __shared__ int abort_storage;
+    volatile int* abort_flag = &abort_storage;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    unsigned rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const bool leader = rank == 0;
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tiles_r = (p.m + kPairTile - 1) / kPairTile;
+    const int tiles_c = (p.n + kPairTile - 1) / kPairTile;
+    const int items = tiles_r * tiles_c;
+
+    if (threadIdx.x == 0) {
+        abort_storage = 0;
+        for (int s = 0; s < stages; ++s) {
+            mc_mbar_init(bar_full + 8 * s, 1);
+            mc_mbar_init(bar_empty + 8 * s, 1);
+        }
+        mc_mbar_init(bar_acc_full, 1);
+        mc_mbar_init(bar_acc_empty, 16);  // the epilogue warps of both CTAs
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mc_smem_addr(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0, issued = 0;
+            unsigned phase = 0;
+            bool ok = true;
+            for (int item = cluster; ok && item < items; item += clusters) {
+                int rb, cb, split;
+                fp4_decode_item(item, tiles_r, tiles_c, 1, rb, cb, split);
+                const int row_tile = 2 * rb + static_cast<int>(rank);
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    ok = mc_mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, MC_FP4_ERR_PRODUCER);
+                    if (!ok) break;
+                    const unsigned full = cluster_address(bar_full + 8 * stage, 0);
+                    const unsigned rows_dst = tiles_base + stage * Pair::kStageBytes;
+                    const unsigned cols_dst = rows_dst + Pair::kRowBytes;
+                    const unsigned row_scales_dst = cols_dst + Pair::kColBytes;
+                    const unsigned col_scales_dst = row_scales_dst + Pair::kRowScaleBytes;
+                    // Boxes count whole, what lies outside their tensor arrives as zeros: scales behind the last column too.
+                    if (leader) mc_mbar_expect_tx(bar_full + 8 * stage, 2 * Pair::kStageBytes);
+                    tma_load_2d_pair(rows_dst, &map_rows, full, kb * 128, row_tile * 128);
+                    tma_load_2d_pair(cols_dst, &map_cols, full, kb * 128, cb * kPairTile + static_cast<int>(rank) * 128);
+                    tma_load_3d_pair(row_scales_dst, &map_row_scales, full, 0, kb * Pair::kScaleTiles, row_tile);
+                    tma_load_3d_pair(col_scales_dst, &map_col_scales, full, 0, kb * Pair::kScaleTiles, 2 * cb);
+                    ++issued;
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok && leader) {
+                const int pending = min(issued, stages);
+                for (int i = 0; i < pending; ++i) {
+                    if (stage == 0) {
+                        stage = stages;
+                        phase ^= 1u;
+                    }
+                    --stage;
+                    const unsigned long long t0 = mc_globaltimer();
+                    while (!mc_mbar_try_wait(bar_full + 8 * stage, phase)) {
+                        if (mc_globaltimer() - t0 > MC_WAIT_NS / 4) {
+                            if (p.status != nullptr) atomicOr(p.status, MC_FP4_ERR_DRAIN);
+                            break;
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr unsigned idesc = fp4_instruction<kFormat>(kPairTile, kPairTile);
+            int stage = 0, acc = 0;
+            unsigned phase = 0;
+            int done_stage = 0;         // the K block two before the one at work
+            unsigned done_phase = 0;
+            int blocks = 0;
+            unsigned empty_phase = 1;  // the first tile waits for nothing
+            bool ok = true;
+            for (int item = cluster; ok && item < items; item += clusters) {
+                ok = mc_mbar_wait(bar_acc_empty, empty_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                if (!ok) break;
+                empty_phase ^= 1u;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned tmem_d = tmem + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    if (blocks >= 2) {
+                        ok = mc_mbar_wait(bar_empty + 8 * done_stage, done_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                        if (!ok) break;
+                        if (++done_stage == stages) {
+                            done_stage = 0;
+                            done_phase ^= 1u;
+                        }
+                    }
+                    ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned rows_src = tiles_base + stage * Pair::kStageBytes;
+                    const unsigned cols_src = rows_src + Pair::kRowBytes;
+                    const unsigned row_scales_src = cols_src + Pair::kColBytes;
+                    const unsigned col_scales_src = row_scales_src + Pair::kRowScaleBytes;
+                    const unsigned scale_r = tmem + Pair::kScaleBase + static_cast<unsigned>((blocks & 1) * Pair::kScaleColumns);
+                    const unsigned scale_c = scale_r + Pair::kRowScaleColumns;
+#pragma unroll
+                    for (int t = 0; t < Pair::kScaleTiles; ++t) {
+                        fp4_scales_to_tmem<2>(scale_r + 4 * t, fp4_scale_desc(row_scales_src + t * kFp4TileBytes));
+                        fp4_scales_to_tmem<2>(scale_c + 8 * t, fp4_scale_desc(col_scales_src + t * kFp4TileBytes));
+                        fp4_scales_to_tmem<2>(scale_c + 8 * t + 4, fp4_scale_desc(col_scales_src + (Pair::kScaleTiles + t) * kFp4TileBytes));
+                    }
+                    const unsigned long long desc_r = fp4_tile_desc(rows_src);
+                    const unsigned long long desc_c = fp4_tile_desc(cols_src);
+#pragma unroll
+                    for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
+                        const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
+                        const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
+                        fp4_mma<kFormat, 2>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 8 * t,
+                                            (kb > 0 || ks > 0) ? 1u : 0u);
+                    }
+                    fp4_commit_pair(bar_empty + 8 * stage);
+                    ++blocks;
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                fp4_commit_pair(bar_acc_full);
+                acc ^= 1;
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        const int half = (warp - 2) >> 2;
+        const unsigned buffer = staging + static_cast<unsigned>(warp - 2) * Pair::kStagingPerWarp;
+        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const unsigned acc_empty = cluster_address(bar_acc_empty, 0);
+        int acc = 0;
+        unsigned full_phase = 0, turn = 0;
+        bool ok = true;
+        for (int item = cluster; ok && item < items; item += clusters) {
+            int rb, cb, split;
+            fp4_decode_item(item, tiles_r, tiles_c, 1, rb, cb, split);
+            ok = mc_mbar_wait(bar_acc_full, full_phase, abort_flag, p.status, MC_FP4_ERR_EPILOGUE);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            full_phase ^= 1u;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16) + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
+            const int row0 = rb * kPairTile + static_cast<int>(rank) * 128 + quarter * 32;
+            const int row = row0 + lane;
+            // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
+            // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
+            auto chunk_at = [&](int i) { return acc ? i : 7 - i; };
+            auto finish = [&](unsigned* v, int chunk) {
+                const int col0 = cb * kPairTile + chunk * 32;
+                if (col0 >= p.n) return;  // warp-uniform
+                float f[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
+                // A box that reaches over the last column is not left to TMA, which cuts rows off at 16 bytes: what lies behind
+                // C's columns inside ldc is not ours.
+                if (p.by_tma && col0 + 32 <= p.n) {
+                    // 32 x 32 boxes through this warp's staging buffer: rows of 128 bytes (f32, 128-byte swizzle) or of 64
+                    // (16 bits, 64-byte swizzle; two boxes take turns in the buffer's halves)
+                    if (p.c_type == MCD_TYPE_F32) {
+                        if (lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)), "f"(f[4 * j]),
+                                         "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3])
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&map_c, buffer, col0, row0);
+                    } else {
+                        const unsigned at = buffer + (turn & 1u) * 2048u;
+                        ++turn;
+                        if (lane == 0) tma_store_wait_read<1>();
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                                         "r"(pack_half2(f[8 * j], f[8 * j + 1], p.c_type)), "r"(pack_half2(f[8 * j + 2], f[8 * j + 3], p.c_type)),
+                                         "r"(pack_half2(f[8 * j + 4], f[8 * j + 5], p.c_type)), "r"(pack_half2(f[8 * j + 6], f[8 * j + 7], p.c_type))
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
+                    }
+                } else if (row < p.m) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (col0 + j < p.n) store_c(p.c, p.c_type, static_cast<long long>(row) * p.ldc + col0 + j, f[j]);
+                    }
+                }
+            };
+            constexpr int kFirst = (Pair::kOverlapChunks + 1) / 2;  // shared chunks of the warps with half == 0
+            unsigned v[kFirst][32];
+#pragma unroll
+            for (int i = 0; i < kFirst; ++i) {
+                if (2 * i + half < Pair::kOverlapChunks) tmem_load32(lanes + static_cast<unsigned>(chunk_at(2 * i + half) * 32), v[i]);
+            }
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int order = 2 * i + half;
+                if (i < kFirst && order < Pair::kOverlapChunks) {
+                    finish(v[i < kFirst ? i : 0], chunk_at(order));
+                } else {
+                    unsigned w[32];
+                    tmem_load32(lanes + static_cast<unsigned>(chunk_at(order) * 32), w);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    finish(w, chunk_at(order));
+                }
+            }
+            acc ^= 1;
+        }
+        if (lane == 0) tma_store_wait_read<0>();
+    }
+
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    // neither CTA gives up its shared memory or TMEM while the other may still use it
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 // The K slices of every element in slice order, times the tensor scales.
 __global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ parts, int splits, long long m, long long n, const float* scale_a,
                                                    const float* scale_b, void* c, int c_type, long long ldc) {
@@ -340,6 +653,7 @@ __global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ par
 // ---------------------------------------------------------------------------------------------------------- host side
 
 struct Plan {
+    bool pairs = false;  // 256 x 256 tiles on SM pairs; the rest describes the one-CTA kernel
     bool swapped = false;
     int tile_cols = 128;
     int splits = 1;
@@ -350,6 +664,9 @@ struct Plan {
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
+    plan.per_split = plan.k_blocks;
+    plan.pairs = ((m + 255) / 256) * ((n + 255) / 256) >= 37;
+    if (plan.pairs) return plan;
     plan.swapped = m <= 128;
     const long long rows = plan.swapped ? n : m;
     const long long cols = plan.swapped ? m : n;
@@ -375,6 +692,37 @@ int encode_codes(McTensorMap* map, const mcd_fp4_tensor& t, unsigned box_rows) {
     return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.codes, dims, strides,
                                                box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled");
+}
+
+// Scales as a tensor of 512-byte tiles [row tiles, k tiles]; a box takes `k_tiles` tiles of `row_tiles` rows of them.
+int encode_scales(McTensorMap* map, const mcd_fp4_tensor& t, unsigned box_k_tiles, unsigned box_row_tiles) {
+    const DriverApi* drv = driver_api();
+    if (drv == nullptr) return fail("the CUDA driver API is unavailable");
+    const Fp4Geometry geo = fp4_geometry(t.format, t.rows, t.cols);
+    const cuuint64_t dims[3] = {kFp4TileBytes / 4, static_cast<cuuint64_t>(geo.k_tiles), static_cast<cuuint64_t>(geo.row_tiles)};
+    const cuuint64_t strides[2] = {kFp4TileBytes, static_cast<cuuint64_t>(geo.k_tiles * kFp4TileBytes)};
+    const cuuint32_t box[3] = {kFp4TileBytes / 4, box_k_tiles, box_row_tiles};
+    const cuuint32_t elem_strides[3] = {1, 1, 1};
+    return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, t.scales, dims, strides,
+                                               box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled");
+}
+
+// C in boxes of 32 x 32.
+int encode_c(McTensorMap* map, void* c, int type, long long m, long long n, long long ldc) {
+    const DriverApi* drv = driver_api();
+    if (drv == nullptr) return fail("the CUDA driver API is unavailable");
+    const bool f32 = type == MCD_TYPE_F32;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(m)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc) * (f32 ? 4 : 2)};
+    const cuuint32_t box[2] = {32, 32};
+    const cuuint32_t elem_strides[2] = {1, 1};
+    return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                                               2, c, dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                               f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
                      "cuTensorMapEncodeTiled");
 }
 
@@ -419,6 +767,45 @@ int launch_format(int tile_cols, const McTensorMap& rows, const McTensorMap& col
         case 64: return launch_one_cta<kFormat, 64>(rows, cols, p, grid, s);
         default: return launch_one_cta<kFormat, 128>(rows, cols, p, grid, s);
     }
+}
+
+template <int kFormat>
+int launch_pairs(const mcd_fp4_gemm_args* args, cudaStream_t s) {
+    using Pair = Fp4Pair<kFormat>;
+    static_assert(Pair::kSmem + 64 <= 227 * 1024, "shared memory");
+    static PerDeviceOnce configured;
+    int device = 0;
+    if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+    if (configured.first_use(device)) {
+        if (int rc = check_rt(cudaFuncSetAttribute(mc_fp4_gemm_pair<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, Pair::kSmem),
+                              "cudaFuncSetAttribute(max dynamic shared memory)")) {
+            configured.forget(device);
+            return rc;
+        }
+    }
+    McTensorMap rows, cols, row_scales, col_scales, c = {};
+    if (int rc = encode_codes(&rows, args->a, 128)) return rc;
+    if (int rc = encode_codes(&cols, args->b, 128)) return rc;
+    if (int rc = encode_scales(&row_scales, args->a, Pair::kScaleTiles, 1)) return rc;
+    if (int rc = encode_scales(&col_scales, args->b, Pair::kScaleTiles, 2)) return rc;
+    Fp4PairParams p;
+    p.row_scale = args->a.tensor_scale;
+    p.col_scale = args->b.tensor_scale;
+    p.c = args->c;
+    p.status = args->status;
+    p.ldc = args->ldc;
+    p.c_type = args->c_type;
+    p.m = static_cast<int>(args->a.rows);
+    p.n = static_cast<int>(args->b.rows);
+    p.k = static_cast<int>(args->a.cols);
+    p.k_blocks = (p.k + kFp4BlockK - 1) / kFp4BlockK;
+    p.by_tma = is_aligned(args->c, 16) && args->ldc % (args->c_type == MCD_TYPE_F32 ? 4 : 8) == 0;
+    if (p.by_tma) {
+        if (int rc = encode_c(&c, args->c, args->c_type, p.m, p.n, args->ldc)) return rc;
+    }
+    const long long tiles = ((args->a.rows + kPairTile - 1) / kPairTile) * ((args->b.rows + kPairTile - 1) / kPairTile);
+    const auto grid = 2 * static_cast<unsigned>(std::min<long long>(tiles, sm_count() / 2));
+    return launch_dependent(mc_fp4_gemm_pair<kFormat>, grid, kPairThreads, Pair::kSmem, s, "mc_fp4_gemm_pair", rows, cols, row_scales, col_scales, c, p);
 }
 
 size_t plan_workspace(const Plan& plan, long long m, long long n) {
@@ -467,6 +854,10 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
     if (int rc = check_device_pointers(who, {args->a.codes, args->a.scales, args->a.tensor_scale, args->b.codes, args->b.scales, args->b.tensor_scale,
                                              args->c, need > 0 ? args->workspace : nullptr, args->status})) {
         return rc;
+    }
+    if (plan.pairs) {
+        auto on = static_cast<cudaStream_t>(stream);
+        return args->a.format == MCD_FP4_E8M0_32 ? launch_pairs<MCD_FP4_E8M0_32>(args, on) : launch_pairs<MCD_FP4_E4M3_16>(args, on);
     }
     const mcd_fp4_tensor& on_rows = plan.swapped ? args->b : args->a;
     const mcd_fp4_tensor& on_cols = plan.swapped ? args->a : args->b;

@@ -51,7 +51,7 @@ inline int check_fp4(const char* who, const mcd_fp4_tensor* t) {
     if (t->format != MCD_FP4_E8M0_32 && t->format != MCD_FP4_E4M3_16) return fail(named(who, "unknown 4-bit format"));
     if (t->batch < 1) return fail(named(who, "no matrices"));
     if (t->rows < 1 || t->cols < 1) return fail(named(who, "empty matrix"));
-    if (t->rows > 2147483647LL || t->cols > (1LL << 30) || !fits(t->batch, t->rows, mcd_fp4_code_pitch(t->cols), 1LL << 46)) {
+    if (t->rows > 2147483647LL - 255 || t->cols > (1LL << 30) || !fits(t->batch, t->rows, mcd_fp4_code_pitch(t->cols), 1LL << 46)) {
         return fail(named(who, "matrix too large"));
     }
     if (t->codes == nullptr || t->scales == nullptr) return fail(named(who, "null codes or scales"));

@@ -111,7 +111,7 @@ def _product(mc, a, b, dtype, ldc=None, offset=0, stream=0):
 @pytest.mark.parametrize("m, n, k", [
     (1, 1, 1), (1, 8, 31), (1, 128, 64), (2, 130, 65), (16, 128, 256), (17, 257, 257), (33, 64, 300), (64, 200, 96), (65, 129, 512),
     (128, 128, 128), (128, 300, 1000), (129, 128, 256), (200, 70, 33), (256, 256, 768), (300, 513, 321), (1, 300, 4096), (40, 100, 5000),
-    (513, 256, 1024), (512, 512, 2080), (700, 900, 640),
+    (513, 256, 1024), (512, 512, 2080), (700, 900, 640), (2100, 1300, 700), (1600, 1600, 2304), (10000, 257, 64), (2305, 2304, 1),
 ])
 def test_exact_data_gives_equal_results(mc, ref, fmt, m, n, k):
     rng = np.random.default_rng(m * 7 + n * 3 + k)
@@ -125,7 +125,7 @@ def test_exact_data_gives_equal_results(mc, ref, fmt, m, n, k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
-@pytest.mark.parametrize("m, n, k", [(1, 512, 2048), (5, 130, 777), (100, 256, 1024), (150, 300, 4096), (1024, 640, 512)])
+@pytest.mark.parametrize("m, n, k", [(1, 512, 2048), (5, 130, 777), (100, 256, 1024), (150, 300, 4096), (1024, 640, 512), (1537, 1800, 1500)])
 def test_normal_data_within_the_bound(mc, ref, fmt, dtype, m, n, k):
     rng = np.random.default_rng(k)
     operands, bound = [], []
@@ -149,7 +149,8 @@ def test_normal_data_within_the_bound(mc, ref, fmt, dtype, m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
-@pytest.mark.parametrize("m, n, ldc, offset", [(20, 100, 101, 1), (20, 100, 104, 8), (200, 100, 131, 3), (300, 256, 264, 16), (200, 128, 128, 1)])
+@pytest.mark.parametrize("m, n, ldc, offset", [(20, 100, 101, 1), (20, 100, 104, 8), (200, 100, 131, 3), (300, 256, 264, 16), (200, 128, 128, 1), (2100, 1300, 1301, 1),
+                                               (2100, 1300, 1304, 16), (2100, 1300, 1304, 1)])
 def test_only_c_is_written(mc, ref, dtype, m, n, ldc, offset):
     rng = np.random.default_rng(ldc)
     a, b = _exact_operand(mc, ref, rng, m, 96, "e8m0_32"), _exact_operand(mc, ref, rng, n, 96, "e8m0_32")
