@@ -29,6 +29,7 @@ namespace {
 #define MC_FP4_ERR_MMA 0x200u
 #define MC_FP4_ERR_EPILOGUE 0x400u
 #define MC_FP4_ERR_DRAIN 0x800u
+#define MC_FP4_ERR_SCALES 0x1000u
 
 constexpr int kTileRows = 128;   // TMEM lanes
 constexpr int kRaster = 16;      // row tiles per band of work items
@@ -330,10 +331,14 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
 // and leave each CTA's 128 rows in its TMEM.
 //
 // TMEM: two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap. The second
-// one begins kOverlap columns before the first one ends, which leaves kOverlap columns for two K blocks' scales (24 columns
-// each for E8M0_32, 48 for E4M3_16). The epilogue takes the shared columns of a tile into registers first and gives them
-// back before it does anything else, so the multiplies of the next tile wait for a few TMEM reads only.
-// A K block's scales go to the half of that space whose last user, the K block two before, has been committed.
+// one begins kOverlap columns before the first one ends, which leaves kOverlap columns for the scales of three K blocks (24
+// columns each for E8M0_32, 48 for E4M3_16). The epilogue takes the shared columns of a tile into registers first and gives
+// them back before it does anything else, so the multiplies of the next tile wait for a few TMEM reads only.
+//
+// Scales reach TMEM through registers: four warps of each CTA load them from shared memory and store them to their quarter
+// of the lanes, three K blocks ahead of the multiplies. Brought by tcgen05.cp they would stand in the tensor core's own
+// queue and cost it about 40 cycles per 512 bytes, six or twelve times per K block of 512 cycles (8192^3: 268 us against 202 with E8M0_32, 363 against 218 with E4M3_16).
+// A buffer is written again once the multiplies that read it have been committed.
 
 template <int kFormat>
 struct Fp4Pair {
@@ -343,19 +348,21 @@ struct Fp4Pair {
     static constexpr int kRowScaleBytes = kScaleTiles * kFp4TileBytes;
     static constexpr int kColScaleBytes = 2 * kRowScaleBytes;
     static constexpr int kStageBytes = kRowBytes + kColBytes + kRowScaleBytes + kColScaleBytes;
+    static constexpr int kTileBytes = kRowBytes + kColBytes;
     static constexpr int kStages = 5;
+    static constexpr int kScaleBuffers = 3;  // K blocks whose scales TMEM holds
     static constexpr int kStagingPerWarp = 4096;
     static constexpr int kBarrierBytes = 1024;
     static constexpr int kSmem = kStages * kStageBytes + 1024 + kBarrierBytes + 8 * kStagingPerWarp;
-    static constexpr int kOverlapChunks = kFormat == MCD_FP4_E8M0_32 ? 2 : 3;  // of 32 columns
+    static constexpr int kOverlapChunks = kFormat == MCD_FP4_E8M0_32 ? 3 : 5;  // of 32 columns
     static constexpr int kOverlap = 32 * kOverlapChunks;
     static constexpr int kScaleBase = 512 - kOverlap;
     static constexpr int kRowScaleColumns = kScaleTiles * 4;
     static constexpr int kScaleColumns = 3 * kRowScaleColumns;  // rows, then columns: 8 per scale tile
-    static_assert(2 * kScaleColumns <= kOverlap, "TMEM columns");
+    static_assert(kScaleBuffers * kScaleColumns <= kOverlap, "TMEM columns");
 };
 
-constexpr int kPairThreads = 64 + 8 * 32;
+constexpr int kPairThreads = 64 + 8 * 32 + 4 * 32;
 constexpr int kPairTile = 256;
 
 struct Fp4PairParams {
@@ -380,8 +387,10 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
     const unsigned tiles_base = (mc_smem_addr(smem_raw) + 1023u) & ~1023u;
     const unsigned staging = tiles_base + stages * Pair::kStageBytes;
     const unsigned bars = staging + 8 * Pair::kStagingPerWarp;
-    // full: the leader's, counts both CTAs' bytes. empty: one in each CTA. acc_full: one in each; acc_empty: the leader's.
-    const unsigned bar_full = bars, bar_empty = bars + 8 * stages, bar_acc_full = bars + 16 * stages, bar_acc_empty = bar_acc_full + 8;
+    // full: the leader's, counts both CTAs' tiles. scales: one in each CTA, counts its own. empty: one in each CTA.
+    // ready: the leader's, the scale warps of both CTAs. acc_full: one in each CTA; acc_empty: the leader's.
+    const unsigned bar_full = bars, bar_empty = bars + 8 * stages, bar_scales = bars + 16 * stages, bar_ready = bars + 24 * stages;
+    const unsigned bar_acc_full = bar_ready + 8 * Pair::kScaleBuffers, bar_acc_empty = bar_acc_full + 8;
     __shared__ unsigned tmem_slot;
     __shared__ int abort_storage;
     volatile int* abort_flag = &abort_storage;
@@ -402,7 +411,9 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         for (int s = 0; s < stages; ++s) {
             mc_mbar_init(bar_full + 8 * s, 1);
             mc_mbar_init(bar_empty + 8 * s, 1);
+            mc_mbar_init(bar_scales + 8 * s, 1);
         }
+        for (int b = 0; b < Pair::kScaleBuffers; ++b) mc_mbar_init(bar_ready + 8 * b, 8);
         mc_mbar_init(bar_acc_full, 1);
         mc_mbar_init(bar_acc_empty, 16);  // the epilogue warps of both CTAs
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -437,11 +448,13 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     const unsigned row_scales_dst = cols_dst + Pair::kColBytes;
                     const unsigned col_scales_dst = row_scales_dst + Pair::kRowScaleBytes;
                     // Boxes count whole, what lies outside their tensor arrives as zeros: scales behind the last column too.
-                    if (leader) mc_mbar_expect_tx(bar_full + 8 * stage, 2 * Pair::kStageBytes);
+                    if (leader) mc_mbar_expect_tx(bar_full + 8 * stage, 2 * Pair::kTileBytes);
+                    const unsigned scales = bar_scales + 8 * stage;
+                    mc_mbar_expect_tx(scales, Pair::kRowScaleBytes + Pair::kColScaleBytes);
+                    tma_load_3d(row_scales_dst, &map_row_scales, scales, 0, kb * Pair::kScaleTiles, row_tile);
+                    tma_load_3d(col_scales_dst, &map_col_scales, scales, 0, kb * Pair::kScaleTiles, 2 * cb);
                     tma_load_2d_pair(rows_dst, &map_rows, full, kb * 128, row_tile * 128);
                     tma_load_2d_pair(cols_dst, &map_cols, full, kb * 128, cb * kPairTile + static_cast<int>(rank) * 128);
-                    tma_load_3d_pair(row_scales_dst, &map_row_scales, full, 0, kb * Pair::kScaleTiles, row_tile);
-                    tma_load_3d_pair(col_scales_dst, &map_col_scales, full, 0, kb * Pair::kScaleTiles, 2 * cb);
                     ++issued;
                     if (++stage == stages) {
                         stage = 0;
@@ -449,7 +462,9 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     }
                 }
             }
-            if (!ok && leader) {
+            if (!ok) {
+                // The copies in flight land before shared memory is given up: each CTA sees its own scales, the leader the
+                // tiles of both.
                 const int pending = min(issued, stages);
                 for (int i = 0; i < pending; ++i) {
                     if (stage == 0) {
@@ -458,7 +473,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     }
                     --stage;
                     const unsigned long long t0 = mc_globaltimer();
-                    while (!mc_mbar_try_wait(bar_full + 8 * stage, phase)) {
+                    while (!mc_mbar_try_wait(bar_scales + 8 * stage, phase) || (leader && !mc_mbar_try_wait(bar_full + 8 * stage, phase))) {
                         if (mc_globaltimer() - t0 > MC_WAIT_NS / 4) {
                             if (p.status != nullptr) atomicOr(p.status, MC_FP4_ERR_DRAIN);
                             break;
@@ -472,9 +487,8 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
             constexpr unsigned idesc = fp4_instruction<kFormat>(kPairTile, kPairTile);
             int stage = 0, acc = 0;
             unsigned phase = 0;
-            int done_stage = 0;         // the K block two before the one at work
-            unsigned done_phase = 0;
-            int blocks = 0;
+            int ready = 0;
+            unsigned ready_phase = 0;
             unsigned empty_phase = 1;  // the first tile waits for nothing
             bool ok = true;
             for (int item = cluster; ok && item < items; item += clusters) {
@@ -484,29 +498,15 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned tmem_d = tmem + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
-                    if (blocks >= 2) {
-                        ok = mc_mbar_wait(bar_empty + 8 * done_stage, done_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
-                        if (!ok) break;
-                        if (++done_stage == stages) {
-                            done_stage = 0;
-                            done_phase ^= 1u;
-                        }
-                    }
                     ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                    if (!ok) break;
+                    ok = mc_mbar_wait(bar_ready + 8 * ready, ready_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned rows_src = tiles_base + stage * Pair::kStageBytes;
                     const unsigned cols_src = rows_src + Pair::kRowBytes;
-                    const unsigned row_scales_src = cols_src + Pair::kColBytes;
-                    const unsigned col_scales_src = row_scales_src + Pair::kRowScaleBytes;
-                    const unsigned scale_r = tmem + Pair::kScaleBase + static_cast<unsigned>((blocks & 1) * Pair::kScaleColumns);
+                    const unsigned scale_r = tmem + Pair::kScaleBase + static_cast<unsigned>(ready * Pair::kScaleColumns);
                     const unsigned scale_c = scale_r + Pair::kRowScaleColumns;
-#pragma unroll
-                    for (int t = 0; t < Pair::kScaleTiles; ++t) {
-                        fp4_scales_to_tmem<2>(scale_r + 4 * t, fp4_scale_desc(row_scales_src + t * kFp4TileBytes));
-                        fp4_scales_to_tmem<2>(scale_c + 8 * t, fp4_scale_desc(col_scales_src + t * kFp4TileBytes));
-                        fp4_scales_to_tmem<2>(scale_c + 8 * t + 4, fp4_scale_desc(col_scales_src + (Pair::kScaleTiles + t) * kFp4TileBytes));
-                    }
                     const unsigned long long desc_r = fp4_tile_desc(rows_src);
                     const unsigned long long desc_c = fp4_tile_desc(cols_src);
 #pragma unroll
@@ -517,7 +517,10 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                                             (kb > 0 || ks > 0) ? 1u : 0u);
                     }
                     fp4_commit_pair(bar_empty + 8 * stage);
-                    ++blocks;
+                    if (++ready == Pair::kScaleBuffers) {
+                        ready = 0;
+                        ready_phase ^= 1u;
+                    }
                     if (++stage == stages) {
                         stage = 0;
                         phase ^= 1u;
@@ -526,6 +529,50 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                 if (!ok) break;
                 fp4_commit_pair(bar_acc_full);
                 acc ^= 1;
+            }
+        }
+    } else if (warp >= 10) {
+        // Scales from shared memory to the 32 TMEM lanes of this warp, the same in every quarter: lane r takes the 16 bytes
+        // of rows r, r + 32, r + 64, r + 96 of a tile as four columns.
+        const unsigned tmem_lanes = tmem + (static_cast<unsigned>((warp & 3) * 32) << 16) + Pair::kScaleBase;
+        const unsigned bar_leader = cluster_address(bar_ready, 0);
+        int stage = 0, done_stage = 0, ready = 0, number = 0;
+        unsigned phase = 0, done_phase = 0;
+        bool ok = true;
+        for (int item = cluster; ok && item < items; item += clusters) {
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                if (number >= Pair::kScaleBuffers) {  // the K block that used this buffer has been multiplied
+                    ok = mc_mbar_wait(bar_empty + 8 * done_stage, done_phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
+                    if (++done_stage == stages) {
+                        done_stage = 0;
+                        done_phase ^= 1u;
+                    }
+                }
+                ok = ok && mc_mbar_wait(bar_scales + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned src = tiles_base + stage * Pair::kStageBytes + Pair::kTileBytes + static_cast<unsigned>(lane * 16);
+                const unsigned dst = tmem_lanes + static_cast<unsigned>(ready * Pair::kScaleColumns);
+                unsigned v[Pair::kScaleColumns];
+#pragma unroll
+                for (int t = 0; t < Pair::kScaleTiles; ++t) {
+                    load_shared_v4(src + t * kFp4TileBytes, v + 4 * t);
+                    load_shared_v4(src + Pair::kRowScaleBytes + t * kFp4TileBytes, v + Pair::kRowScaleColumns + 8 * t);
+                    load_shared_v4(src + Pair::kRowScaleBytes + (Pair::kScaleTiles + t) * kFp4TileBytes, v + Pair::kRowScaleColumns + 8 * t + 4);
+                }
+#pragma unroll
+                for (int c = 0; c < Pair::kScaleColumns; c += 8) tmem_store8(dst + c, v + c);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(bar_leader + 8 * ready);
+                ++number;
+                if (++ready == Pair::kScaleBuffers) ready = 0;
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
         }
     } else {

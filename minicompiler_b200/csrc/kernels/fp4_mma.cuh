@@ -93,10 +93,11 @@ __device__ __forceinline__ void tma_load_2d_pair(unsigned smem_dst, const McTens
         "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(unsigned smem_dst, const McTensorMap* map, unsigned bar_cluster_addr, int c0, int c1, int c2) {
+// A three-dimensional box, counted on a barrier of this CTA.
+__device__ __forceinline__ void tma_load_3d(unsigned smem_dst, const McTensorMap* map, unsigned bar, int c0, int c1, int c2) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
-        "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 // One box out of shared memory; what lies outside the tensor is not written.
@@ -124,6 +125,16 @@ __device__ __forceinline__ void tmem_load16(unsigned taddr, unsigned* v) {
           "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
+}
+
+__device__ __forceinline__ void load_shared_v4(unsigned addr, unsigned* v) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void tmem_store8(unsigned taddr, const unsigned* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned* v) {
