@@ -487,6 +487,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
             constexpr unsigned idesc = fp4_instruction<kFormat>(kPairTile, kPairTile);
             int stage = 0, acc = 0;
             unsigned phase = 0;
+            bool seen = false;  // the next K block was seen to be ready while the one before it was being issued
             int ready = 0;
             unsigned ready_phase = 0;
             unsigned empty_phase = 1;  // the first tile waits for nothing
@@ -498,10 +499,11 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned tmem_d = tmem + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
-                    ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA);
-                    if (!ok) break;
-                    ok = mc_mbar_wait(bar_ready + 8 * ready, ready_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
-                    if (!ok) break;
+                    if (!seen) {
+                        ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA) &&
+                             mc_mbar_wait(bar_ready + 8 * ready, ready_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
+                        if (!ok) break;
+                    }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned rows_src = tiles_base + stage * Pair::kStageBytes;
                     const unsigned cols_src = rows_src + Pair::kRowBytes;
@@ -509,14 +511,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     const unsigned scale_c = scale_r + Pair::kRowScaleColumns;
                     const unsigned long long desc_r = fp4_tile_desc(rows_src);
                     const unsigned long long desc_c = fp4_tile_desc(cols_src);
-#pragma unroll
-                    for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
-                        const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
-                        const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
-                        fp4_mma<kFormat, 2>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 8 * t,
-                                            (kb > 0 || ks > 0) ? 1u : 0u);
-                    }
-                    fp4_commit_pair(bar_empty + 8 * stage);
+                    const int this_stage = stage;
                     if (++ready == Pair::kScaleBuffers) {
                         ready = 0;
                         ready_phase ^= 1u;
@@ -525,6 +520,17 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                         stage = 0;
                         phase ^= 1u;
                     }
+#pragma unroll
+                    for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
+                        // The answers of these tests are needed only behind the last multiply: their latency (some 80 cycles
+                        // each, in which a queue of one or two multiplies runs dry) passes while they are being issued.
+                        if (ks == 2) seen = mbar_test(bar_full + 8 * stage, phase) & mbar_test(bar_ready + 8 * ready, ready_phase);
+                        const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
+                        const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
+                        fp4_mma<kFormat, 2>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 8 * t,
+                                            (kb > 0 || ks > 0) ? 1u : 0u);
+                    }
+                    fp4_commit_pair(bar_empty + 8 * this_stage);
                 }
                 if (!ok) break;
                 fp4_commit_pair(bar_acc_full);
@@ -541,17 +547,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         bool ok = true;
         for (int item = cluster; ok && item < items; item += clusters) {
             for (int kb = 0; kb < p.k_blocks; ++kb) {
-                if (number >= Pair::kScaleBuffers) {  // the K block that used this buffer has been multiplied
-                    ok = mc_mbar_wait(bar_empty + 8 * done_stage, done_phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
-                    if (++done_stage == stages) {
-                        done_stage = 0;
-                        done_phase ^= 1u;
-                    }
-                }
-                ok = ok && mc_mbar_wait(bar_scales + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                ok = mc_mbar_wait(bar_scales + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
                 const unsigned src = tiles_base + stage * Pair::kStageBytes + Pair::kTileBytes + static_cast<unsigned>(lane * 16);
                 const unsigned dst = tmem_lanes + static_cast<unsigned>(ready * Pair::kScaleColumns);
                 unsigned v[Pair::kScaleColumns];
@@ -561,6 +557,16 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     load_shared_v4(src + Pair::kRowScaleBytes + t * kFp4TileBytes, v + Pair::kRowScaleColumns + 8 * t);
                     load_shared_v4(src + Pair::kRowScaleBytes + (Pair::kScaleTiles + t) * kFp4TileBytes, v + Pair::kRowScaleColumns + 8 * t + 4);
                 }
+                if (ok && number >= Pair::kScaleBuffers) {  // the K block that used this buffer has been multiplied
+                    ok = mc_mbar_wait(bar_empty + 8 * done_stage, done_phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
+                    if (++done_stage == stages) {
+                        done_stage = 0;
+                        done_phase ^= 1u;
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < Pair::kScaleColumns; c += 8) tmem_store8(dst + c, v + c);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
