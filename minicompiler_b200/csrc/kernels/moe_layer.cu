@@ -17,9 +17,17 @@
 // matching values of a token, instead of the interleaved order of the fragment's definition.
 // Scales: E8M0_32 - 32 columns (one block) are two multiplies into a fresh sum, which then counts scale times; E4M3_16 -
 // code * scale is exact in f16 (6 bits, 2^-10 .. 2688), so the codes are scaled before the multiply.
-// x and h come to f16 as well, after a power of two per token (x) or per token and expert (h) that takes the largest
-// magnitude to [2^14, 2^15): 11 bits are kept of values down to 2^-29 of the largest. bf16 and f16 inputs lose nothing
-// above that, h is rounded to 11 bits.
+//
+// x and h come to f16 as well, after a power of two that takes the largest magnitude to [2^14, 2^15): one per token for x,
+// and for h one per token, expert and 8 rows (those of one warp's tile, which knows them without asking anybody); the
+// down projection brings them to the power of the largest. 11 bits are kept of values down to 2^-29 of the largest: bf16
+// and f16 inputs lose nothing above that, h is rounded to 11 bits.
+//
+// How the weights stream: a CTA has 8 warps, four tiles of 16 rows by two halves of k. Every warp keeps a ring of its own
+// in shared memory filled by 16-byte cp.async, three steps of 256 columns ahead of the multiplies and across the ends of
+// rows, tokens and experts; two CTAs per SM have some 100 KB in flight, which is what the memory's latency asks for. No
+// barrier orders the weights: a warp waits for its own copies. The tokens' values are prefetched into registers one round
+// (1024 columns) ahead and pass through two buffers that the CTA shares.
 
 #include "minicompiler_b200_device.h"
 
@@ -39,17 +47,21 @@ using namespace mcd;
 namespace {
 
 constexpr int kTokenTile = 8;        // columns of one mma
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStageK = 256;         // codes per row and stage: 128 bytes
-constexpr int kStages = 6;
-constexpr int kChunkK = 1024;        // values of a token in shared memory at a time
-constexpr int kValuePitch = 2 * (kChunkK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
+constexpr int kTiles = 4;            // of 16 rows, per CTA
+constexpr int kHalves = 2;           // of the columns of a round
+constexpr int kThreads = kTiles * kHalves * 32;
+constexpr int kStageK = 256;         // codes per row and step: 128 bytes
+constexpr int kRoundSteps = 2;       // per warp
+constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
+constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
+constexpr int kValueBytes = kTokenTile * kValuePitch;
+constexpr int kPieces = kTokenTile * kRoundK / 8 / kThreads;  // of 8 values, per thread and round
 constexpr int kMaxSlots = MCD_MOE_MAX_TOKENS * MCD_MOE_MAX_TOP_K;
-constexpr int kDownRows = 64;
+constexpr int kDownRows = kTiles * 16;
 constexpr int kDownPitch = kDownRows + 4;
 constexpr int kRouterCluster = 8;
 constexpr int kRouterThreads = 256;
+constexpr int kUpStages = 4, kDownStages = 3;  // depth of a warp's ring; the down projection keeps sums beside it
 
 template <int kFormat>
 struct Stage {
@@ -63,7 +75,7 @@ struct Matrix4 {
     const unsigned char* scales;
     const float* tensor_scale;
     long long matrix_codes, matrix_scales, pitch;
-    int k_tiles, stages;  // per row
+    int k_tiles, stages, rounds;  // per row
 };
 
 struct MoeParams {
@@ -73,17 +85,20 @@ struct MoeParams {
     long long ldx, ld_router, ldy;
     int type, tokens, top_k, renormalize, experts;
     int d, f;
+    int f_pitch;     // f in whole groups of 8
+    int f_groups;    // tiles of 8 rows of h: 16 for every 128 rows begun
     int x_vec;       // rows of x start on 16-byte boundaries
     int router_vec;  // rows of x and of the router do
     Matrix4 gate_up, down;
     int* chosen_out;
     float* weights_out;
     // workspace
-    int* chosen;           // [tokens * top_k]
-    float* weights;        // [tokens * top_k]
-    float* x_shift;        // [tokens]: the power of two that x is multiplied with
-    unsigned* h_max;       // [tokens * top_k]: bits of the largest |h|
-    float* h;              // [tokens * top_k][f]
+    int* chosen;              // [tokens * top_k]
+    float* weights;           // [tokens * top_k]
+    int* h_max;               // [tokens * top_k]: the largest of h_exponent
+    float* x_shift;           // [tokens]: the power of two that x is multiplied with
+    unsigned char* h_exponent;  // [tokens * top_k][f_groups]: f32 exponent of the largest |h| among a tile's rows
+    unsigned short* h;        // [tokens * top_k][f_pitch]: f16 after shift_for of that exponent
 };
 
 __device__ __forceinline__ float value16(unsigned short v, int type) {
@@ -96,13 +111,10 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
     return d;
 }
 
-// The power of two that takes a largest magnitude (as bits) to [2^14, 2^15). Zero, infinity and NaN are left alone; the
-// exponent stops where the factor or its inverse would leave f32.
-__device__ __forceinline__ float shift_for(unsigned max_bits) {
-    if (max_bits == 0 || max_bits >= 0x7f800000u) return 1.0f;
-    const int e = max(-113, min(120, 14 - (static_cast<int>(max_bits >> 23) - 127)));
-    return __uint_as_float(static_cast<unsigned>(e + 127) << 23);
-}
+// The exponent of the power of two that takes magnitudes of f32 exponent `e` (biased) to [2^14, 2^15). Zero, infinity and
+// NaN are left alone; it stops where the factor or its inverse would leave f32.
+__device__ __forceinline__ int shift_of(int e) { return e == 0 || e >= 255 ? 0 : max(-113, min(120, 14 - (e - 127))); }
+__device__ __forceinline__ float power(int e) { return __uint_as_float(static_cast<unsigned>(e + 127) << 23); }
 __device__ __forceinline__ float inverse_power(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
@@ -124,17 +136,38 @@ __device__ __forceinline__ unsigned peer_address(unsigned addr, unsigned rank) {
 
 // ------------------------------------------------------------------------------------------------------------- router
 
-// True when (a, i) comes before (b, j): the larger logit, ties to the lower index, NaN behind every number.
-__device__ __forceinline__ bool before(double a, int i, double b, int j) {
-    const bool a_nan = a != a, b_nan = b != b;
-    if (a_nan != b_nan) return b_nan;
-    if (!a_nan && a != b) return a > b;
-    return i < j;
+// A logit as an unsigned number of the same order; NaN below every number.
+__device__ __forceinline__ unsigned long long sort_key(double l) {
+    const auto bits = static_cast<unsigned long long>(__double_as_longlong(l));
+    if (l != l) return 0ull;
+    return bits >> 63 ? ~bits : bits | (1ull << 63);
+}
+
+// sum + c is the running sum to twice f32's precision: the exact error of each addition is collected.
+__device__ __forceinline__ void add_exactly(float& sum, float& c, float v) {
+    const float t = __fadd_rn(sum, v);
+    const float b = __fsub_rn(t, sum);
+    c = __fadd_rn(c, __fadd_rn(__fsub_rn(sum, __fsub_rn(t, b)), __fsub_rn(v, b)));
+    sum = t;
+}
+
+__device__ __forceinline__ void add_products(float& sum, float& c, const uint4& a, const uint4& b, int type) {
+    const unsigned aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // products of 16-bit values are exact in f32
+        add_exactly(sum, c, value16(aw[i] & 0xffffu, type) * value16(bw[i] & 0xffffu, type));
+        add_exactly(sum, c, value16(aw[i] >> 16, type) * value16(bw[i] >> 16, type));
+    }
 }
 
 __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads) mc_moe_router(const MoeParams p) {
-    __shared__ double logits[MCD_MOE_MAX_EXPERTS];  // of the cluster's first CTA
+    // used in the cluster's first CTA
+    __shared__ double logits[MCD_MOE_MAX_EXPERTS];
+    __shared__ unsigned long long keys[MCD_MOE_MAX_EXPERTS];
+    __shared__ int order[MCD_MOE_MAX_EXPERTS];
+    __shared__ int best[MCD_MOE_MAX_TOP_K];
     __shared__ unsigned warp_max[kRouterThreads / 32];
+    __shared__ float warp_sum[kRouterThreads / 32];
     const int token = blockIdx.x / kRouterCluster;
     const unsigned rank = cluster_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -142,151 +175,181 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned short* x = p.x + token * p.ldx;
     const unsigned logits_first = peer_address(smem_u32(logits), 0);
-    cluster_sync_all();  // every CTA of the cluster runs before its shared memory is written
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    bool started = false;
 
-    for (int e = static_cast<int>(rank) * (kRouterThreads / 32) + warp; e < p.experts; e += kRouterCluster * (kRouterThreads / 32)) {
-        const unsigned short* r = p.router + e * p.ld_router;
-        double sum = 0.0;
-        if (p.router_vec) {
-            for (int c = lane * 8; c + 8 <= p.d; c += 256) {
-                const uint4 a = *reinterpret_cast<const uint4*>(x + c), b = *reinterpret_cast<const uint4*>(r + c);
-                const unsigned aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    for (int e = static_cast<int>(rank) * (kRouterThreads / 32) + warp; e < p.experts || !started; e += kRouterCluster * (kRouterThreads / 32)) {
+        double total = 0.0;
+        if (e < p.experts) {
+            const unsigned short* r = p.router + e * p.ld_router;
+            float sum[2] = {0.0f, 0.0f}, c[2] = {0.0f, 0.0f};
+            int at = lane * 8;
+            if (p.router_vec) {
+                for (; at + 768 + 8 <= p.d; at += 1024) {  // four loads of each row in flight
+                    uint4 a[4], b[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {  // products of 16-bit values are exact in f32
-                    sum += static_cast<double>(value16(aw[i] & 0xffffu, p.type) * value16(bw[i] & 0xffffu, p.type));
-                    sum += static_cast<double>(value16(aw[i] >> 16, p.type) * value16(bw[i] >> 16, p.type));
+                    for (int i = 0; i < 4; ++i) {
+                        a[i] = *reinterpret_cast<const uint4*>(x + at + 256 * i);
+                        b[i] = __ldcs(reinterpret_cast<const uint4*>(r + at + 256 * i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) add_products(sum[i & 1], c[i & 1], a[i], b[i], p.type);
+                }
+                for (; at + 8 <= p.d; at += 256) {
+                    add_products(sum[0], c[0], *reinterpret_cast<const uint4*>(x + at), *reinterpret_cast<const uint4*>(r + at), p.type);
                 }
             }
-        }
-        for (int c = (p.router_vec ? p.d / 8 * 8 : 0) + lane; c < p.d; c += 32) sum += static_cast<double>(value16(x[c], p.type)) * value16(r[c], p.type);
+            for (int k = (p.router_vec ? p.d / 8 * 8 : 0) + lane; k < p.d; k += 32) add_exactly(sum[0], c[0], value16(x[k], p.type) * value16(r[k], p.type));
+            // an infinite or NaN sum has no error to speak of
+            const float whole = sum[0] + sum[1];
+            const bool finite = fabsf(whole) <= 3.402823466e38f;
+            total = finite ? (static_cast<double>(sum[0]) + sum[1]) + (static_cast<double>(c[0]) + c[1]) : static_cast<double>(whole);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(sum) : "memory");
+            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        }
+        if (!started) {  // the first CTA of the cluster runs before its shared memory is written
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            started = true;
+        }
+        if (e < p.experts && lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(total) : "memory");
     }
     unsigned largest = 0;
     if (rank == 0) {
         for (int c = threadIdx.x; c < p.d; c += kRouterThreads) largest = max(largest, __float_as_uint(value16(x[c], p.type)) & 0x7fffffffu);
         largest = __reduce_max_sync(0xffffffffu, largest);
         if (lane == 0) warp_max[warp] = largest;
+        for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) order[e] = 0;
+        if (threadIdx.x < p.top_k) p.h_max[token * p.top_k + threadIdx.x] = 0;
     }
     cluster_sync_all();
     if (rank != 0) return;
-    if (threadIdx.x < p.top_k) p.h_max[token * p.top_k + threadIdx.x] = 0u;
-    if (warp != 0) return;
-    largest = __reduce_max_sync(0xffffffffu, lane < kRouterThreads / 32 ? warp_max[lane] : 0u);
-    if (lane == 0) p.x_shift[token] = shift_for(largest);
 
-    // best logit first; then the softmax's sum, one lane's share after the other's in a fixed tree
-    constexpr int kPerLane = MCD_MOE_MAX_EXPERTS / 32;
-    double top = 0.0;
-    float total = 0.0f, kept = 0.0f;
-    float mine = 0.0f;  // lane j keeps the weight of the j-th choice
-    int my_choice = 0;
-    unsigned taken = 0;
-    for (int j = 0; j < p.top_k; ++j) {
-        double best = 0.0;
-        int at = 0x7fffffff;
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const int e = i * 32 + lane;
-            if (e < p.experts && !((taken >> i) & 1u)) {
-                const double l = logits[e];
-                if (!any || before(l, e, best, at)) best = l, at = e, any = true;
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double other = __shfl_xor_sync(0xffffffffu, best, o);
-            const int other_at = __shfl_xor_sync(0xffffffffu, at, o);
-            const bool other_any = __shfl_xor_sync(0xffffffffu, static_cast<int>(any), o) != 0;
-            if (other_any && (!any || before(other, other_at, best, at))) best = other, at = other_at, any = true;
-        }
-        if ((at & 31) == lane) taken |= 1u << (at >> 5);
-        if (j == 0) {
-            top = best;
-            for (int e = lane; e < p.experts; e += 32) total += expf(static_cast<float>(logits[e] - top));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        }
-        const float w = expf(static_cast<float>(best - top)) / total;
-        kept += w;
-        if (lane == j) mine = w, my_choice = at;
+    for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) keys[e] = sort_key(logits[e]);
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kRouterThreads / 32; ++w) largest = max(largest, warp_max[w]);
+        p.x_shift[token] = power(shift_of(static_cast<int>(largest >> 23)));
     }
+    __syncthreads();
+    // An expert's place is the number of experts that come before it: the larger logit, ties to the lower index. Several
+    // threads share the comparisons of one expert where there are fewer than threads.
+    const int shares = max(1, kRouterThreads / p.experts);
+    for (int i = threadIdx.x; i < p.experts * shares; i += kRouterThreads) {
+        const int e = i % p.experts;
+        const unsigned long long key = keys[e];
+        int before = 0;
+        for (int j = i / p.experts; j < p.experts; j += shares) before += keys[j] > key || (keys[j] == key && j < e) ? 1 : 0;
+        if (before != 0) atomicAdd(&order[e], before);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) {
+        if (order[e] < p.top_k) best[order[e]] = e;
+    }
+    __syncthreads();
+    const double top = logits[best[0]];
+    float total = 0.0f;
+    for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) total += expf(static_cast<float>(logits[e] - top));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) warp_sum[warp] = total;
+    __syncthreads();
+    if (warp != 0) return;
+    total = 0.0f;
+    for (int w = 0; w < kRouterThreads / 32; ++w) total += warp_sum[w];
+    float weight = 0.0f, kept = 0.0f;
+    if (lane < p.top_k) weight = expf(static_cast<float>(logits[best[lane]] - top)) / total;
+    for (int j = 0; j < p.top_k; ++j) kept += __shfl_sync(0xffffffffu, weight, j);
     if (lane < p.top_k) {
-        const float w = p.renormalize ? mine / kept : mine;
+        if (p.renormalize) weight /= kept;
         const int slot = token * p.top_k + lane;
-        p.chosen[slot] = my_choice;
-        p.weights[slot] = w;
-        if (p.chosen_out != nullptr) p.chosen_out[slot] = my_choice;
-        if (p.weights_out != nullptr) p.weights_out[slot] = w;
+        p.chosen[slot] = best[lane];
+        p.weights[slot] = weight;
+        if (p.chosen_out != nullptr) p.chosen_out[slot] = best[lane];
+        if (p.weights_out != nullptr) p.weights_out[slot] = weight;
     }
 }
 
 // ------------------------------------------------------------------------------------------- rows of codes times tokens
 
-// Experts that somebody chose, in order of their index.
+// The experts that somebody chose, in order of their index, and who chose them. The order of an expert's slots is left to
+// the atomics: each is a column of its own, and nothing is added up over an expert's columns.
 struct Routing {
-    int chosen[kMaxSlots];
     short active[MCD_MOE_MAX_EXPERTS];
-    int count[MCD_MOE_MAX_EXPERTS];
+    short start[MCD_MOE_MAX_EXPERTS + 1];  // of each active expert's slots
+    short slots[kMaxSlots];                // token * top_k + rank
     int num_active;
-    int slots[MCD_MOE_MAX_TOKENS];  // of the expert at work: token * top_k + rank, in that order (a token names it once)
-    int num_slots;
 };
 
-__device__ __forceinline__ void load_routing(Routing& r, const MoeParams& p) {
+// `scratch`: an int per expert. Ends with a barrier.
+__device__ __forceinline__ void load_routing(Routing& r, int* scratch, const MoeParams& p) {
     const int all = p.tokens * p.top_k;
-    for (int e = threadIdx.x; e < p.experts; e += kThreads) r.count[e] = 0;
+    for (int e = threadIdx.x; e < p.experts; e += kThreads) scratch[e] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < all; i += kThreads) {
-        const int e = p.chosen[i];
-        r.chosen[i] = e;
-        atomicAdd(&r.count[e], 1);
-    }
+    for (int i = threadIdx.x; i < all; i += kThreads) atomicAdd(&scratch[p.chosen[i]], 1);
     __syncthreads();
     if (threadIdx.x < 32) {
-        int n = 0;
+        int n = 0, slots = 0;
         for (int base = 0; base < p.experts; base += 32) {
             const int e = base + static_cast<int>(threadIdx.x);
-            const bool used = e < p.experts && r.count[e] > 0;
-            const unsigned mask = __ballot_sync(0xffffffffu, used);
-            if (used) r.active[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = static_cast<short>(e);
+            const int count = e < p.experts ? scratch[e] : 0;
+            const unsigned mask = __ballot_sync(0xffffffffu, count > 0);
+            int sum = count;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int below = __shfl_up_sync(0xffffffffu, sum, o);
+                if (static_cast<int>(threadIdx.x) >= o) sum += below;
+            }
+            if (count > 0) {
+                const int at = n + __popc(mask & ((1u << threadIdx.x) - 1u));
+                r.active[at] = static_cast<short>(e);
+                r.start[at] = static_cast<short>(slots + sum - count);
+                scratch[e] = slots + sum - count;
+            }
             n += __popc(mask);
+            slots += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (threadIdx.x == 0) r.num_active = n;
+        if (threadIdx.x == 0) {
+            r.num_active = n;
+            r.start[n] = static_cast<short>(slots);
+        }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < all; i += kThreads) r.slots[atomicAdd(&scratch[p.chosen[i]], 1)] = static_cast<short>(i);
     __syncthreads();
 }
 
-// Slots of expert e into r.slots. The caller has a barrier before (nobody reads the old ones) and after.
-__device__ __forceinline__ void list_slots(Routing& r, int e, int all) {
-    if (threadIdx.x < 32) {
-        int n = 0;
-        for (int base = 0; base < all; base += 32) {
-            const int i = base + static_cast<int>(threadIdx.x);
-            const bool mine = i < all && r.chosen[i] == e;
-            const unsigned mask = __ballot_sync(0xffffffffu, mine);
-            if (mine) r.slots[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = i;
-            n += __popc(mask);
-        }
-        if (threadIdx.x == 0) r.num_slots = n;
-    }
-}
+// What a CTA works through: rows of an expert against up to 8 of its slots.
+struct Pass {
+    int item;    // up: (active expert, group of rows); down: active expert
+    int first;   // slot within the expert
+};
 
-// The 16 rows of a warp's tile as it streams them: row[i] of the lane's four 16-byte copies per stage (rows i * 4 + lane / 8)
-// and the rows of its scale words.
-template <int kFormat>
+// Copies of a warp's 16 rows: four 16-byte pieces per lane and step (rows i * 4 + lane / 8), and the scale words of row
+// lane % 16.
+template <int kFormat, int kStages>
 struct RowStream {
     const unsigned char* codes[4];   // nullptr: no such row
     const unsigned char* scales;     // of row lane % 16: its word in the first scale tile of its row group
     long long pitch;
     int k_tiles;
-    unsigned ring;                   // this warp's stages in shared memory
 
-    __device__ __forceinline__ void issue(int s) const {
+    // Rows of the tile: row_of(i) for i = 0 .. 15, negative where there is none.
+    template <typename RowOf>
+    __device__ __forceinline__ void aim(const Matrix4& m, int expert, RowOf&& row_of) {
         const int lane = threadIdx.x & 31;
-        const unsigned base = ring + static_cast<unsigned>(s % kStages) * Stage<kFormat>::kBytes;
+        const unsigned char* matrix = m.codes + expert * m.matrix_codes;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row_of(i * 4 + (lane >> 3));
+            codes[i] = r < 0 ? nullptr : matrix + r * m.pitch;
+        }
+        const int r = max(0, row_of(lane & 15));  // no such row: its sums go nowhere, any scale will do
+        scales = m.scales + expert * m.matrix_scales + fp4_scale_offset(r, 0, m.k_tiles);
+        pitch = m.pitch;
+        k_tiles = m.k_tiles;
+    }
+
+    __device__ __forceinline__ void issue(int s, unsigned base) const {
+        const int lane = threadIdx.x & 31;
         const int c = lane & 7;
         const long long at = static_cast<long long>(s) * 128 + c * 16;
 #pragma unroll
@@ -310,26 +373,10 @@ struct RowStream {
     }
 };
 
-__device__ __forceinline__ void copies_done_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
-__device__ __forceinline__ unsigned lds32(unsigned a) {
-    unsigned v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint4 lds128(unsigned a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
 __device__ __forceinline__ void mma16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned mul_f16x2(unsigned a, unsigned b) {
     unsigned d;
@@ -343,22 +390,29 @@ __device__ __forceinline__ void e8m0x2(unsigned two, float& lo, float& hi) {
     lo = __uint_as_float(d << 16);
     hi = __uint_as_float(d & 0xffff0000u);
 }
+// Byte `which & 7` of a word as e4m3, in both halves of an f16 pair.
+__device__ __forceinline__ unsigned e4m3_pair(unsigned word, unsigned which) {
+    unsigned d;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(__byte_perm(word, 0, which)));
+    return d;
+}
 
-// One stage: 16 rows x 256 codes of the ring slot at `base`, times the values at `values` (f16, token rows kValuePitch apart).
+// One step: 16 rows x 256 codes at `base` times the values at `values` (f16, token rows kValuePitch apart).
 template <int kFormat>
-__device__ __forceinline__ void multiply_stage(unsigned base, unsigned values, float (&acc)[4]) {
+__device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[4]) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const unsigned scales = base + Stage<kFormat>::kCodeBytes;
-    const unsigned v_at = values + static_cast<unsigned>(g * kValuePitch + t * 16);
-    const unsigned sel = static_cast<unsigned>(t >> 1) * 0x11u;
+    const unsigned char* scales = base + Stage<kFormat>::kCodeBytes + g * 4;
+    const unsigned char* v_at = values + g * kValuePitch + t * 16;
+    const unsigned char* c_at = base + g * 128 + t * 4;
+    const unsigned which = static_cast<unsigned>(t >> 1) * 0x11u;
     float scale_lo[4], scale_hi[4];
     unsigned word_lo = 0, word_hi = 0;
 #pragma unroll
     for (int b = 0; b < kStageK / 32; ++b) {
-        const unsigned at = base + static_cast<unsigned>(g * 128 + ((b ^ g) << 4) + t * 4);
-        const unsigned lo = lds32(at), hi = lds32(at + 8 * 128);
-        const uint4 v = lds128(v_at + b * 64);
+        const unsigned lo = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4));
+        const unsigned hi = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4) + 8 * 128);
+        const uint4 v = *reinterpret_cast<const uint4*>(v_at + b * 64);
         unsigned a[4], c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -367,7 +421,8 @@ __device__ __forceinline__ void multiply_stage(unsigned base, unsigned values, f
         }
         if constexpr (kFormat == MCD_FP4_E8M0_32) {
             if ((b & 3) == 0) {
-                word_lo = lds32(scales + (b >> 2) * 64 + g * 4), word_hi = lds32(scales + (b >> 2) * 64 + (g + 8) * 4);
+                word_lo = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64);
+                word_hi = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64 + 32);
                 e8m0x2(word_lo & 0xffffu, scale_lo[0], scale_lo[1]);
                 e8m0x2(word_lo >> 16, scale_lo[2], scale_lo[3]);
                 e8m0x2(word_hi & 0xffffu, scale_hi[0], scale_hi[1]);
@@ -381,11 +436,11 @@ __device__ __forceinline__ void multiply_stage(unsigned base, unsigned values, f
             acc[2] = fmaf(s[2], scale_hi[b & 3], acc[2]);
             acc[3] = fmaf(s[3], scale_hi[b & 3], acc[3]);
         } else {
-            if ((b & 1) == 0) word_lo = lds32(scales + (b >> 1) * 64 + g * 4), word_hi = lds32(scales + (b >> 1) * 64 + (g + 8) * 4);
-            const unsigned which = sel + (b & 1 ? 0x22u : 0u);
-            unsigned s_lo, s_hi;
-            asm("{\n\t.reg .b32 w;\n\t.reg .b16 t;\n\tprmt.b32 w, %1, 0, %2;\n\tcvt.u16.u32 t, w;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(s_lo) : "r"(word_lo), "r"(which));
-            asm("{\n\t.reg .b32 w;\n\t.reg .b16 t;\n\tprmt.b32 w, %1, 0, %2;\n\tcvt.u16.u32 t, w;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(s_hi) : "r"(word_hi), "r"(which));
+            if ((b & 1) == 0) {
+                word_lo = *reinterpret_cast<const unsigned*>(scales + (b >> 1) * 64);
+                word_hi = *reinterpret_cast<const unsigned*>(scales + (b >> 1) * 64 + 32);
+            }
+            const unsigned s_lo = e4m3_pair(word_lo, which + (b & 1 ? 0x22u : 0u)), s_hi = e4m3_pair(word_hi, which + (b & 1 ? 0x22u : 0u));
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] = mul_f16x2(a[i], s_lo), c[i] = mul_f16x2(c[i], s_hi);
             mma16816(acc, a[0], c[0], a[1], c[1], v.x, v.y);
@@ -394,194 +449,314 @@ __device__ __forceinline__ void multiply_stage(unsigned base, unsigned values, f
     }
 }
 
-// acc = 16 rows (this warp's) x 8 tokens over the whole of k. `stage_values(first, count)` has the CTA's threads bring values
-// first .. first + count of the current tokens to shared memory.
-template <int kFormat, typename Values>
-__device__ __forceinline__ void multiply_rows(const RowStream<kFormat>& rows, int stages, unsigned values, float (&acc)[4], Values&& stage_values) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (s < stages) rows.issue(s);
-        copies_done_group();
-    }
-    constexpr int kPerChunk = kChunkK / kStageK;
-    for (int s = 0; s < stages; ++s) {
-        if (s % kPerChunk == 0) {
-            __syncthreads();  // the chunk before has been read
-            stage_values(s * kStageK, min(kChunkK, (stages - s) * kStageK));
-            __syncthreads();
-        }
-        copies_wait<kStages - 2>();
-        __syncwarp();
-        multiply_stage<kFormat>(rows.ring + static_cast<unsigned>(s % kStages) * Stage<kFormat>::kBytes,
-                                values + static_cast<unsigned>(s % kPerChunk) * kStageK * 2, acc);
-        __syncwarp();
-        if (s + kStages - 1 < stages) rows.issue(s + kStages - 1);
-        copies_done_group();
-    }
-    copies_wait<0>();
-    __syncwarp();
-}
-
-// Rows of a warp's tile: row_of(i) for i = 0 .. 15, negative where there is none.
-template <int kFormat, typename RowOf>
-__device__ __forceinline__ void aim(RowStream<kFormat>& s, const Matrix4& m, int expert, unsigned ring, RowOf&& row_of) {
-    const int lane = threadIdx.x & 31;
-    const unsigned char* codes = m.codes + expert * m.matrix_codes;
-    const unsigned char* scales = m.scales + expert * m.matrix_scales;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = row_of(i * 4 + (lane >> 3));
-        s.codes[i] = r < 0 ? nullptr : codes + r * m.pitch;
-    }
-    const int r = max(0, row_of(lane & 15));  // a row that is not there: its codes are 0, any scale of this matrix but NaN would do
-    s.scales = scales + fp4_scale_offset(r, 0, m.k_tiles);
-    s.pitch = m.pitch;
-    s.k_tiles = m.k_tiles;
-    s.ring = ring;
-}
-
-__device__ __forceinline__ void store_values(unsigned values, int token, int k, const float (&v)[8]) {
-    const unsigned a = values + static_cast<unsigned>(token * kValuePitch + k * 2);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(pack_f16(v[0], v[1])), "r"(pack_f16(v[2], v[3])),
-                 "r"(pack_f16(v[4], v[5])), "r"(pack_f16(v[6], v[7]))
-                 : "memory");
-}
-
-template <int kFormat>
-constexpr int kRingBytes = kWarps * kStages * Stage<kFormat>::kBytes;
-constexpr int kValueBytes = kTokenTile * kValuePitch;
-
-template <int kFormat>
-__global__ void __launch_bounds__(kThreads) mc_moe_up(const MoeParams p) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ Routing routing;
+// The two projections differ in what a pass is, where values come from and what becomes of the sums; Work supplies these:
+//   begin(pass), next(pass)   the CTA's first pass, the one after: false when there is none
+//   expert(pass)              its active expert
+//   aim(rows, pass)           point the stream at the warp's rows
+//   load(pass, k, n)          8 values of the n-th slot from column k on, as they lie in memory
+//   finish(loaded)            the same in f16
+//   done(pass, here, acc)     a warp's sums, both halves of k
+template <int kFormat, int kStages, typename Work>
+__device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned values = smem_u32(smem);
-    const unsigned ring = values + kValueBytes + static_cast<unsigned>(warp * kStages * Stage<kFormat>::kBytes);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    load_routing(routing, p);
-    const int groups = (p.f + 127) / 128 * 4;  // 32 rows of G each
-    const int items = routing.num_active * groups;
-    const int all = p.tokens * p.top_k;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int expert = routing.active[item / groups];
-        const int group = item % groups;
-        // Rows of a 128-row scale tile that share 32 bytes of scales: two neighbours in each of the four groups of 32.
-        auto row_in_f = [&](int g) { return (group >> 2) * 128 + 32 * (g >> 1) + 8 * (group & 3) + 2 * warp + (g & 1); };
-        RowStream<kFormat> rows;
-        aim(rows, p.gate_up, expert, ring, [&](int i) {
-            const int r = row_in_f(i & 7);
+    const int tile = warp % kTiles, half = warp / kTiles;
+    unsigned char* ring = rings + warp * kStages * Stage<kFormat>::kBytes;
+    const unsigned ring_at = smem_u32(ring);
+    const int steps = m.rounds * kRoundSteps;
+
+    // three walks over the same passes: the copies run ahead of the values, the values ahead of the multiplies
+    Pass at;
+    bool more = work.begin(at);
+    if (!more) return;
+    Pass ahead = at;
+    bool ahead_more = true;
+    int ahead_step = 0, ahead_slot = 0;
+    RowStream<kFormat, kStages> rows;
+    work.aim(rows, ahead, tile);
+    auto copy_next = [&] {
+        if (ahead_more) {
+            const int s = (ahead_step / kRoundSteps) * (kRoundSteps * kHalves) + half * kRoundSteps + ahead_step % kRoundSteps;
+            if (s < m.stages) rows.issue(s, ring_at + static_cast<unsigned>(ahead_slot * Stage<kFormat>::kBytes));
+            if (++ahead_slot == kStages) ahead_slot = 0;
+            if (++ahead_step == steps) {
+                ahead_step = 0;
+                const int item = ahead.item;
+                ahead_more = work.next(ahead);
+                if (ahead_more && ahead.item != item) work.aim(rows, ahead, tile);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy_next();
+
+    Pass value_pass = at;
+    bool value_more = true;
+    int value_round = 0;
+    typename Work::Piece pieces[kPieces];
+    auto slots_of = [&](const Pass& pass) {
+        const int e = work.active(pass);
+        return min(kTokenTile, routing.start[e + 1] - routing.start[e] - pass.first);
+    };
+    auto load_values = [&] {
+        if (!value_more) return;
+        const int here = slots_of(value_pass);
+        const short* slots = routing.slots + routing.start[work.active(value_pass)] + value_pass.first;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int piece = i * kThreads + static_cast<int>(threadIdx.x);
+            const int n = piece / (kRoundK / 8);
+            if (n < here) work.load(pieces[i], slots[n], value_round * kRoundK + piece % (kRoundK / 8) * 8);
+        }
+    };
+    auto store_values = [&](unsigned char* to) {
+        if (!value_more) return;
+        const int here = slots_of(value_pass);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int piece = i * kThreads + static_cast<int>(threadIdx.x);
+            const int n = piece / (kRoundK / 8);
+            if (n < here) *reinterpret_cast<uint4*>(to + n * kValuePitch + piece % (kRoundK / 8) * 16) = work.finish(pieces[i]);
+        }
+        if (++value_round == m.rounds) {
+            value_round = 0;
+            value_more = work.next(value_pass);
+        }
+    };
+    load_values();
+    store_values(values);
+    int buffer = 0, slot = 0;
+
+    while (more) {
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int round = 0; round < m.rounds; ++round) {
+            __syncthreads();  // this round's values are there, nobody reads the other buffer any more
+            load_values();
+#pragma unroll
+            for (int j = 0; j < kRoundSteps; ++j) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                __syncwarp();
+                copy_next();  // into the slot of the step before, which all lanes have left
+                const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
+                if (s < m.stages) {
+                    multiply_step<kFormat>(ring + slot * Stage<kFormat>::kBytes, values + buffer * kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), acc);
+                }
+                if (++slot == kStages) slot = 0;
+            }
+            buffer ^= 1;
+            store_values(values + buffer * kValueBytes);
+        }
+        if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        __syncthreads();
+        if (half == 0) {
+            const float4 other = halves[tile * 32 + lane];
+            acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
+            work.done(at, slots_of(at), tile, acc);
+        }
+        more = work.next(at);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// -------------------------------------------------------------------------------------------------------- up and down
+
+struct UpWork {
+    struct Piece {
+        uint4 raw;
+        float shift;
+    };
+    const MoeParams& p;
+    const Routing& routing;
+    int groups;  // of 32 rows of G (and of U): four for every 128 rows begun
+
+    __device__ __forceinline__ bool begin(Pass& pass) const {
+        pass.item = blockIdx.x;
+        pass.first = 0;
+        return pass.item < routing.num_active * groups;
+    }
+    __device__ __forceinline__ int active(const Pass& pass) const { return pass.item / groups; }
+    __device__ __forceinline__ bool next(Pass& pass) const {
+        const int a = active(pass);
+        pass.first += kTokenTile;
+        if (pass.first < routing.start[a + 1] - routing.start[a]) return true;
+        pass.first = 0;
+        pass.item += gridDim.x;
+        return pass.item < routing.num_active * groups;
+    }
+    // Rows that share 32 bytes of scales: two neighbours in each of the four groups of 32 of a 128-row tile.
+    __device__ __forceinline__ int row_in_f(const Pass& pass, int tile, int g) const {
+        const int group = pass.item % groups;
+        return (group >> 2) * 128 + 32 * (g >> 1) + 8 * (group & 3) + 2 * tile + (g & 1);
+    }
+    template <typename Rows>
+    __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
+        rows.aim(p.gate_up, routing.active[active(pass)], [&](int i) {
+            const int r = row_in_f(pass, tile, i & 7);
             return r >= p.f ? -1 : i < 8 ? r : p.f + r;
         });
-        __syncthreads();
-        list_slots(routing, expert, all);
-        __syncthreads();
-        const float scale = p.gate_up.tensor_scale != nullptr ? p.gate_up.tensor_scale[expert] : 1.0f;
-        for (int first = 0; first < routing.num_slots; first += kTokenTile) {
-            const int here = min(kTokenTile, routing.num_slots - first);
-            float acc[4];
-            multiply_rows<kFormat>(rows, p.gate_up.stages, values, acc, [&](int k0, int count) {
-                for (int i = threadIdx.x; i < here * (count / 8); i += kThreads) {
-                    const int n = i / (count / 8), k = (i - n * (count / 8)) * 8;
-                    const int token = routing.slots[first + n] / p.top_k;
-                    const unsigned short* x = p.x + token * p.ldx;
-                    const float shift = p.x_shift[token];
-                    float v[8];
-                    const int c = k0 + k;
-                    if (p.x_vec && c + 8 <= p.d) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(x + c);
-                        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+    }
+    __device__ __forceinline__ void load(Piece& piece, int slot, int k) const {
+        const int token = slot / p.top_k;
+        const unsigned short* x = p.x + token * p.ldx + k;
+        piece.shift = p.x_shift[token];
+        if (p.x_vec && k + 8 <= p.d) {
+            piece.raw = *reinterpret_cast<const uint4*>(x);
+        } else {
+            unsigned v[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[2 * j] = value16(w[j] & 0xffffu, p.type) * shift, v[2 * j + 1] = value16(w[j] >> 16, p.type) * shift;
-                    } else {
+            for (int j = 0; j < 8; ++j) v[j] = k + j < p.d ? x[j] : 0u;
+            piece.raw = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+        }
+    }
+    __device__ __forceinline__ uint4 finish(const Piece& piece) const {
+        const unsigned w[4] = {piece.raw.x, piece.raw.y, piece.raw.z, piece.raw.w};
+        unsigned v[4];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = c + j < p.d ? value16(x[c + j], p.type) * shift : 0.0f;
-                    }
-                    store_values(values, n, k, v);
+        for (int j = 0; j < 4; ++j) v[j] = pack_f16(value16(w[j] & 0xffffu, p.type) * piece.shift, value16(w[j] >> 16, p.type) * piece.shift);
+        return make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
+        const int lane = threadIdx.x & 31;
+        const int g = lane >> 2, t = lane & 3;
+        const int a = active(pass);
+        const int r = row_in_f(pass, tile, g);
+        const float scale = p.gate_up.tensor_scale != nullptr ? p.gate_up.tensor_scale[routing.active[a]] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int n = 2 * t + j;
+            const int slot = n < here ? routing.slots[routing.start[a] + pass.first + n] : 0;
+            float h = 0.0f;
+            if (n < here && r < p.f) {
+                const float back = inverse_power(p.x_shift[slot / p.top_k]) * scale;
+                const float gate = acc[j] * back, up = acc[2 + j] * back;
+                h = gate / (1.0f + expf(-gate)) * up;
+            }
+            int e = static_cast<int>((__float_as_uint(h) >> 23) & 0xffu);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+            if (n < here) {
+                const float shifted = h * power(shift_of(e));
+                if (r < p.f_pitch) p.h[static_cast<long long>(slot) * p.f_pitch + r] = static_cast<unsigned short>(pack_f16(shifted, 0.0f) & 0xffffu);
+                if (g == 0) {
+                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.item % groups * kTiles + tile] = static_cast<unsigned char>(e);
+                    atomicMax(p.h_max + slot, e);
                 }
-            });
-            const int g = lane >> 2, t = lane & 3;
-            const int r = row_in_f(g);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = 2 * t + j;
-                unsigned largest = 0;
-                if (n < here && r < p.f) {
-                    const int slot = routing.slots[first + n];
-                    const float back = inverse_power(p.x_shift[slot / p.top_k]) * scale;
-                    const float gate = acc[j] * back, up = acc[2 + j] * back;
-                    const float h = gate / (1.0f + expf(-gate)) * up;
-                    p.h[static_cast<long long>(slot) * p.f + r] = h;
-                    largest = __float_as_uint(h) & 0x7fffffffu;
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-                if (g == 0 && n < here && largest != 0) atomicMax(p.h_max + routing.slots[first + n], largest);
             }
         }
     }
-}
+};
 
 template <int kFormat>
-__global__ void __launch_bounds__(kThreads) mc_moe_down(const MoeParams p, int cluster) {
+constexpr int ring_bytes(int stages) { return kTiles * kHalves * stages * Stage<kFormat>::kBytes; }
+template <int kFormat>
+constexpr int kUpSmem = 2 * kValueBytes + ring_bytes<kFormat>(kUpStages);
+template <int kFormat>
+constexpr int kDownSmem = MCD_MOE_MAX_TOKENS * kDownPitch * 4 + 2 * kValueBytes + ring_bytes<kFormat>(kDownStages);
+
+template <int kFormat>
+__global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* sums = reinterpret_cast<float*>(smem);  // [tokens][kDownPitch]
-    const unsigned values = smem_u32(smem) + static_cast<unsigned>(MCD_MOE_MAX_TOKENS * kDownPitch * 4);
-    const unsigned ring = values + kValueBytes + static_cast<unsigned>(warp * kStages * Stage<kFormat>::kBytes);
-    const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int group = blockIdx.x / cluster;  // 64 rows of y: one half of the 16 rows in each group of 32 of a 128-row tile
+    __shared__ float4 halves[kTiles * 32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    load_routing(routing, p);
-    for (int i = threadIdx.x; i < p.tokens * kDownPitch; i += kThreads) sums[i] = 0.0f;
-    const int all = p.tokens * p.top_k;
-    auto row_in_y = [&](int i) { return (group >> 1) * 128 + 32 * (i >> 2) + 16 * (group & 1) + 4 * warp + (i & 3); };
-    for (int a = rank; a < routing.num_active; a += cluster) {
-        const int expert = routing.active[a];
-        RowStream<kFormat> rows;
-        aim(rows, p.down, expert, ring, [&](int i) {
-            const int r = row_in_y(i);
+    load_routing(routing, reinterpret_cast<int*>(smem), p);
+    UpWork work{p, routing, p.f_groups / kTiles};
+    run_passes<kFormat, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * kValueBytes, halves);
+}
+
+struct DownWork {
+    struct Piece {
+        uint4 raw;
+        unsigned exponents;
+        int largest;
+    };
+    const MoeParams& p;
+    const Routing& routing;
+    float* sums;  // [tokens][kDownPitch]
+    int group;    // 64 rows of y: one half of the 16 rows in each group of 32 of a 128-row tile
+    int first, step;
+
+    __device__ __forceinline__ bool begin(Pass& pass) const {
+        pass.item = first;
+        pass.first = 0;
+        return pass.item < routing.num_active;
+    }
+    __device__ __forceinline__ int active(const Pass& pass) const { return pass.item; }
+    __device__ __forceinline__ bool next(Pass& pass) const {
+        pass.first += kTokenTile;
+        if (pass.first < routing.start[pass.item + 1] - routing.start[pass.item]) return true;
+        pass.first = 0;
+        pass.item += step;
+        return pass.item < routing.num_active;
+    }
+    // Row i of a tile: four neighbours in each group of 32, so that a warp uses 64 of 128 bytes of scales, the tile beside it the rest.
+    __device__ __forceinline__ int row_in_y(int tile, int i) const { return (group >> 1) * 128 + 32 * (i >> 2) + 16 * (group & 1) + 4 * tile + (i & 3); }
+    template <typename Rows>
+    __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
+        rows.aim(p.down, routing.active[pass.item], [&](int i) {
+            const int r = row_in_y(tile, i);
             return r < p.d ? r : -1;
         });
-        __syncthreads();
-        list_slots(routing, expert, all);
-        __syncthreads();
-        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[expert] : 1.0f;
-        for (int first = 0; first < routing.num_slots; first += kTokenTile) {
-            const int here = min(kTokenTile, routing.num_slots - first);
-            float acc[4];
-            multiply_rows<kFormat>(rows, p.down.stages, values, acc, [&](int k0, int count) {
-                for (int i = threadIdx.x; i < here * (count / 8); i += kThreads) {
-                    const int n = i / (count / 8), k = (i - n * (count / 8)) * 8;
-                    const int slot = routing.slots[first + n];
-                    const float* h = p.h + static_cast<long long>(slot) * p.f;
-                    const float shift = shift_for(p.h_max[slot]);
-                    float v[8];
+    }
+    // Columns k .. k + 7 are two rows each of four of the tiles that h came from.
+    __device__ __forceinline__ void load(Piece& piece, int slot, int k) const {
+        piece.largest = p.h_max[slot];
+        if (k < p.f_pitch) {
+            piece.raw = *reinterpret_cast<const uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
+            piece.exponents = *reinterpret_cast<const unsigned*>(p.h_exponent + static_cast<long long>(slot) * p.f_groups + (k >> 7) * 16 + ((k >> 3) & 3) * 4);
+        } else {
+            piece.raw = make_uint4(0, 0, 0, 0);
+            piece.exponents = 0;
+        }
+    }
+    __device__ __forceinline__ uint4 finish(const Piece& piece) const {
+        const int to = shift_of(piece.largest);
+        unsigned w[4] = {piece.raw.x, piece.raw.y, piece.raw.z, piece.raw.w};
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = k0 + k + j < p.f ? h[k0 + k + j] * shift : 0.0f;
-                    store_values(values, n, k, v);
-                }
-            });
-            const int g = lane >> 2, t = lane & 3;
+        for (int j = 0; j < 4; ++j) {
+            // 2^(to - from) as f16, at most 1 (what came from a smaller largest is multiplied up less); below 2^-24 it is 0
+            const int down = shift_of(static_cast<int>((piece.exponents >> (8 * j)) & 0xffu)) - to;
+            const unsigned factor = down <= 0 ? 0x3c00u : down <= 14 ? static_cast<unsigned>(15 - down) << 10 : down <= 24 ? 1u << (24 - down) : 0u;
+            w[j] = mul_f16x2(w[j], factor | factor << 16);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
+        const int lane = threadIdx.x & 31;
+        const int g = lane >> 2, t = lane & 3;
+        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.item]] : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = 2 * t + j;
-                if (n < here) {
-                    const int slot = routing.slots[first + n];
-                    const float back = inverse_power(shift_for(p.h_max[slot])) * scale;
-                    const float w = p.weights[slot];
-                    // this warp's 16 columns; nobody else adds to them
-                    float* sum = sums + slot / p.top_k * kDownPitch + warp * 16;
-                    sum[g] += w * (acc[j] * back);
-                    sum[g + 8] += w * (acc[2 + j] * back);
-                }
+        for (int j = 0; j < 2; ++j) {
+            const int n = 2 * t + j;
+            if (n < here) {
+                const int slot = routing.slots[routing.start[pass.item] + pass.first + n];
+                const float back = power(-shift_of(p.h_max[slot])) * scale;
+                const float w = p.weights[slot];
+                // this warp's 16 columns; nobody else adds to them
+                float* sum = sums + slot / p.top_k * kDownPitch + tile * 16;
+                sum[g] += w * (acc[j] * back);
+                sum[g + 8] += w * (acc[2 + j] * back);
             }
         }
     }
+};
+
+template <int kFormat>
+__global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ Routing routing;
+    __shared__ float4 halves[kTiles * 32];
+    float* sums = reinterpret_cast<float*>(smem);
+    unsigned char* values = smem + MCD_MOE_MAX_TOKENS * kDownPitch * 4;
+    const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int group = blockIdx.x / cluster;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    load_routing(routing, reinterpret_cast<int*>(values), p);
+    for (int i = threadIdx.x; i < p.tokens * kDownPitch; i += kThreads) sums[i] = 0.0f;
+    __syncthreads();
+    DownWork work{p, routing, sums, group, rank, cluster};
+    run_passes<kFormat, kDownStages>(work, p.down, routing, values, values + 2 * kValueBytes, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
     // Every CTA of the cluster finishes its share of the elements: the partial sums in rank order.
@@ -600,8 +775,7 @@ __global__ void __launch_bounds__(kThreads) mc_moe_down(const MoeParams p, int c
             }
             v += part;
         }
-        const int w = c >> 4, k = c & 15;
-        const int r = (group >> 1) * 128 + 32 * (k >> 2) + 16 * (group & 1) + 4 * w + (k & 3);
+        const int r = work.row_in_y(c >> 4, c & 15);
         if (r < p.d) {
             unsigned short out;
             if (p.type == MCD_HALF_BF16) {
@@ -614,11 +788,6 @@ __global__ void __launch_bounds__(kThreads) mc_moe_down(const MoeParams p, int c
     }
     if (cluster > 1) cluster_sync_all();  // shared memory stays until the last peer has read it
 }
-
-template <int kFormat>
-constexpr int kUpSmem = kValueBytes + kRingBytes<kFormat>;
-template <int kFormat>
-constexpr int kDownSmem = MCD_MOE_MAX_TOKENS * kDownPitch * 4 + kValueBytes + kRingBytes<kFormat>;
 
 // ---------------------------------------------------------------------------------------------------------- host side
 
@@ -658,7 +827,7 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     // The router's clusters are declared with the kernel.
     if (int rc = launch(mc_moe_router, static_cast<unsigned>(p.tokens * kRouterCluster), 1, kRouterThreads, 0, s, "mc_moe_router", p)) return rc;
     const int reached = std::min(p.experts, p.tokens * p.top_k);
-    const long long most = static_cast<long long>(reached) * ((p.f + 127) / 128 * 4);
+    const long long most = static_cast<long long>(reached) * (p.f_groups / kTiles);
     const auto up_grid = static_cast<unsigned>(std::min<long long>(most, 2LL * sm_count()));
     if (int rc = launch(mc_moe_up<kFormat>, up_grid, 1, kThreads, kUpSmem<kFormat>, s, "mc_moe_up", p)) return rc;
     int cluster = 8;
@@ -668,6 +837,9 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
 }
 
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
+size_t f_pitch(long long f) { return static_cast<size_t>((f + 7) / 8 * 8); }
+size_t f_groups(long long f) { return static_cast<size_t>((f + 127) / 128 * 16); }
 
 Matrix4 matrix_of(const mcd_fp4_tensor& t) {
     const Fp4Geometry geo = fp4_geometry(t.format, t.rows, t.cols);
@@ -680,6 +852,7 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
     m.pitch = geo.pitch;
     m.k_tiles = static_cast<int>(geo.k_tiles);
     m.stages = static_cast<int>((t.cols + kStageK - 1) / kStageK);
+    m.rounds = static_cast<int>((t.cols + kRoundK - 1) / kRoundK);
     return m;
 }
 
@@ -688,7 +861,7 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
 extern "C" size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f) {
     if (tokens < 1 || tokens > MCD_MOE_MAX_TOKENS || experts < 1 || top_k < 1 || top_k > MCD_MOE_MAX_TOP_K || d < 1 || f < 1) return 0;
     const size_t slots = static_cast<size_t>(tokens) * static_cast<size_t>(top_k);
-    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + rounded(slots * static_cast<size_t>(f) * 4);
+    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + rounded(slots * f_groups(f)) + rounded(slots * f_pitch(f) * 2);
 }
 
 extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
@@ -741,6 +914,8 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     p.experts = experts;
     p.d = static_cast<int>(d);
     p.f = static_cast<int>(f);
+    p.f_pitch = static_cast<int>(f_pitch(f));
+    p.f_groups = static_cast<int>(f_groups(f));
     p.x_vec = is_aligned(args->x, 16) && args->ldx % 8 == 0;
     p.router_vec = p.x_vec && is_aligned(args->router, 16) && args->ld_router % 8 == 0;
     p.gate_up = matrix_of(gu);
@@ -751,9 +926,10 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     auto* at = static_cast<unsigned char*>(args->workspace);
     p.chosen = reinterpret_cast<int*>(at);
     p.weights = reinterpret_cast<float*>(at += rounded(slots * 4));
-    p.h_max = reinterpret_cast<unsigned*>(at += rounded(slots * 4));
+    p.h_max = reinterpret_cast<int*>(at += rounded(slots * 4));
     p.x_shift = reinterpret_cast<float*>(at += rounded(slots * 4));
-    p.h = reinterpret_cast<float*>(at += rounded(static_cast<size_t>(args->tokens) * 4));
+    p.h_exponent = at += rounded(static_cast<size_t>(args->tokens) * 4);
+    p.h = reinterpret_cast<unsigned short*>(at += rounded(slots * f_groups(f)));
     auto s = static_cast<cudaStream_t>(stream);
     return gu.format == MCD_FP4_E8M0_32 ? launch_layer<MCD_FP4_E8M0_32>(p, s) : launch_layer<MCD_FP4_E4M3_16>(p, s);
 }
