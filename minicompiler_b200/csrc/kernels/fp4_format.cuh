@@ -38,18 +38,28 @@ __device__ __forceinline__ long long fp4_scale_offset(long long r, long long b, 
     return ((r >> 7) * k_tiles + (b >> 2)) * kFp4TileBytes + ((r & 31) << 4) + (((r >> 5) & 3) << 2) + (b & 3);
 }
 
-// Two codes, round to nearest even, magnitudes over 6 become 6; `lo` goes to the low four bits.
-__device__ __forceinline__ unsigned fp4_encode2(float lo, float hi) {
+// The conversions below take words apart, and put them together, by vector moves of 8- and 16-bit registers: the compiler
+// then lets the conversion itself pick its byte. With shifts and masks instead, eight codes take 12 integer
+// instructions where these take 4 (10.5 against 5.3 words per cycle and SM).
+
+// Eight codes from v[0 .. 7], round to nearest even, magnitudes over 6 become 6; v[0] goes to the lowest four bits.
+__device__ __forceinline__ unsigned fp4_encode8(const float* v) {
     unsigned r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
 
-// The values of the two codes of the low byte, as packed f16 (the low half holds the low four bits).
-__device__ __forceinline__ unsigned fp4_decode2(unsigned byte) {
-    unsigned r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(r) : "r"(byte));
-    return r;
+// The values of the eight codes of a word as four f16 pairs, the lowest four bits in the low half of the first.
+__device__ __forceinline__ void fp4_decode8(unsigned word, unsigned (&pairs)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(pairs[0]), "=r"(pairs[1]), "=r"(pairs[2]), "=r"(pairs[3])
+        : "r"(word));
 }
 
 __device__ __forceinline__ float f16_lo(unsigned h2) {

@@ -162,12 +162,9 @@ __global__ void __launch_bounds__(kThreads) mc_fp4_quantize(const QuantizeParams
                 inverse = s_g == 0.0f ? 0.0f : fminf(__fdiv_rn(1.0f, s_g), 3.402823466e38f);
             }
             const bool bad = byte == (kFormat == MCD_FP4_E8M0_32 ? 255u : 0x7fu);  // the NaN scales; no rounding gives them
-            unsigned lo = 0, hi = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                lo |= fp4_encode2(__fmul_rn(v[2 * i], inverse), __fmul_rn(v[2 * i + 1], inverse)) << (8 * i);
-                hi |= fp4_encode2(__fmul_rn(v[8 + 2 * i], inverse), __fmul_rn(v[9 + 2 * i], inverse)) << (8 * i);
-            }
+            for (int i = 0; i < kUnit; ++i) v[i] = __fmul_rn(v[i], inverse);
+            unsigned lo = fp4_encode8(v), hi = fp4_encode8(v + 8);
             if (bad) lo = hi = 0;
             if (real && live && c0 / 2 < p.code_pitch) *reinterpret_cast<uint2*>(codes + c0 / 2) = make_uint2(lo, hi);
             if (inside && live) {
@@ -220,10 +217,14 @@ __global__ void __launch_bounds__(kThreads) mc_fp4_dequantize(const DequantizePa
             }
             float v[kUnit];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned h2 = fp4_decode2(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu);
-                v[2 * i] = f16_lo(h2) * scale;  // exact: at most 6 significant bits
-                v[2 * i + 1] = f16_hi(h2) * scale;
+            for (int i = 0; i < 2; ++i) {
+                unsigned pairs[4];
+                fp4_decode8(i == 0 ? w.x : w.y, pairs);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[8 * i + 2 * j] = f16_lo(pairs[j]) * scale;  // exact: at most 6 significant bits
+                    v[8 * i + 2 * j + 1] = f16_hi(pairs[j]) * scale;
+                }
             }
             if (kFormat == MCD_FP4_E4M3_16) {
 #pragma unroll

@@ -383,17 +383,19 @@ __device__ __forceinline__ unsigned mul_f16x2(unsigned a, unsigned b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// Two e8m0 bytes -> two f32 (bf16 holds every power of two they stand for, and NaN).
-__device__ __forceinline__ void e8m0x2(unsigned two, float& lo, float& hi) {
-    unsigned d;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, t;\n\t}" : "=r"(d) : "r"(two));
-    lo = __uint_as_float(d << 16);
-    hi = __uint_as_float(d & 0xffff0000u);
+// Four e8m0 bytes -> four f32 (bf16 holds every power of two they stand for, and NaN).
+__device__ __forceinline__ void e8m0x4(unsigned word, float (&s)[4]) {
+    unsigned lo, hi;
+    asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %2;\n\tcvt.rn.bf16x2.ue8m0x2 %0, t;\n\tcvt.rn.bf16x2.ue8m0x2 %1, u;\n\t}" : "=r"(lo), "=r"(hi) : "r"(word));
+    s[0] = __uint_as_float(lo << 16);
+    s[1] = __uint_as_float(lo & 0xffff0000u);
+    s[2] = __uint_as_float(hi << 16);
+    s[3] = __uint_as_float(hi & 0xffff0000u);
 }
 // Byte `which & 7` of a word as e4m3, in both halves of an f16 pair.
 __device__ __forceinline__ unsigned e4m3_pair(unsigned word, unsigned which) {
     unsigned d;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(__byte_perm(word, 0, which)));
+    asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(__byte_perm(word, 0, which)));
     return d;
 }
 
@@ -414,19 +416,14 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
         const unsigned hi = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4) + 8 * 128);
         const uint4 v = *reinterpret_cast<const uint4*>(v_at + b * 64);
         unsigned a[4], c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = fp4_decode2((lo >> (8 * i)) & 0xffu);
-            c[i] = fp4_decode2((hi >> (8 * i)) & 0xffu);
-        }
+        fp4_decode8(lo, a);
+        fp4_decode8(hi, c);
         if constexpr (kFormat == MCD_FP4_E8M0_32) {
             if ((b & 3) == 0) {
                 word_lo = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64);
                 word_hi = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64 + 32);
-                e8m0x2(word_lo & 0xffffu, scale_lo[0], scale_lo[1]);
-                e8m0x2(word_lo >> 16, scale_lo[2], scale_lo[3]);
-                e8m0x2(word_hi & 0xffffu, scale_hi[0], scale_hi[1]);
-                e8m0x2(word_hi >> 16, scale_hi[2], scale_hi[3]);
+                e8m0x4(word_lo, scale_lo);
+                e8m0x4(word_hi, scale_hi);
             }
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma16816(s, a[0], c[0], a[1], c[1], v.x, v.y);
