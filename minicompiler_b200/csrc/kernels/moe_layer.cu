@@ -276,6 +276,7 @@ struct Routing {
     short active[MCD_MOE_MAX_EXPERTS];
     short start[MCD_MOE_MAX_EXPERTS + 1];  // of each active expert's slots
     short slots[kMaxSlots];                // token * top_k + rank
+    unsigned char tokens[kMaxSlots];       // of each of them
     int num_active;
 };
 
@@ -313,62 +314,91 @@ __device__ __forceinline__ void load_routing(Routing& r, int* scratch, const Moe
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < all; i += kThreads) r.slots[atomicAdd(&scratch[p.chosen[i]], 1)] = static_cast<short>(i);
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+        const int at = atomicAdd(&scratch[p.chosen[i]], 1);
+        r.slots[at] = static_cast<short>(i);
+        r.tokens[at] = static_cast<unsigned char>(i / p.top_k);
+    }
     __syncthreads();
 }
 
 // What a CTA works through: rows of an expert against up to 8 of its slots.
 struct Pass {
-    int item;    // up: (active expert, group of rows); down: active expert
+    int active;  // which of the active experts
+    int group;   // of rows (up only)
     int first;   // slot within the expert
 };
 
+// Where the 16-byte piece c of a row lies within the row's 128 bytes of a step, so that what lanes read together falls
+// into different banks: E8M0_32 reads words of eight rows at a time, E4M3_16 whole pieces of two rows.
+template <int kFormat>
+__device__ __forceinline__ int piece_at(int row, int c) {
+    return kFormat == MCD_FP4_E8M0_32 ? c ^ (row & 7) : c ^ ((row & 1) << 2);
+}
+
 // Copies of a warp's 16 rows: four 16-byte pieces per lane and step (rows i * 4 + lane / 8), and the scale words of row
 // lane % 16.
-template <int kFormat, int kStages>
+template <int kFormat>
 struct RowStream {
-    const unsigned char* codes[4];   // nullptr: no such row
-    const unsigned char* scales;     // of row lane % 16: its word in the first scale tile of its row group
-    long long pitch;
-    int k_tiles;
+    const unsigned char* codes[4];   // at this lane's piece of the first step; any address where there is no such row
+    const unsigned char* scales;     // at this lane's first word
+    unsigned there;                  // bit i: row i exists; all ones where every row of the tile does
+    int piece;                       // bytes from the start of a row
+    int pitch, k_tiles;
 
     // Rows of the tile: row_of(i) for i = 0 .. 15, negative where there is none.
     template <typename RowOf>
     __device__ __forceinline__ void aim(const Matrix4& m, int expert, RowOf&& row_of) {
         const int lane = threadIdx.x & 31;
         const unsigned char* matrix = m.codes + expert * m.matrix_codes;
+        piece = (lane & 7) * 16;
+        there = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = row_of(i * 4 + (lane >> 3));
-            codes[i] = r < 0 ? nullptr : matrix + r * m.pitch;
+            codes[i] = matrix + max(r, 0) * m.pitch + piece;
+            there |= r >= 0 ? 1u << i : 0u;
         }
+        if (__all_sync(0xffffffffu, there == 15u)) there = ~0u;
         const int r = max(0, row_of(lane & 15));  // no such row: its sums go nowhere, any scale will do
-        scales = m.scales + expert * m.matrix_scales + fp4_scale_offset(r, 0, m.k_tiles);
-        pitch = m.pitch;
+        scales = m.scales + expert * m.matrix_scales + fp4_scale_offset(r, 0, m.k_tiles) + (lane >> 4) * kFp4TileBytes;
+        pitch = static_cast<int>(m.pitch);
         k_tiles = m.k_tiles;
     }
 
     __device__ __forceinline__ void issue(int s, unsigned base) const {
         const int lane = threadIdx.x & 31;
-        const int c = lane & 7;
-        const long long at = static_cast<long long>(s) * 128 + c * 16;
+        const long long at = static_cast<long long>(s) * 128;
+        const long long scales_at = static_cast<long long>(s) * (Stage<kFormat>::kScaleWords * kFp4TileBytes);
+        const unsigned dst = base + (lane >> 3) * 128;
+        const unsigned scales_dst = base + Stage<kFormat>::kCodeBytes + lane * 4;
+        // rows i * 4 + lane / 8: the swizzle goes by the row's low bits
+        const unsigned even = dst + (piece_at<kFormat>(lane >> 3, lane & 7) << 4), odd = dst + (piece_at<kFormat>(4 + (lane >> 3), lane & 7) << 4);
+        if (there == ~0u && at + 128 <= pitch && (s + 1) * Stage<kFormat>::kScaleWords <= k_tiles) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((i & 1 ? odd : even) + i * 512), "l"(codes[i] + at) : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_dst + i * 128), "l"(scales + scales_at + i * 2 * kFp4TileBytes) : "memory");
+            }
+            return;
+        }
+        // the end of the rows, or rows that are not there: zeros
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = i * 4 + (lane >> 3);
-            const bool there = codes[i] != nullptr && at < pitch;
-            const unsigned dst = base + row * 128 + ((c ^ (row & 7)) << 4);
-            const void* src = there ? codes[i] + at : static_cast<const void*>(scales);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+            const bool real = ((there >> i) & 1u) != 0 && at + piece < pitch;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((i & 1 ? odd : even) + i * 512), "l"(real ? codes[i] + at : scales - (lane >> 4) * kFp4TileBytes),
+                         "r"(real ? 16 : 0)
+                         : "memory");
         }
-        const int row = lane & 15;
 #pragma unroll
         for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
-            const int word = i * 2 + (lane >> 4);
-            const int tile = s * Stage<kFormat>::kScaleWords + word;
-            const bool there = tile < k_tiles;
-            const unsigned dst = base + Stage<kFormat>::kCodeBytes + (word * 16 + row) * 4;
-            const void* src = there ? scales + static_cast<long long>(tile) * kFp4TileBytes : scales;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+            const bool real = s * Stage<kFormat>::kScaleWords + i * 2 + (lane >> 4) < k_tiles;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_dst + i * 128),
+                         "l"(real ? scales + scales_at + i * 2 * kFp4TileBytes : scales - (lane >> 4) * kFp4TileBytes), "r"(real ? 4 : 0)
+                         : "memory");
         }
     }
 };
@@ -392,67 +422,87 @@ __device__ __forceinline__ void e8m0x4(unsigned word, float (&s)[4]) {
     s[2] = __uint_as_float(hi << 16);
     s[3] = __uint_as_float(hi & 0xffff0000u);
 }
-// Byte `which & 7` of a word as e4m3, in both halves of an f16 pair.
-__device__ __forceinline__ unsigned e4m3_pair(unsigned word, unsigned which) {
-    unsigned d;
-    asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(__byte_perm(word, 0, which)));
-    return d;
+// Two e4m3 bytes -> two f16 pairs, each of one scale twice.
+__device__ __forceinline__ void e4m3_pairs(unsigned short two, unsigned& first, unsigned& second) {
+    unsigned both;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(both) : "h"(two));
+    first = __byte_perm(both, 0, 0x1010);
+    second = __byte_perm(both, 0, 0x3232);
+}
+
+// Where the 8 values from column k on lie in a token's row (in pieces of 16 bytes), so that the pieces that the four
+// lanes of a token read together are neighbours. E8M0_32: lane t takes columns 8 t of every block of 32, which is the
+// columns' own order. E4M3_16: lane t takes 32 columns in a row, a quarter of them at a time.
+template <int kFormat>
+__device__ __forceinline__ int value_piece(int k) {
+    const int i = k >> 3;
+    return kFormat == MCD_FP4_E8M0_32 ? i : (i & ~15) | (i & 3) << 2 | (i >> 2 & 3);
 }
 
 // One step: 16 rows x 256 codes at `base` times the values at `values` (f16, token rows kValuePitch apart).
 template <int kFormat>
-__device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[4]) {
+__device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[2][4]) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const unsigned char* scales = base + Stage<kFormat>::kCodeBytes + g * 4;
     const unsigned char* v_at = values + g * kValuePitch + t * 16;
-    const unsigned char* c_at = base + g * 128 + t * 4;
-    const unsigned which = static_cast<unsigned>(t >> 1) * 0x11u;
-    float scale_lo[4], scale_hi[4];
-    unsigned word_lo = 0, word_hi = 0;
+    if constexpr (kFormat == MCD_FP4_E8M0_32) {
+        const unsigned char* scales = base + Stage<kFormat>::kCodeBytes + g * 4;
+        const unsigned char* c_at = base + g * 128 + t * 4;
+        float scale_lo[4], scale_hi[4];
 #pragma unroll
-    for (int b = 0; b < kStageK / 32; ++b) {
-        const unsigned lo = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4));
-        const unsigned hi = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4) + 8 * 128);
-        const uint4 v = *reinterpret_cast<const uint4*>(v_at + b * 64);
-        unsigned a[4], c[4];
-        fp4_decode8(lo, a);
-        fp4_decode8(hi, c);
-        if constexpr (kFormat == MCD_FP4_E8M0_32) {
+        for (int b = 0; b < kStageK / 32; ++b) {
+            const unsigned lo = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4));
+            const unsigned hi = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4) + 8 * 128);
+            const uint4 v = *reinterpret_cast<const uint4*>(v_at + b * 64);
             if ((b & 3) == 0) {
-                word_lo = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64);
-                word_hi = *reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64 + 32);
-                e8m0x4(word_lo, scale_lo);
-                e8m0x4(word_hi, scale_hi);
+                e8m0x4(*reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64), scale_lo);
+                e8m0x4(*reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64 + 32), scale_hi);
             }
+            unsigned a[4], c[4];
+            fp4_decode8(lo, a);
+            fp4_decode8(hi, c);
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma16816(s, a[0], c[0], a[1], c[1], v.x, v.y);
             mma16816(s, a[2], c[2], a[3], c[3], v.z, v.w);
-            acc[0] = fmaf(s[0], scale_lo[b & 3], acc[0]);
-            acc[1] = fmaf(s[1], scale_lo[b & 3], acc[1]);
-            acc[2] = fmaf(s[2], scale_hi[b & 3], acc[2]);
-            acc[3] = fmaf(s[3], scale_hi[b & 3], acc[3]);
-        } else {
-            if ((b & 1) == 0) {
-                word_lo = *reinterpret_cast<const unsigned*>(scales + (b >> 1) * 64);
-                word_hi = *reinterpret_cast<const unsigned*>(scales + (b >> 1) * 64 + 32);
-            }
-            const unsigned s_lo = e4m3_pair(word_lo, which + (b & 1 ? 0x22u : 0u)), s_hi = e4m3_pair(word_hi, which + (b & 1 ? 0x22u : 0u));
+            acc[b & 1][0] = fmaf(s[0], scale_lo[b & 3], acc[b & 1][0]);
+            acc[b & 1][1] = fmaf(s[1], scale_lo[b & 3], acc[b & 1][1]);
+            acc[b & 1][2] = fmaf(s[2], scale_hi[b & 3], acc[b & 1][2]);
+            acc[b & 1][3] = fmaf(s[3], scale_hi[b & 3], acc[b & 1][3]);
+        }
+    } else {
+        // lane t: pieces t and t + 4 of a row, each two blocks of 16; their scales are one half of word (t + 4 q) / 2
+        const unsigned char* scales = base + Stage<kFormat>::kCodeBytes + (t >> 1) * 64 + g * 4 + (t & 1) * 2;
+        const int c_at = g * 128 + (piece_at<kFormat>(g, t) << 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = mul_f16x2(a[i], s_lo), c[i] = mul_f16x2(c[i], s_hi);
-            mma16816(acc, a[0], c[0], a[1], c[1], v.x, v.y);
-            mma16816(acc, a[2], c[2], a[3], c[3], v.z, v.w);
+        for (int q = 0; q < 2; ++q) {
+            const unsigned char* c_q = base + (c_at ^ (q << 6));  // piece t + 4 lies in the other half of the 128 bytes
+            const uint4 lo = *reinterpret_cast<const uint4*>(c_q);
+            const uint4 hi = *reinterpret_cast<const uint4*>(c_q + 8 * 128);
+            unsigned s_lo[2], s_hi[2];
+            e4m3_pairs(*reinterpret_cast<const unsigned short*>(scales + q * 128), s_lo[0], s_lo[1]);
+            e4m3_pairs(*reinterpret_cast<const unsigned short*>(scales + q * 128 + 32), s_hi[0], s_hi[1]);
+            const unsigned lo_w[4] = {lo.x, lo.y, lo.z, lo.w}, hi_w[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(v_at + q * 256 + i * 64);
+                unsigned a[4], c[4];
+                fp4_decode8(lo_w[i], a);
+                fp4_decode8(hi_w[i], c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = mul_f16x2(a[j], s_lo[i >> 1]), c[j] = mul_f16x2(c[j], s_hi[i >> 1]);
+                mma16816(acc[0], a[0], c[0], a[1], c[1], v.x, v.y);
+                mma16816(acc[1], a[2], c[2], a[3], c[3], v.z, v.w);
+            }
         }
     }
 }
 
 // The two projections differ in what a pass is, where values come from and what becomes of the sums; Work supplies these:
 //   begin(pass), next(pass)   the CTA's first pass, the one after: false when there is none
-//   expert(pass)              its active expert
 //   aim(rows, pass)           point the stream at the warp's rows
-//   load(pass, k, n)          8 values of the n-th slot from column k on, as they lie in memory
-//   finish(loaded)            the same in f16
-//   done(pass, here, acc)     a warp's sums, both halves of k
+//   load(piece, n, k)         8 values of slot n (of all slots) from column k on, as they lie in memory
+//   finish(piece)             the same in f16
+//   done(pass, here, tile, acc)  a warp's sums, both halves of k
 template <int kFormat, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -468,7 +518,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
     Pass ahead = at;
     bool ahead_more = true;
     int ahead_step = 0, ahead_slot = 0;
-    RowStream<kFormat, kStages> rows;
+    RowStream<kFormat> rows;
     work.aim(rows, ahead, tile);
     auto copy_next = [&] {
         if (ahead_more) {
@@ -477,33 +527,30 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
             if (++ahead_slot == kStages) ahead_slot = 0;
             if (++ahead_step == steps) {
                 ahead_step = 0;
-                const int item = ahead.item;
                 ahead_more = work.next(ahead);
-                if (ahead_more && ahead.item != item) work.aim(rows, ahead, tile);
+                if (ahead_more && ahead.first == 0) work.aim(rows, ahead, tile);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
+    // One copy of the code for each of these: unrolled, the loop outgrows the instruction cache (a third of all stalls).
+#pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) copy_next();
 
     Pass value_pass = at;
     bool value_more = true;
     int value_round = 0;
     typename Work::Piece pieces[kPieces];
-    auto slots_of = [&](const Pass& pass) {
-        const int e = work.active(pass);
-        return min(kTokenTile, routing.start[e + 1] - routing.start[e] - pass.first);
-    };
+    auto slots_of = [&](const Pass& pass) { return min(kTokenTile, routing.start[pass.active + 1] - routing.start[pass.active] - pass.first); };
     auto load_values = [&] {
         if (!value_more) return;
         const int here = slots_of(value_pass);
-        const short* slots = routing.slots + routing.start[work.active(value_pass)] + value_pass.first;
+        const int first = routing.start[value_pass.active] + value_pass.first;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * kThreads + static_cast<int>(threadIdx.x);
             const int n = piece / (kRoundK / 8);
-            if (n < here) work.load(pieces[i], slots[n], value_round * kRoundK + piece % (kRoundK / 8) * 8);
+            if (n < here) work.load(pieces[i], first + n, value_round * kRoundK + piece % (kRoundK / 8) * 8);
         }
     };
     auto store_values = [&](unsigned char* to) {
@@ -513,36 +560,40 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * kThreads + static_cast<int>(threadIdx.x);
             const int n = piece / (kRoundK / 8);
-            if (n < here) *reinterpret_cast<uint4*>(to + n * kValuePitch + piece % (kRoundK / 8) * 16) = work.finish(pieces[i]);
+            if (n < here) *reinterpret_cast<uint4*>(to + n * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16) = work.finish(pieces[i]);
         }
         if (++value_round == m.rounds) {
             value_round = 0;
             value_more = work.next(value_pass);
         }
     };
-    load_values();
-    store_values(values);
-    int buffer = 0, slot = 0;
-
+    int buffer = 1, slot = 0, round = -1;  // round -1: the first values only
+    float sums[2][4] = {};                 // two chains
     while (more) {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int round = 0; round < m.rounds; ++round) {
+#pragma unroll 1
+        for (; round < m.rounds; ++round) {
             __syncthreads();  // this round's values are there, nobody reads the other buffer any more
             load_values();
-#pragma unroll
+            if (round >= 0) {
+#pragma unroll 1
             for (int j = 0; j < kRoundSteps; ++j) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
                 __syncwarp();
                 copy_next();  // into the slot of the step before, which all lanes have left
                 const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
                 if (s < m.stages) {
-                    multiply_step<kFormat>(ring + slot * Stage<kFormat>::kBytes, values + buffer * kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), acc);
+                    multiply_step<kFormat>(ring + slot * Stage<kFormat>::kBytes, values + buffer * kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
                 }
                 if (++slot == kStages) slot = 0;
+            }
             }
             buffer ^= 1;
             store_values(values + buffer * kValueBytes);
         }
+        round = 0;
+        float acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = sums[0][i] + sums[1][i], sums[0][i] = sums[1][i] = 0.0f;
         if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         __syncthreads();
         if (half == 0) {
@@ -565,35 +616,40 @@ struct UpWork {
     const MoeParams& p;
     const Routing& routing;
     int groups;  // of 32 rows of G (and of U): four for every 128 rows begun
+    int skip_active, skip_groups;  // gridDim.x items further on
 
-    __device__ __forceinline__ bool begin(Pass& pass) const {
-        pass.item = blockIdx.x;
-        pass.first = 0;
-        return pass.item < routing.num_active * groups;
+    __device__ __forceinline__ UpWork(const MoeParams& params, const Routing& r) : p(params), routing(r), groups(params.f_groups / kTiles) {
+        skip_active = gridDim.x / groups;
+        skip_groups = gridDim.x - skip_active * groups;
     }
-    __device__ __forceinline__ int active(const Pass& pass) const { return pass.item / groups; }
-    __device__ __forceinline__ bool next(Pass& pass) const {
-        const int a = active(pass);
-        pass.first += kTokenTile;
-        if (pass.first < routing.start[a + 1] - routing.start[a]) return true;
+    __device__ __forceinline__ bool begin(Pass& pass) const {
+        pass.active = blockIdx.x / groups;
+        pass.group = blockIdx.x - pass.active * groups;
         pass.first = 0;
-        pass.item += gridDim.x;
-        return pass.item < routing.num_active * groups;
+        return pass.active < routing.num_active;
+    }
+    __device__ __forceinline__ bool next(Pass& pass) const {
+        pass.first += kTokenTile;
+        if (pass.first < routing.start[pass.active + 1] - routing.start[pass.active]) return true;
+        pass.first = 0;
+        pass.active += skip_active;
+        pass.group += skip_groups;
+        if (pass.group >= groups) pass.group -= groups, ++pass.active;
+        return pass.active < routing.num_active;
     }
     // Rows that share 32 bytes of scales: two neighbours in each of the four groups of 32 of a 128-row tile.
     __device__ __forceinline__ int row_in_f(const Pass& pass, int tile, int g) const {
-        const int group = pass.item % groups;
-        return (group >> 2) * 128 + 32 * (g >> 1) + 8 * (group & 3) + 2 * tile + (g & 1);
+        return (pass.group >> 2) * 128 + 32 * (g >> 1) + 8 * (pass.group & 3) + 2 * tile + (g & 1);
     }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
-        rows.aim(p.gate_up, routing.active[active(pass)], [&](int i) {
+        rows.aim(p.gate_up, routing.active[pass.active], [&](int i) {
             const int r = row_in_f(pass, tile, i & 7);
             return r >= p.f ? -1 : i < 8 ? r : p.f + r;
         });
     }
-    __device__ __forceinline__ void load(Piece& piece, int slot, int k) const {
-        const int token = slot / p.top_k;
+    __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
+        const int token = routing.tokens[n];
         const unsigned short* x = p.x + token * p.ldx + k;
         piece.shift = p.x_shift[token];
         if (p.x_vec && k + 8 <= p.d) {
@@ -615,16 +671,16 @@ struct UpWork {
     __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
         const int lane = threadIdx.x & 31;
         const int g = lane >> 2, t = lane & 3;
-        const int a = active(pass);
+        const int first = routing.start[pass.active] + pass.first;
         const int r = row_in_f(pass, tile, g);
-        const float scale = p.gate_up.tensor_scale != nullptr ? p.gate_up.tensor_scale[routing.active[a]] : 1.0f;
+        const float scale = p.gate_up.tensor_scale != nullptr ? p.gate_up.tensor_scale[routing.active[pass.active]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int n = 2 * t + j;
-            const int slot = n < here ? routing.slots[routing.start[a] + pass.first + n] : 0;
+            const int slot = n < here ? routing.slots[first + n] : 0;
             float h = 0.0f;
             if (n < here && r < p.f) {
-                const float back = inverse_power(p.x_shift[slot / p.top_k]) * scale;
+                const float back = inverse_power(p.x_shift[routing.tokens[first + n]]) * scale;
                 const float gate = acc[j] * back, up = acc[2 + j] * back;
                 h = gate / (1.0f + expf(-gate)) * up;
             }
@@ -635,7 +691,7 @@ struct UpWork {
                 const float shifted = h * power(shift_of(e));
                 if (r < p.f_pitch) p.h[static_cast<long long>(slot) * p.f_pitch + r] = static_cast<unsigned short>(pack_f16(shifted, 0.0f) & 0xffffu);
                 if (g == 0) {
-                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.item % groups * kTiles + tile] = static_cast<unsigned char>(e);
+                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.group * kTiles + tile] = static_cast<unsigned char>(e);
                     atomicMax(p.h_max + slot, e);
                 }
             }
@@ -658,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     load_routing(routing, reinterpret_cast<int*>(smem), p);
-    UpWork work{p, routing, p.f_groups / kTiles};
+    UpWork work(p, routing);
     run_passes<kFormat, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * kValueBytes, halves);
 }
 
@@ -675,29 +731,30 @@ struct DownWork {
     int first, step;
 
     __device__ __forceinline__ bool begin(Pass& pass) const {
-        pass.item = first;
+        pass.active = first;
+        pass.group = 0;
         pass.first = 0;
-        return pass.item < routing.num_active;
+        return pass.active < routing.num_active;
     }
-    __device__ __forceinline__ int active(const Pass& pass) const { return pass.item; }
     __device__ __forceinline__ bool next(Pass& pass) const {
         pass.first += kTokenTile;
-        if (pass.first < routing.start[pass.item + 1] - routing.start[pass.item]) return true;
+        if (pass.first < routing.start[pass.active + 1] - routing.start[pass.active]) return true;
         pass.first = 0;
-        pass.item += step;
-        return pass.item < routing.num_active;
+        pass.active += step;
+        return pass.active < routing.num_active;
     }
     // Row i of a tile: four neighbours in each group of 32, so that a warp uses 64 of 128 bytes of scales, the tile beside it the rest.
     __device__ __forceinline__ int row_in_y(int tile, int i) const { return (group >> 1) * 128 + 32 * (i >> 2) + 16 * (group & 1) + 4 * tile + (i & 3); }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
-        rows.aim(p.down, routing.active[pass.item], [&](int i) {
+        rows.aim(p.down, routing.active[pass.active], [&](int i) {
             const int r = row_in_y(tile, i);
             return r < p.d ? r : -1;
         });
     }
     // Columns k .. k + 7 are two rows each of four of the tiles that h came from.
-    __device__ __forceinline__ void load(Piece& piece, int slot, int k) const {
+    __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
+        const int slot = routing.slots[n];
         piece.largest = p.h_max[slot];
         if (k < p.f_pitch) {
             piece.raw = *reinterpret_cast<const uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
@@ -722,16 +779,17 @@ struct DownWork {
     __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
         const int lane = threadIdx.x & 31;
         const int g = lane >> 2, t = lane & 3;
-        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.item]] : 1.0f;
+        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.active]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int n = 2 * t + j;
             if (n < here) {
-                const int slot = routing.slots[routing.start[pass.item] + pass.first + n];
+                const int at = routing.start[pass.active] + pass.first + n;
+                const int slot = routing.slots[at];
                 const float back = power(-shift_of(p.h_max[slot])) * scale;
                 const float w = p.weights[slot];
                 // this warp's 16 columns; nobody else adds to them
-                float* sum = sums + slot / p.top_k * kDownPitch + tile * 16;
+                float* sum = sums + routing.tokens[at] * kDownPitch + tile * 16;
                 sum[g] += w * (acc[j] * back);
                 sum[g + 8] += w * (acc[2 + j] * back);
             }
