@@ -47,18 +47,28 @@ using namespace mcd;
 namespace {
 
 constexpr int kTokenTile = 8;        // columns of one mma
-constexpr int kTiles = 4;            // of 16 rows, per CTA
-constexpr int kHalves = 2;           // of the columns of a round
-constexpr int kThreads = kTiles * kHalves * 32;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
 constexpr int kStageK = 256;         // codes per row and step: 128 bytes
-constexpr int kRoundSteps = 2;       // per warp
-constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
-constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
-constexpr int kValueBytes = kTokenTile * kValuePitch;
-constexpr int kPieces = kTokenTile * kRoundK / 8 / kThreads;  // of 8 values, per thread and round
 constexpr int kMaxSlots = MCD_MOE_MAX_TOKENS * MCD_MOE_MAX_TOP_K;
-constexpr int kDownRows = kTiles * 16;
-constexpr int kDownPitch = kDownRows + 4;
+
+// How a CTA's warps divide their work: tiles of 16 rows, and halves of the columns of a round. With two halves there are
+// twice as many, shorter passes: for a few tokens, which could not occupy the SMs otherwise. With one, what a pass costs
+// beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns.
+template <int kHalves>
+struct Shape {
+    static constexpr int kTiles = kWarps / kHalves;
+    static constexpr int kRoundSteps = 4 / kHalves;  // per warp
+    static constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
+    static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
+    static constexpr int kValueBytes = kTokenTile * kValuePitch;
+    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kThreads;  // of 8 values, per thread and round
+    static constexpr int kUpGroups = 16 / kTiles;     // groups of rows of G (and of U) in 128
+    static constexpr int kDownGroups = 8 / kTiles;    // groups of rows of y in 128
+    static constexpr int kDownRows = kTiles * 16;
+    static constexpr int kDownPitch = kDownRows + 4;
+};
+
 constexpr int kRouterCluster = 8;
 constexpr int kRouterThreads = 256;
 constexpr int kUpStages = 4, kDownStages = 3;  // depth of a warp's ring; the down projection keeps sums beside it
@@ -75,7 +85,8 @@ struct Matrix4 {
     const unsigned char* scales;
     const float* tensor_scale;
     long long matrix_codes, matrix_scales, pitch;
-    int k_tiles, stages, rounds;  // per row
+    int k_tiles, stages;  // per row
+    int rounds;           // of a CTA's shape
 };
 
 struct MoeParams {
@@ -280,12 +291,56 @@ struct Routing {
     int num_active;
 };
 
-// `scratch`: an int per expert. Ends with a barrier.
+// `scratch`: an int per expert. Waits for the launch before this one; ends with a barrier.
 __device__ __forceinline__ void load_routing(Routing& r, int* scratch, const MoeParams& p) {
     const int all = p.tokens * p.top_k;
+    if (all <= 32) {
+        // One warp, without counting: a lane per slot, equal experts found by a vote.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (threadIdx.x < 32) {
+            const int lane = threadIdx.x;
+            const int e = lane < all ? p.chosen[lane] : 0x7fffffff;
+            const unsigned mine = __match_any_sync(0xffffffffu, e);
+            const bool first = lane < all && (mine & ((1u << lane) - 1u)) == 0;
+            const unsigned firsts = __ballot_sync(0xffffffffu, first);
+            int experts_before = 0, slots_before = 0;
+            for (unsigned left = firsts; left != 0; left &= left - 1) {
+                const int at = __ffs(left) - 1;
+                const int other = __shfl_sync(0xffffffffu, e, at);
+                const int count = __popc(__shfl_sync(0xffffffffu, mine, at));
+                if (other < e) ++experts_before, slots_before += count;
+            }
+            if (first) {
+                r.active[experts_before] = static_cast<short>(e);
+                r.start[experts_before] = static_cast<short>(slots_before);
+            }
+            if (lane < all) {
+                const int at = slots_before + __popc(mine & ((1u << lane) - 1u));
+                r.slots[at] = static_cast<short>(lane);
+                r.tokens[at] = static_cast<unsigned char>(lane / p.top_k);
+            }
+            if (lane == 0) {
+                r.num_active = __popc(firsts);
+                r.start[__popc(firsts)] = static_cast<short>(all);
+            }
+        }
+        __syncthreads();
+        return;
+    }
     for (int e = threadIdx.x; e < p.experts; e += kThreads) scratch[e] = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     __syncthreads();
-    for (int i = threadIdx.x; i < all; i += kThreads) atomicAdd(&scratch[p.chosen[i]], 1);
+    constexpr int kMost = kMaxSlots / kThreads;
+    int chosen[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int slot = i * kThreads + static_cast<int>(threadIdx.x);
+        chosen[i] = slot < all ? p.chosen[slot] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        if (chosen[i] >= 0) atomicAdd(&scratch[chosen[i]], 1);
+    }
     __syncthreads();
     if (threadIdx.x < 32) {
         int n = 0, slots = 0;
@@ -314,10 +369,13 @@ __device__ __forceinline__ void load_routing(Routing& r, int* scratch, const Moe
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < all; i += kThreads) {
-        const int at = atomicAdd(&scratch[p.chosen[i]], 1);
-        r.slots[at] = static_cast<short>(i);
-        r.tokens[at] = static_cast<unsigned char>(i / p.top_k);
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        if (chosen[i] < 0) continue;
+        const int slot = i * kThreads + static_cast<int>(threadIdx.x);
+        const int at = atomicAdd(&scratch[chosen[i]], 1);
+        r.slots[at] = static_cast<short>(slot);
+        r.tokens[at] = static_cast<unsigned char>(slot / p.top_k);
     }
     __syncthreads();
 }
@@ -337,69 +395,53 @@ __device__ __forceinline__ int piece_at(int row, int c) {
 }
 
 // Copies of a warp's 16 rows: four 16-byte pieces per lane and step (rows i * 4 + lane / 8), and the scale words of row
-// lane % 16.
+// lane % 16. The four rows of a lane lie (i & 1) * near + (i >> 1) * far bytes behind the first.
 template <int kFormat>
 struct RowStream {
-    const unsigned char* codes[4];   // at this lane's piece of the first step; any address where there is no such row
-    const unsigned char* scales;     // at this lane's first word
+    const unsigned char* codes;      // this lane's piece of its first row, first step
+    const unsigned char* scales;     // this lane's first word
+    long long near, far;
     unsigned there;                  // bit i: row i exists; all ones where every row of the tile does
-    int piece;                       // bytes from the start of a row
     int pitch, k_tiles;
-
-    // Rows of the tile: row_of(i) for i = 0 .. 15, negative where there is none.
-    template <typename RowOf>
-    __device__ __forceinline__ void aim(const Matrix4& m, int expert, RowOf&& row_of) {
-        const int lane = threadIdx.x & 31;
-        const unsigned char* matrix = m.codes + expert * m.matrix_codes;
-        piece = (lane & 7) * 16;
-        there = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = row_of(i * 4 + (lane >> 3));
-            codes[i] = matrix + max(r, 0) * m.pitch + piece;
-            there |= r >= 0 ? 1u << i : 0u;
-        }
-        if (__all_sync(0xffffffffu, there == 15u)) there = ~0u;
-        const int r = max(0, row_of(lane & 15));  // no such row: its sums go nowhere, any scale will do
-        scales = m.scales + expert * m.matrix_scales + fp4_scale_offset(r, 0, m.k_tiles) + (lane >> 4) * kFp4TileBytes;
-        pitch = static_cast<int>(m.pitch);
-        k_tiles = m.k_tiles;
-    }
 
     __device__ __forceinline__ void issue(int s, unsigned base) const {
         const int lane = threadIdx.x & 31;
-        const long long at = static_cast<long long>(s) * 128;
-        const long long scales_at = static_cast<long long>(s) * (Stage<kFormat>::kScaleWords * kFp4TileBytes);
+        const unsigned char* from = codes + static_cast<long long>(s) * 128;
+        const unsigned char* scales_from = scales + static_cast<long long>(s) * (Stage<kFormat>::kScaleWords * kFp4TileBytes);
         const unsigned dst = base + (lane >> 3) * 128;
         const unsigned scales_dst = base + Stage<kFormat>::kCodeBytes + lane * 4;
         // rows i * 4 + lane / 8: the swizzle goes by the row's low bits
         const unsigned even = dst + (piece_at<kFormat>(lane >> 3, lane & 7) << 4), odd = dst + (piece_at<kFormat>(4 + (lane >> 3), lane & 7) << 4);
-        if (there == ~0u && at + 128 <= pitch && (s + 1) * Stage<kFormat>::kScaleWords <= k_tiles) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((i & 1 ? odd : even) + i * 512), "l"(codes[i] + at) : "memory");
-            }
+        if (there == ~0u && (s + 1) * 128 <= pitch && (s + 1) * Stage<kFormat>::kScaleWords <= k_tiles) {
+            copy16(even, from);
+            copy16(odd + 512, from + near);
+            copy16(even + 1024, from + far);
+            copy16(odd + 1536, from + near + far);
 #pragma unroll
             for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_dst + i * 128), "l"(scales + scales_at + i * 2 * kFp4TileBytes) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_dst + i * 128), "l"(scales_from + i * 2 * kFp4TileBytes) : "memory");
             }
             return;
         }
         // the end of the rows, or rows that are not there: zeros
+        const unsigned char* anywhere = scales - (lane >> 4) * kFp4TileBytes;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool real = ((there >> i) & 1u) != 0 && at + piece < pitch;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((i & 1 ? odd : even) + i * 512), "l"(real ? codes[i] + at : scales - (lane >> 4) * kFp4TileBytes),
-                         "r"(real ? 16 : 0)
+            const bool real = ((there >> i) & 1u) != 0 && s * 128 + (lane & 7) * 16 < pitch;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((i & 1 ? odd : even) + i * 512),
+                         "l"(real ? from + (i & 1) * near + (i >> 1) * far : anywhere), "r"(real ? 16 : 0)
                          : "memory");
         }
 #pragma unroll
         for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
             const bool real = s * Stage<kFormat>::kScaleWords + i * 2 + (lane >> 4) < k_tiles;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_dst + i * 128),
-                         "l"(real ? scales + scales_at + i * 2 * kFp4TileBytes : scales - (lane >> 4) * kFp4TileBytes), "r"(real ? 4 : 0)
+                         "l"(real ? scales_from + i * 2 * kFp4TileBytes : anywhere), "r"(real ? 4 : 0)
                          : "memory");
         }
+    }
+    static __device__ __forceinline__ void copy16(unsigned dst, const void* src) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     }
 };
 
@@ -440,7 +482,7 @@ __device__ __forceinline__ int value_piece(int k) {
 }
 
 // One step: 16 rows x 256 codes at `base` times the values at `values` (f16, token rows kValuePitch apart).
-template <int kFormat>
+template <int kFormat, int kValuePitch>
 __device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[2][4]) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -499,12 +541,14 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 
 // The two projections differ in what a pass is, where values come from and what becomes of the sums; Work supplies these:
 //   begin(pass), next(pass)   the CTA's first pass, the one after: false when there is none
-//   aim(rows, pass)           point the stream at the warp's rows
+//   stride(rows), aim(rows, pass, tile)  point the stream at the warp's rows
 //   load(piece, n, k)         8 values of slot n (of all slots) from column k on, as they lie in memory
 //   finish(piece)             the same in f16
 //   done(pass, here, tile, acc)  a warp's sums, both halves of k
-template <int kFormat, int kStages, typename Work>
+template <int kFormat, int kHalves, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
+    using S = Shape<kHalves>;
+    constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kPieces = S::kPieces, kValuePitch = S::kValuePitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile = warp % kTiles, half = warp / kTiles;
     unsigned char* ring = rings + warp * kStages * Stage<kFormat>::kBytes;
@@ -519,6 +563,9 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
     bool ahead_more = true;
     int ahead_step = 0, ahead_slot = 0;
     RowStream<kFormat> rows;
+    rows.pitch = static_cast<int>(m.pitch);
+    rows.k_tiles = m.k_tiles;
+    work.stride(rows);
     work.aim(rows, ahead, tile);
     auto copy_next = [&] {
         if (ahead_more) {
@@ -582,25 +629,27 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
                 copy_next();  // into the slot of the step before, which all lanes have left
                 const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
                 if (s < m.stages) {
-                    multiply_step<kFormat>(ring + slot * Stage<kFormat>::kBytes, values + buffer * kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
+                    multiply_step<kFormat, kValuePitch>(ring + slot * Stage<kFormat>::kBytes, values + buffer * S::kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
                 }
                 if (++slot == kStages) slot = 0;
             }
             }
             buffer ^= 1;
-            store_values(values + buffer * kValueBytes);
+            store_values(values + buffer * S::kValueBytes);
         }
         round = 0;
         float acc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = sums[0][i] + sums[1][i], sums[0][i] = sums[1][i] = 0.0f;
-        if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        __syncthreads();
-        if (half == 0) {
-            const float4 other = halves[tile * 32 + lane];
-            acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
-            work.done(at, slots_of(at), tile, acc);
+        if constexpr (kHalves == 2) {
+            if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            __syncthreads();
+            if (half == 0) {
+                const float4 other = halves[tile * 32 + lane];
+                acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
+            }
         }
+        if (half == 0) work.done(at, slots_of(at), tile, acc);
         more = work.next(at);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -608,17 +657,19 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
 
 // -------------------------------------------------------------------------------------------------------- up and down
 
+template <int kHalves>
 struct UpWork {
+    using S = Shape<kHalves>;
     struct Piece {
         uint4 raw;
         float shift;
     };
     const MoeParams& p;
     const Routing& routing;
-    int groups;  // of 32 rows of G (and of U): four for every 128 rows begun
+    int groups;                    // of rows of an expert
     int skip_active, skip_groups;  // gridDim.x items further on
 
-    __device__ __forceinline__ UpWork(const MoeParams& params, const Routing& r) : p(params), routing(r), groups(params.f_groups / kTiles) {
+    __device__ __forceinline__ UpWork(const MoeParams& params, const Routing& r) : p(params), routing(r), groups(params.f_groups / S::kTiles) {
         skip_active = gridDim.x / groups;
         skip_groups = gridDim.x - skip_active * groups;
     }
@@ -639,14 +690,24 @@ struct UpWork {
     }
     // Rows that share 32 bytes of scales: two neighbours in each of the four groups of 32 of a 128-row tile.
     __device__ __forceinline__ int row_in_f(const Pass& pass, int tile, int g) const {
-        return (pass.group >> 2) * 128 + 32 * (g >> 1) + 8 * (pass.group & 3) + 2 * tile + (g & 1);
+        return pass.group / S::kUpGroups * 128 + 32 * (g >> 1) + 2 * S::kTiles * (pass.group % S::kUpGroups) + 2 * tile + (g & 1);
+    }
+    // Rows 0 .. 7 of a tile are G's, 8 .. 15 the same of U.
+    template <typename Rows>
+    __device__ __forceinline__ void stride(Rows& rows) const {
+        rows.near = 64 * p.gate_up.pitch;
+        rows.far = p.f * p.gate_up.pitch;
     }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
-        rows.aim(p.gate_up, routing.active[pass.active], [&](int i) {
-            const int r = row_in_f(pass, tile, i & 7);
-            return r >= p.f ? -1 : i < 8 ? r : p.f + r;
-        });
+        const int lane = threadIdx.x & 31;
+        const int expert = routing.active[pass.active];
+        const int r = row_in_f(pass, tile, lane >> 3);
+        rows.codes = p.gate_up.codes + expert * p.gate_up.matrix_codes + r * p.gate_up.pitch + (lane & 7) * 16;
+        rows.there = (r < p.f ? 5u : 0u) | (r + 64 < p.f ? 10u : 0u);
+        if (__all_sync(0xffffffffu, rows.there == 15u)) rows.there = ~0u;
+        const int q = min(row_in_f(pass, tile, lane & 7), p.f - 1) + (lane & 8 ? p.f : 0);  // no such row: its sums go nowhere, any scale will do
+        rows.scales = p.gate_up.scales + expert * p.gate_up.matrix_scales + fp4_scale_offset(q, 0, p.gate_up.k_tiles) + (lane >> 4) * kFp4TileBytes;
     }
     __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
         const int token = routing.tokens[n];
@@ -682,7 +743,7 @@ struct UpWork {
             if (n < here && r < p.f) {
                 const float back = inverse_power(p.x_shift[routing.tokens[first + n]]) * scale;
                 const float gate = acc[j] * back, up = acc[2 + j] * back;
-                h = gate / (1.0f + expf(-gate)) * up;
+                h = __fdividef(gate, 1.0f + expf(-gate)) * up;
             }
             int e = static_cast<int>((__float_as_uint(h) >> 23) & 0xffu);
 #pragma unroll
@@ -691,7 +752,7 @@ struct UpWork {
                 const float shifted = h * power(shift_of(e));
                 if (r < p.f_pitch) p.h[static_cast<long long>(slot) * p.f_pitch + r] = static_cast<unsigned short>(pack_f16(shifted, 0.0f) & 0xffffu);
                 if (g == 0) {
-                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.group * kTiles + tile] = static_cast<unsigned char>(e);
+                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.group * S::kTiles + tile] = static_cast<unsigned char>(e);
                     atomicMax(p.h_max + slot, e);
                 }
             }
@@ -700,25 +761,27 @@ struct UpWork {
 };
 
 template <int kFormat>
-constexpr int ring_bytes(int stages) { return kTiles * kHalves * stages * Stage<kFormat>::kBytes; }
+constexpr int ring_bytes(int stages) { return kWarps * stages * Stage<kFormat>::kBytes; }
+template <int kFormat, int kHalves>
+constexpr int kUpSmem = 2 * Shape<kHalves>::kValueBytes + ring_bytes<kFormat>(kUpStages);
 template <int kFormat>
-constexpr int kUpSmem = 2 * kValueBytes + ring_bytes<kFormat>(kUpStages);
-template <int kFormat>
-constexpr int kDownSmem = MCD_MOE_MAX_TOKENS * kDownPitch * 4 + 2 * kValueBytes + ring_bytes<kFormat>(kDownStages);
+constexpr int down_smem(int tokens) {
+    return tokens * Shape<2>::kDownPitch * 4 + 2 * Shape<2>::kValueBytes + ring_bytes<kFormat>(kDownStages);
+}
 
-template <int kFormat>
+template <int kFormat, int kHalves>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
-    __shared__ float4 halves[kTiles * 32];
+    __shared__ float4 halves[kWarps / 2 * 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     load_routing(routing, reinterpret_cast<int*>(smem), p);
-    UpWork work(p, routing);
-    run_passes<kFormat, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * kValueBytes, halves);
+    UpWork<kHalves> work(p, routing);
+    run_passes<kFormat, kHalves, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves>::kValueBytes, halves);
 }
 
 struct DownWork {
+    using S = Shape<2>;
     struct Piece {
         uint4 raw;
         unsigned exponents;
@@ -727,7 +790,7 @@ struct DownWork {
     const MoeParams& p;
     const Routing& routing;
     float* sums;  // [tokens][kDownPitch]
-    int group;    // 64 rows of y: one half of the 16 rows in each group of 32 of a 128-row tile
+    int group;    // of rows of y: their share of each group of 32 of a 128-row tile
     int first, step;
 
     __device__ __forceinline__ bool begin(Pass& pass) const {
@@ -744,13 +807,24 @@ struct DownWork {
         return pass.active < routing.num_active;
     }
     // Row i of a tile: four neighbours in each group of 32, so that a warp uses 64 of 128 bytes of scales, the tile beside it the rest.
-    __device__ __forceinline__ int row_in_y(int tile, int i) const { return (group >> 1) * 128 + 32 * (i >> 2) + 16 * (group & 1) + 4 * tile + (i & 3); }
+    __device__ __forceinline__ int row_in_y(int tile, int i) const {
+        return group / S::kDownGroups * 128 + 32 * (i >> 2) + 4 * S::kTiles * (group % S::kDownGroups) + 4 * tile + (i & 3);
+    }
+    template <typename Rows>
+    __device__ __forceinline__ void stride(Rows& rows) const {
+        rows.near = 32 * p.down.pitch;
+        rows.far = 64 * p.down.pitch;
+    }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
-        rows.aim(p.down, routing.active[pass.active], [&](int i) {
-            const int r = row_in_y(tile, i);
-            return r < p.d ? r : -1;
-        });
+        const int lane = threadIdx.x & 31;
+        const int expert = routing.active[pass.active];
+        const int r = row_in_y(tile, lane >> 3);
+        rows.codes = p.down.codes + expert * p.down.matrix_codes + r * p.down.pitch + (lane & 7) * 16;
+        rows.there = (r < p.d ? 1u : 0u) | (r + 32 < p.d ? 2u : 0u) | (r + 64 < p.d ? 4u : 0u) | (r + 96 < p.d ? 8u : 0u);
+        if (__all_sync(0xffffffffu, rows.there == 15u)) rows.there = ~0u;
+        const int q = min(row_in_y(tile, lane & 15), p.d - 1);  // no such row: its sums go nowhere, any scale will do
+        rows.scales = p.down.scales + expert * p.down.matrix_scales + fp4_scale_offset(q, 0, p.down.k_tiles) + (lane >> 4) * kFp4TileBytes;
     }
     // Columns k .. k + 7 are two rows each of four of the tiles that h came from.
     __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
@@ -789,7 +863,7 @@ struct DownWork {
                 const float back = power(-shift_of(p.h_max[slot])) * scale;
                 const float w = p.weights[slot];
                 // this warp's 16 columns; nobody else adds to them
-                float* sum = sums + routing.tokens[at] * kDownPitch + tile * 16;
+                float* sum = sums + routing.tokens[at] * S::kDownPitch + tile * 16;
                 sum[g] += w * (acc[j] * back);
                 sum[g + 8] += w * (acc[2 + j] * back);
             }
@@ -799,19 +873,20 @@ struct DownWork {
 
 template <int kFormat>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
+    using S = Shape<2>;
+    constexpr int kDownRows = S::kDownRows, kDownPitch = S::kDownPitch;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
-    __shared__ float4 halves[kTiles * 32];
-    float* sums = reinterpret_cast<float*>(smem);
-    unsigned char* values = smem + MCD_MOE_MAX_TOKENS * kDownPitch * 4;
+    __shared__ float4 halves[kWarps / 2 * 32];
+    unsigned char* values = smem;
+    unsigned char* rings = values + 2 * S::kValueBytes;
+    float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kDownStages));
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int group = blockIdx.x / cluster;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    load_routing(routing, reinterpret_cast<int*>(values), p);
     for (int i = threadIdx.x; i < p.tokens * kDownPitch; i += kThreads) sums[i] = 0.0f;
-    __syncthreads();
+    load_routing(routing, reinterpret_cast<int*>(values), p);
     DownWork work{p, routing, sums, group, rank, cluster};
-    run_passes<kFormat, kDownStages>(work, p.down, routing, values, values + 2 * kValueBytes, halves);
+    run_passes<kFormat, 2, kDownStages>(work, p.down, routing, values, rings, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
     // Every CTA of the cluster finishes its share of the elements: the partial sums in rank order.
@@ -866,29 +941,47 @@ int launch(void (*kernel)(Params...), unsigned grid, unsigned cluster, unsigned 
     return check_rt(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
 
-template <int kFormat>
-int launch_layer(const MoeParams& p, cudaStream_t s) {
-    static PerDeviceOnce configured;
+template <typename Kernel>
+int ready(PerDeviceOnce& once, Kernel kernel, int smem) {
     int device = 0;
     if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
-    if (configured.first_use(device)) {
-        cudaError_t err = cudaFuncSetAttribute(mc_moe_up<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, kUpSmem<kFormat>);
-        if (err == cudaSuccess) err = cudaFuncSetAttribute(mc_moe_down<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDownSmem<kFormat>);
-        if (int rc = check_rt(err, "cudaFuncSetAttribute(max dynamic shared memory)")) {
-            configured.forget(device);
-            return rc;
-        }
-    }
+    if (!once.first_use(device)) return 0;
+    const int rc = check_rt(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(max dynamic shared memory)");
+    if (rc != 0) once.forget(device);
+    return rc;
+}
+
+template <int kFormat, int kHalves>
+int launch_up(MoeParams p, int reached, cudaStream_t s) {
+    using S = Shape<kHalves>;
+    static PerDeviceOnce once;
+    if (int rc = ready(once, mc_moe_up<kFormat, kHalves>, kUpSmem<kFormat, kHalves>)) return rc;
+    p.gate_up.rounds = (p.d + S::kRoundK - 1) / S::kRoundK;
+    const long long items = static_cast<long long>(reached) * (p.f_groups / S::kTiles);
+    const auto grid = static_cast<unsigned>(std::min<long long>(items, 2LL * sm_count()));
+    return launch(mc_moe_up<kFormat, kHalves>, grid, 1, kThreads, kUpSmem<kFormat, kHalves>, s, "mc_moe_up", p);
+}
+
+template <int kFormat>
+int launch_down(MoeParams p, int reached, cudaStream_t s) {
+    using S = Shape<2>;
+    static PerDeviceOnce once;
+    if (int rc = ready(once, mc_moe_down<kFormat>, down_smem<kFormat>(MCD_MOE_MAX_TOKENS))) return rc;
+    p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
+    int cluster = 8;
+    while (cluster > reached) cluster /= 2;
+    const auto grid = static_cast<unsigned>((p.d + 127) / 128 * S::kDownGroups * cluster);
+    return launch(mc_moe_down<kFormat>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat>(p.tokens), s, "mc_moe_down", p, cluster);
+}
+
+template <int kFormat>
+int launch_layer(const MoeParams& p, cudaStream_t s) {
     // The router's clusters are declared with the kernel.
     if (int rc = launch(mc_moe_router, static_cast<unsigned>(p.tokens * kRouterCluster), 1, kRouterThreads, 0, s, "mc_moe_router", p)) return rc;
     const int reached = std::min(p.experts, p.tokens * p.top_k);
-    const long long most = static_cast<long long>(reached) * (p.f_groups / kTiles);
-    const auto up_grid = static_cast<unsigned>(std::min<long long>(most, 2LL * sm_count()));
-    if (int rc = launch(mc_moe_up<kFormat>, up_grid, 1, kThreads, kUpSmem<kFormat>, s, "mc_moe_up", p)) return rc;
-    int cluster = 8;
-    while (cluster > reached) cluster /= 2;
-    const auto down_grid = static_cast<unsigned>((p.d + 127) / 128 * 2 * cluster);
-    return launch(mc_moe_down<kFormat>, down_grid, static_cast<unsigned>(cluster), kThreads, kDownSmem<kFormat>, s, "mc_moe_down", p, cluster);
+    const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2>::kTiles) > 4LL * sm_count();
+    if (int rc = many ? launch_up<kFormat, 1>(p, reached, s) : launch_up<kFormat, 2>(p, reached, s)) return rc;
+    return launch_down<kFormat>(p, reached, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -907,7 +1000,7 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
     m.pitch = geo.pitch;
     m.k_tiles = static_cast<int>(geo.k_tiles);
     m.stages = static_cast<int>((t.cols + kStageK - 1) / kStageK);
-    m.rounds = static_cast<int>((t.cols + kRoundK - 1) / kRoundK);
+    m.rounds = 0;
     return m;
 }
 
