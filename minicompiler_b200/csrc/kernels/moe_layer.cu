@@ -63,12 +63,14 @@ struct Shape {
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
     static constexpr int kValueBytes = kTokenTile * kValuePitch;
     static constexpr int kPieces = kTokenTile * kRoundK / 8 / kThreads;  // of 8 values, per thread and round
-    static constexpr int kUpGroups = 16 / kTiles;     // groups of rows of G (and of U) in 128
-    static constexpr int kDownGroups = 8 / kTiles;    // groups of rows of y in 128
-    static constexpr int kDownRows = kTiles * 16;
-    static constexpr int kDownPitch = kDownRows + 4;
+    static constexpr int kUpGroups = 16 / kTiles;  // groups of rows of G (and of U) in 128
 };
 
+// The down projection always works in two halves (whole rows left it 128 CTAs of 2048 rows' worth, 160 against 136 us for
+// 32 tokens of a layer of 128 experts).
+constexpr int kDownGroups = 2;  // groups of rows of y in 128
+constexpr int kDownRows = 128 / kDownGroups;
+constexpr int kDownPitch = kDownRows + 4;
 constexpr int kRouterCluster = 8;
 constexpr int kRouterThreads = 256;
 constexpr int kUpStages = 4, kDownStages = 3;  // depth of a warp's ring; the down projection keeps sums beside it
@@ -96,10 +98,9 @@ struct MoeParams {
     long long ldx, ld_router, ldy;
     int type, tokens, top_k, renormalize, experts;
     int d, f;
-    int f_pitch;     // f in whole groups of 8
+    int d_pitch, f_pitch;  // in whole groups of 8
     int f_groups;    // tiles of 8 rows of h: 16 for every 128 rows begun
-    int x_vec;       // rows of x start on 16-byte boundaries
-    int router_vec;  // rows of x and of the router do
+    int router_vec;  // rows of x and of the router start on 16-byte boundaries
     Matrix4 gate_up, down;
     int* chosen_out;
     float* weights_out;
@@ -108,6 +109,7 @@ struct MoeParams {
     float* weights;           // [tokens * top_k]
     int* h_max;               // [tokens * top_k]: the largest of h_exponent
     float* x_shift;           // [tokens]: the power of two that x is multiplied with
+    unsigned short* x16;      // [tokens][d_pitch]: x in f16 after that
     unsigned char* h_exponent;  // [tokens * top_k][f_groups]: f32 exponent of the largest |h| among a tile's rows
     unsigned short* h;        // [tokens * top_k][f_pitch]: f16 after shift_for of that exponent
 };
@@ -224,11 +226,19 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
         }
         if (e < p.experts && lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(total) : "memory");
     }
+    // Every CTA of the cluster finds the token's largest magnitude and brings its share of x to f16.
     unsigned largest = 0;
+    for (int c = threadIdx.x; c < p.d; c += kRouterThreads) largest = max(largest, __float_as_uint(value16(x[c], p.type)) & 0x7fffffffu);
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0) warp_max[warp] = largest;
+    __syncthreads();
+    for (int w = 0; w < kRouterThreads / 32; ++w) largest = max(largest, warp_max[w]);
+    const float shift = power(shift_of(static_cast<int>(largest >> 23)));
+    for (int c = static_cast<int>(rank) * kRouterThreads + static_cast<int>(threadIdx.x); c < p.d_pitch; c += kRouterCluster * kRouterThreads) {
+        p.x16[token * static_cast<long long>(p.d_pitch) + c] = static_cast<unsigned short>(c < p.d ? pack_f16(value16(x[c], p.type) * shift, 0.0f) & 0xffffu : 0u);
+    }
     if (rank == 0) {
-        for (int c = threadIdx.x; c < p.d; c += kRouterThreads) largest = max(largest, __float_as_uint(value16(x[c], p.type)) & 0x7fffffffu);
-        largest = __reduce_max_sync(0xffffffffu, largest);
-        if (lane == 0) warp_max[warp] = largest;
+        if (threadIdx.x == 0) p.x_shift[token] = shift;
         for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) order[e] = 0;
         if (threadIdx.x < p.top_k) p.h_max[token * p.top_k + threadIdx.x] = 0;
     }
@@ -236,10 +246,6 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     if (rank != 0) return;
 
     for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) keys[e] = sort_key(logits[e]);
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kRouterThreads / 32; ++w) largest = max(largest, warp_max[w]);
-        p.x_shift[token] = power(shift_of(static_cast<int>(largest >> 23)));
-    }
     __syncthreads();
     // An expert's place is the number of experts that come before it: the larger logit, ties to the lower index. Several
     // threads share the comparisons of one expert where there are fewer than threads.
@@ -395,53 +401,39 @@ __device__ __forceinline__ int piece_at(int row, int c) {
 }
 
 // Copies of a warp's 16 rows: four 16-byte pieces per lane and step (rows i * 4 + lane / 8), and the scale words of row
-// lane % 16. The four rows of a lane lie (i & 1) * near + (i >> 1) * far bytes behind the first.
+// lane % 16. Nothing is tested on the way: behind the end of a row its last piece comes again, where the values it meets
+// are 0 (and its scales are the row's own, so a NaN among them belongs to the row); for a row that is not there another
+// one comes, whose sums go nowhere. The copies carry no memory clobber, so that their arithmetic is scheduled among that
+// of the multiplies behind them; they write a slot of the ring that nothing else touches until the next wait.
 template <int kFormat>
 struct RowStream {
-    const unsigned char* codes;      // this lane's piece of its first row, first step
-    const unsigned char* scales;     // this lane's first word
-    long long near, far;
-    unsigned there;                  // bit i: row i exists; all ones where every row of the tile does
-    int pitch, k_tiles;
+    const unsigned char* codes;      // this lane's first row
+    const unsigned char* scales;     // of this lane's row, first tile
+    long long offset[3];             // of its other rows
+    int last_piece, last_tile;
 
-    __device__ __forceinline__ void issue(int s, unsigned base) const {
+    // `wanted` false: zeros instead, and nothing is read.
+    __device__ __forceinline__ void issue(int s, unsigned base, bool wanted) const {
         const int lane = threadIdx.x & 31;
-        const unsigned char* from = codes + static_cast<long long>(s) * 128;
-        const unsigned char* scales_from = scales + static_cast<long long>(s) * (Stage<kFormat>::kScaleWords * kFp4TileBytes);
+        const unsigned char* from = codes + min(s * 128 + (lane & 7) * 16, last_piece);
         const unsigned dst = base + (lane >> 3) * 128;
-        const unsigned scales_dst = base + Stage<kFormat>::kCodeBytes + lane * 4;
         // rows i * 4 + lane / 8: the swizzle goes by the row's low bits
         const unsigned even = dst + (piece_at<kFormat>(lane >> 3, lane & 7) << 4), odd = dst + (piece_at<kFormat>(4 + (lane >> 3), lane & 7) << 4);
-        if (there == ~0u && (s + 1) * 128 <= pitch && (s + 1) * Stage<kFormat>::kScaleWords <= k_tiles) {
-            copy16(even, from);
-            copy16(odd + 512, from + near);
-            copy16(even + 1024, from + far);
-            copy16(odd + 1536, from + near + far);
-#pragma unroll
-            for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_dst + i * 128), "l"(scales_from + i * 2 * kFp4TileBytes) : "memory");
-            }
-            return;
-        }
-        // the end of the rows, or rows that are not there: zeros
-        const unsigned char* anywhere = scales - (lane >> 4) * kFp4TileBytes;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool real = ((there >> i) & 1u) != 0 && s * 128 + (lane & 7) * 16 < pitch;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((i & 1 ? odd : even) + i * 512),
-                         "l"(real ? from + (i & 1) * near + (i >> 1) * far : anywhere), "r"(real ? 16 : 0)
-                         : "memory");
-        }
+        const int bytes = wanted ? 16 : 0;
+        copy16(even, from, bytes);
+        copy16(odd + 512, from + offset[0], bytes);
+        copy16(even + 1024, from + offset[1], bytes);
+        copy16(odd + 1536, from + offset[2], bytes);
+        const unsigned scales_dst = base + Stage<kFormat>::kCodeBytes + lane * 4;
 #pragma unroll
         for (int i = 0; i < Stage<kFormat>::kScaleWords / 2; ++i) {
-            const bool real = s * Stage<kFormat>::kScaleWords + i * 2 + (lane >> 4) < k_tiles;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_dst + i * 128),
-                         "l"(real ? scales_from + i * 2 * kFp4TileBytes : anywhere), "r"(real ? 4 : 0)
-                         : "memory");
+            const int tile = min(s * Stage<kFormat>::kScaleWords + i * 2 + (lane >> 4), last_tile);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_dst + i * 128), "l"(scales + static_cast<long long>(tile) * kFp4TileBytes),
+                         "r"(bytes >> 2));
         }
     }
-    static __device__ __forceinline__ void copy16(unsigned dst, const void* src) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    static __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
     }
 };
 
@@ -541,10 +533,11 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 
 // The two projections differ in what a pass is, where values come from and what becomes of the sums; Work supplies these:
 //   begin(pass), next(pass)   the CTA's first pass, the one after: false when there is none
-//   stride(rows), aim(rows, pass, tile)  point the stream at the warp's rows
+//   aim(rows, pass, tile)     point the stream at the warp's rows
 //   load(piece, n, k)         8 values of slot n (of all slots) from column k on, as they lie in memory
 //   finish(piece)             the same in f16
-//   done(pass, here, tile, acc)  a warp's sums, both halves of k
+//   look(pass, here)          what a lane will need of its two columns, read before the multiplies
+//   done(pass, here, tile, side, acc)  a warp's sums, both halves of k
 template <int kFormat, int kHalves, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
     using S = Shape<kHalves>;
@@ -563,26 +556,26 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
     bool ahead_more = true;
     int ahead_step = 0, ahead_slot = 0;
     RowStream<kFormat> rows;
-    rows.pitch = static_cast<int>(m.pitch);
-    rows.k_tiles = m.k_tiles;
-    work.stride(rows);
+    rows.last_piece = static_cast<int>(m.pitch) - 16;
+    rows.last_tile = m.k_tiles - 1;
     work.aim(rows, ahead, tile);
     auto copy_next = [&] {
-        if (ahead_more) {
-            const int s = (ahead_step / kRoundSteps) * (kRoundSteps * kHalves) + half * kRoundSteps + ahead_step % kRoundSteps;
-            if (s < m.stages) rows.issue(s, ring_at + static_cast<unsigned>(ahead_slot * Stage<kFormat>::kBytes));
-            if (++ahead_slot == kStages) ahead_slot = 0;
-            if (++ahead_step == steps) {
-                ahead_step = 0;
-                ahead_more = work.next(ahead);
-                if (ahead_more && ahead.first == 0) work.aim(rows, ahead, tile);
-            }
+        const int s = (ahead_step / kRoundSteps) * (kRoundSteps * kHalves) + half * kRoundSteps + ahead_step % kRoundSteps;
+        rows.issue(s, ring_at + static_cast<unsigned>(ahead_slot * Stage<kFormat>::kBytes), ahead_more && s < m.stages);
+        if (++ahead_slot == kStages) ahead_slot = 0;
+        if (++ahead_step == steps) {
+            ahead_step = 0;
+            if (ahead_more) ahead_more = work.next(ahead);
+            if (ahead_more && ahead.first == 0) work.aim(rows, ahead, tile);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto copies_end = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     // One copy of the code for each of these: unrolled, the loop outgrows the instruction cache (a third of all stalls).
 #pragma unroll 1
-    for (int i = 0; i < kStages - 1; ++i) copy_next();
+    for (int i = 0; i < kStages - 1; ++i) {
+        copy_next();
+        copies_end();
+    }
 
     Pass value_pass = at;
     bool value_more = true;
@@ -617,6 +610,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
     int buffer = 1, slot = 0, round = -1;  // round -1: the first values only
     float sums[2][4] = {};                 // two chains
     while (more) {
+        const typename Work::Side side = work.look(at, slots_of(at));
 #pragma unroll 1
         for (; round < m.rounds; ++round) {
             __syncthreads();  // this round's values are there, nobody reads the other buffer any more
@@ -631,6 +625,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
                 if (s < m.stages) {
                     multiply_step<kFormat, kValuePitch>(ring + slot * Stage<kFormat>::kBytes, values + buffer * S::kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
                 }
+                copies_end();
                 if (++slot == kStages) slot = 0;
             }
             }
@@ -649,7 +644,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
                 acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
             }
         }
-        if (half == 0) work.done(at, slots_of(at), tile, acc);
+        if (half == 0) work.done(at, slots_of(at), tile, side, acc);
         more = work.next(at);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -660,10 +655,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
 template <int kHalves>
 struct UpWork {
     using S = Shape<kHalves>;
-    struct Piece {
-        uint4 raw;
-        float shift;
-    };
+    using Piece = uint4;
     const MoeParams& p;
     const Routing& routing;
     int groups;                    // of rows of an expert
@@ -694,55 +686,49 @@ struct UpWork {
     }
     // Rows 0 .. 7 of a tile are G's, 8 .. 15 the same of U.
     template <typename Rows>
-    __device__ __forceinline__ void stride(Rows& rows) const {
-        rows.near = 64 * p.gate_up.pitch;
-        rows.far = p.f * p.gate_up.pitch;
-    }
-    template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
         const int lane = threadIdx.x & 31;
         const int expert = routing.active[pass.active];
-        const int r = row_in_f(pass, tile, lane >> 3);
-        rows.codes = p.gate_up.codes + expert * p.gate_up.matrix_codes + r * p.gate_up.pitch + (lane & 7) * 16;
-        rows.there = (r < p.f ? 5u : 0u) | (r + 64 < p.f ? 10u : 0u);
-        if (__all_sync(0xffffffffu, rows.there == 15u)) rows.there = ~0u;
-        const int q = min(row_in_f(pass, tile, lane & 7), p.f - 1) + (lane & 8 ? p.f : 0);  // no such row: its sums go nowhere, any scale will do
-        rows.scales = p.gate_up.scales + expert * p.gate_up.matrix_scales + fp4_scale_offset(q, 0, p.gate_up.k_tiles) + (lane >> 4) * kFp4TileBytes;
+        const int r = min(row_in_f(pass, tile, lane >> 3), p.f - 1);
+        rows.codes = p.gate_up.codes + expert * p.gate_up.matrix_codes + r * p.gate_up.pitch;
+        rows.offset[0] = r + 64 < p.f ? 64 * p.gate_up.pitch : 0;
+        rows.offset[1] = p.f * p.gate_up.pitch;
+        rows.offset[2] = rows.offset[0] + rows.offset[1];
+        const int q = min(row_in_f(pass, tile, lane & 7), p.f - 1) + (lane & 8 ? p.f : 0);
+        rows.scales = p.gate_up.scales + expert * p.gate_up.matrix_scales + fp4_scale_offset(q, 0, p.gate_up.k_tiles);
     }
     __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
-        const int token = routing.tokens[n];
-        const unsigned short* x = p.x + token * p.ldx + k;
-        piece.shift = p.x_shift[token];
-        if (p.x_vec && k + 8 <= p.d) {
-            piece.raw = *reinterpret_cast<const uint4*>(x);
-        } else {
-            unsigned v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + j < p.d ? x[j] : 0u;
-            piece.raw = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-        }
+        piece = make_uint4(0, 0, 0, 0);
+        if (k < p.d_pitch) piece = *reinterpret_cast<const uint4*>(p.x16 + routing.tokens[n] * static_cast<long long>(p.d_pitch) + k);
     }
-    __device__ __forceinline__ uint4 finish(const Piece& piece) const {
-        const unsigned w[4] = {piece.raw.x, piece.raw.y, piece.raw.z, piece.raw.w};
-        unsigned v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = pack_f16(value16(w[j] & 0xffffu, p.type) * piece.shift, value16(w[j] >> 16, p.type) * piece.shift);
-        return make_uint4(v[0], v[1], v[2], v[3]);
-    }
-    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
-        const int lane = threadIdx.x & 31;
-        const int g = lane >> 2, t = lane & 3;
+    __device__ __forceinline__ uint4 finish(const Piece& piece) const { return piece; }
+    struct Side {
+        float back[2];  // undoes x's shift, times the expert's tensor scale
+        int slot[2];
+    };
+    __device__ __forceinline__ Side look(const Pass& pass, int here) const {
+        Side side;
         const int first = routing.start[pass.active] + pass.first;
-        const int r = row_in_f(pass, tile, g);
         const float scale = p.gate_up.tensor_scale != nullptr ? p.gate_up.tensor_scale[routing.active[pass.active]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            const int n = min(static_cast<int>(threadIdx.x & 3) * 2 + j, here - 1);
+            side.slot[j] = routing.slots[first + n];
+            side.back[j] = inverse_power(p.x_shift[routing.tokens[first + n]]) * scale;
+        }
+        return side;
+    }
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[4]) const {
+        const int lane = threadIdx.x & 31;
+        const int g = lane >> 2, t = lane & 3;
+        const int r = row_in_f(pass, tile, g);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
             const int n = 2 * t + j;
-            const int slot = n < here ? routing.slots[first + n] : 0;
+            const int slot = side.slot[j];
             float h = 0.0f;
             if (n < here && r < p.f) {
-                const float back = inverse_power(p.x_shift[routing.tokens[first + n]]) * scale;
-                const float gate = acc[j] * back, up = acc[2 + j] * back;
+                const float gate = acc[j] * side.back[j], up = acc[2 + j] * side.back[j];
                 h = __fdividef(gate, 1.0f + expf(-gate)) * up;
             }
             int e = static_cast<int>((__float_as_uint(h) >> 23) & 0xffu);
@@ -766,7 +752,7 @@ template <int kFormat, int kHalves>
 constexpr int kUpSmem = 2 * Shape<kHalves>::kValueBytes + ring_bytes<kFormat>(kUpStages);
 template <int kFormat>
 constexpr int down_smem(int tokens) {
-    return tokens * Shape<2>::kDownPitch * 4 + 2 * Shape<2>::kValueBytes + ring_bytes<kFormat>(kDownStages);
+    return tokens * kDownPitch * 4 + 2 * Shape<2>::kValueBytes + ring_bytes<kFormat>(kDownStages);
 }
 
 template <int kFormat, int kHalves>
@@ -780,6 +766,39 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     run_passes<kFormat, kHalves, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves>::kValueBytes, halves);
 }
 
+// Columns k .. k + 7 of h (k a multiple of 8) are two rows each of four of the tiles that h came from: their exponents.
+__device__ __forceinline__ unsigned exponents_at(const MoeParams& p, int slot, int k) {
+    return *reinterpret_cast<const unsigned*>(p.h_exponent + static_cast<long long>(slot) * p.f_groups + (k >> 7) * 16 + ((k >> 3) & 3) * 4);
+}
+
+// Eight values of h brought from their tiles' powers of two to that of the slot's largest.
+__device__ __forceinline__ uint4 levelled(const uint4& raw, unsigned exponents, int largest) {
+    const int to = shift_of(largest);
+    unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        // 2^(to - from) as f16, at most 1 (what came from a smaller largest is multiplied up less); below 2^-24 it is 0
+        const int down = shift_of(static_cast<int>((exponents >> (8 * j)) & 0xffu)) - to;
+        const unsigned factor = down <= 0 ? 0x3c00u : down <= 14 ? static_cast<unsigned>(15 - down) << 10 : down <= 24 ? 1u << (24 - down) : 0u;
+        w[j] = mul_f16x2(w[j], factor | factor << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// All of h, in place.
+__global__ void __launch_bounds__(128) mc_moe_level(const MoeParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int slot = blockIdx.x;
+    const int largest = p.h_max[slot];
+    for (int k = threadIdx.x * 8; k < p.f_pitch; k += 128 * 8) {
+        auto* at = reinterpret_cast<uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
+        *at = levelled(*at, exponents_at(p, slot, k), largest);
+    }
+}
+
+// kLevel: h lies as mc_moe_level left it, one power of two per slot; otherwise as mc_moe_up did, one per tile of 8 rows.
+template <bool kLevel>
 struct DownWork {
     using S = Shape<2>;
     struct Piece {
@@ -808,73 +827,66 @@ struct DownWork {
     }
     // Row i of a tile: four neighbours in each group of 32, so that a warp uses 64 of 128 bytes of scales, the tile beside it the rest.
     __device__ __forceinline__ int row_in_y(int tile, int i) const {
-        return group / S::kDownGroups * 128 + 32 * (i >> 2) + 4 * S::kTiles * (group % S::kDownGroups) + 4 * tile + (i & 3);
-    }
-    template <typename Rows>
-    __device__ __forceinline__ void stride(Rows& rows) const {
-        rows.near = 32 * p.down.pitch;
-        rows.far = 64 * p.down.pitch;
+        return group / kDownGroups * 128 + 32 * (i >> 2) + 4 * S::kTiles * (group % kDownGroups) + 4 * tile + (i & 3);
     }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
         const int lane = threadIdx.x & 31;
         const int expert = routing.active[pass.active];
-        const int r = row_in_y(tile, lane >> 3);
-        rows.codes = p.down.codes + expert * p.down.matrix_codes + r * p.down.pitch + (lane & 7) * 16;
-        rows.there = (r < p.d ? 1u : 0u) | (r + 32 < p.d ? 2u : 0u) | (r + 64 < p.d ? 4u : 0u) | (r + 96 < p.d ? 8u : 0u);
-        if (__all_sync(0xffffffffu, rows.there == 15u)) rows.there = ~0u;
-        const int q = min(row_in_y(tile, lane & 15), p.d - 1);  // no such row: its sums go nowhere, any scale will do
-        rows.scales = p.down.scales + expert * p.down.matrix_scales + fp4_scale_offset(q, 0, p.down.k_tiles) + (lane >> 4) * kFp4TileBytes;
+        const int r = min(row_in_y(tile, lane >> 3), p.d - 1);
+        rows.codes = p.down.codes + expert * p.down.matrix_codes + r * p.down.pitch;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) rows.offset[i] = r + 32 * (i + 1) < p.d ? 32 * (i + 1) * p.down.pitch : 0;
+        rows.scales = p.down.scales + expert * p.down.matrix_scales + fp4_scale_offset(min(row_in_y(tile, lane & 15), p.d - 1), 0, p.down.k_tiles);
     }
-    // Columns k .. k + 7 are two rows each of four of the tiles that h came from.
     __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
         const int slot = routing.slots[n];
-        piece.largest = p.h_max[slot];
+        piece.raw = make_uint4(0, 0, 0, 0);
+        piece.exponents = 0;
+        if (!kLevel) piece.largest = p.h_max[slot];
         if (k < p.f_pitch) {
             piece.raw = *reinterpret_cast<const uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
-            piece.exponents = *reinterpret_cast<const unsigned*>(p.h_exponent + static_cast<long long>(slot) * p.f_groups + (k >> 7) * 16 + ((k >> 3) & 3) * 4);
-        } else {
-            piece.raw = make_uint4(0, 0, 0, 0);
-            piece.exponents = 0;
+            if (!kLevel) piece.exponents = exponents_at(p, slot, k);
         }
     }
-    __device__ __forceinline__ uint4 finish(const Piece& piece) const {
-        const int to = shift_of(piece.largest);
-        unsigned w[4] = {piece.raw.x, piece.raw.y, piece.raw.z, piece.raw.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // 2^(to - from) as f16, at most 1 (what came from a smaller largest is multiplied up less); below 2^-24 it is 0
-            const int down = shift_of(static_cast<int>((piece.exponents >> (8 * j)) & 0xffu)) - to;
-            const unsigned factor = down <= 0 ? 0x3c00u : down <= 14 ? static_cast<unsigned>(15 - down) << 10 : down <= 24 ? 1u << (24 - down) : 0u;
-            w[j] = mul_f16x2(w[j], factor | factor << 16);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const float (&acc)[4]) const {
-        const int lane = threadIdx.x & 31;
-        const int g = lane >> 2, t = lane & 3;
+    __device__ __forceinline__ uint4 finish(const Piece& piece) const { return kLevel ? piece.raw : levelled(piece.raw, piece.exponents, piece.largest); }
+    struct Side {
+        float back[2];    // undoes h's shift, times the expert's tensor scale
+        float weight[2];
+        int token[2];
+    };
+    __device__ __forceinline__ Side look(const Pass& pass, int here) const {
+        Side side;
+        const int first_slot = routing.start[pass.active] + pass.first;
         const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.active]] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int n = 2 * t + j;
-            if (n < here) {
-                const int at = routing.start[pass.active] + pass.first + n;
-                const int slot = routing.slots[at];
-                const float back = power(-shift_of(p.h_max[slot])) * scale;
-                const float w = p.weights[slot];
+            const int at = first_slot + min(static_cast<int>(threadIdx.x & 3) * 2 + j, here - 1);
+            const int slot = routing.slots[at];
+            side.back[j] = power(-shift_of(p.h_max[slot])) * scale;
+            side.weight[j] = p.weights[slot];
+            side.token[j] = routing.tokens[at];
+        }
+        return side;
+    }
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[4]) const {
+        const int lane = threadIdx.x & 31;
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (2 * t + j < here) {
                 // this warp's 16 columns; nobody else adds to them
-                float* sum = sums + routing.tokens[at] * S::kDownPitch + tile * 16;
-                sum[g] += w * (acc[j] * back);
-                sum[g + 8] += w * (acc[2 + j] * back);
+                float* sum = sums + side.token[j] * kDownPitch + tile * 16;
+                sum[g] += side.weight[j] * (acc[j] * side.back[j]);
+                sum[g + 8] += side.weight[j] * (acc[2 + j] * side.back[j]);
             }
         }
     }
 };
 
-template <int kFormat>
+template <int kFormat, bool kLevel>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
     using S = Shape<2>;
-    constexpr int kDownRows = S::kDownRows, kDownPitch = S::kDownPitch;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
     __shared__ float4 halves[kWarps / 2 * 32];
@@ -885,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, in
     const int group = blockIdx.x / cluster;
     for (int i = threadIdx.x; i < p.tokens * kDownPitch; i += kThreads) sums[i] = 0.0f;
     load_routing(routing, reinterpret_cast<int*>(values), p);
-    DownWork work{p, routing, sums, group, rank, cluster};
+    DownWork<kLevel> work{p, routing, sums, group, rank, cluster};
     run_passes<kFormat, 2, kDownStages>(work, p.down, routing, values, rings, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
@@ -962,16 +974,16 @@ int launch_up(MoeParams p, int reached, cudaStream_t s) {
     return launch(mc_moe_up<kFormat, kHalves>, grid, 1, kThreads, kUpSmem<kFormat, kHalves>, s, "mc_moe_up", p);
 }
 
-template <int kFormat>
+template <int kFormat, bool kLevel>
 int launch_down(MoeParams p, int reached, cudaStream_t s) {
     using S = Shape<2>;
     static PerDeviceOnce once;
-    if (int rc = ready(once, mc_moe_down<kFormat>, down_smem<kFormat>(MCD_MOE_MAX_TOKENS))) return rc;
+    if (int rc = ready(once, mc_moe_down<kFormat, kLevel>, down_smem<kFormat>(MCD_MOE_MAX_TOKENS))) return rc;
     p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
     int cluster = 8;
     while (cluster > reached) cluster /= 2;
-    const auto grid = static_cast<unsigned>((p.d + 127) / 128 * S::kDownGroups * cluster);
-    return launch(mc_moe_down<kFormat>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat>(p.tokens), s, "mc_moe_down", p, cluster);
+    const auto grid = static_cast<unsigned>((p.d + 127) / 128 * kDownGroups * cluster);
+    return launch(mc_moe_down<kFormat, kLevel>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat>(p.tokens), s, "mc_moe_down", p, cluster);
 }
 
 template <int kFormat>
@@ -981,12 +993,15 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     const int reached = std::min(p.experts, p.tokens * p.top_k);
     const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2>::kTiles) > 4LL * sm_count();
     if (int rc = many ? launch_up<kFormat, 1>(p, reached, s) : launch_up<kFormat, 2>(p, reached, s)) return rc;
-    return launch_down<kFormat>(p, reached, s);
+    // A launch of its own for h pays where many CTAs would each level the same rows of it: 32 row groups for every 2048 of d.
+    if (p.tokens * p.top_k <= 32) return launch_down<kFormat, false>(p, reached, s);
+    if (int rc = launch(mc_moe_level, static_cast<unsigned>(p.tokens * p.top_k), 1, 128, 0, s, "mc_moe_level", p)) return rc;
+    return launch_down<kFormat, true>(p, reached, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-size_t f_pitch(long long f) { return static_cast<size_t>((f + 7) / 8 * 8); }
+size_t in_eights(long long n) { return static_cast<size_t>((n + 7) / 8 * 8); }
 size_t f_groups(long long f) { return static_cast<size_t>((f + 127) / 128 * 16); }
 
 Matrix4 matrix_of(const mcd_fp4_tensor& t) {
@@ -1009,7 +1024,8 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
 extern "C" size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f) {
     if (tokens < 1 || tokens > MCD_MOE_MAX_TOKENS || experts < 1 || top_k < 1 || top_k > MCD_MOE_MAX_TOP_K || d < 1 || f < 1) return 0;
     const size_t slots = static_cast<size_t>(tokens) * static_cast<size_t>(top_k);
-    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + rounded(slots * f_groups(f)) + rounded(slots * f_pitch(f) * 2);
+    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + rounded(slots * f_groups(f)) + rounded(slots * in_eights(f) * 2) +
+           rounded(static_cast<size_t>(tokens) * in_eights(d) * 2);
 }
 
 extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
@@ -1062,10 +1078,10 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     p.experts = experts;
     p.d = static_cast<int>(d);
     p.f = static_cast<int>(f);
-    p.f_pitch = static_cast<int>(f_pitch(f));
+    p.d_pitch = static_cast<int>(in_eights(d));
+    p.f_pitch = static_cast<int>(in_eights(f));
     p.f_groups = static_cast<int>(f_groups(f));
-    p.x_vec = is_aligned(args->x, 16) && args->ldx % 8 == 0;
-    p.router_vec = p.x_vec && is_aligned(args->router, 16) && args->ld_router % 8 == 0;
+    p.router_vec = is_aligned(args->x, 16) && args->ldx % 8 == 0 && is_aligned(args->router, 16) && args->ld_router % 8 == 0;
     p.gate_up = matrix_of(gu);
     p.down = matrix_of(dn);
     p.chosen_out = args->chosen;
@@ -1078,6 +1094,7 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     p.x_shift = reinterpret_cast<float*>(at += rounded(slots * 4));
     p.h_exponent = at += rounded(static_cast<size_t>(args->tokens) * 4);
     p.h = reinterpret_cast<unsigned short*>(at += rounded(slots * f_groups(f)));
+    p.x16 = reinterpret_cast<unsigned short*>(at += rounded(slots * in_eights(f) * 2));
     auto s = static_cast<cudaStream_t>(stream);
     return gu.format == MCD_FP4_E8M0_32 ? launch_layer<MCD_FP4_E8M0_32>(p, s) : launch_layer<MCD_FP4_E4M3_16>(p, s);
 }
