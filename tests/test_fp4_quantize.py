@@ -182,7 +182,7 @@ def test_every_byte_is_the_definitions(mc, ref, fmt, dtype, rows, cols):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", ("f32", "f16"))
-@pytest.mark.parametrize("pitch, offset", [(80, 0), (77, 1), (79, 3), (96, 16)])
+@pytest.mark.parametrize("pitch, offset", [(80, 0), (77, 1), (79, 3), (96, 16), (72, 0), (76, 4), (72, 8)])
 def test_strides_and_alignment(mc, ref, fmt, dtype, pitch, offset):
     rng = np.random.default_rng(pitch)
     x = _values(rng, 3 * 130, 70, dtype).view(3, 130, 70)
