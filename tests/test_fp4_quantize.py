@@ -301,6 +301,41 @@ def test_side_stream_and_replayed_graph(mc, ref, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows, cols", [(4, 96), (1024, 4096)])
+def test_a_chain_of_calls_reads_what_the_call_before_wrote(mc, ref, rows, cols):
+    """Launches may start before the one in front of them is done: dequantise into x, take x's scale, quantise x, and again."""
+    import torch
+
+    rng = np.random.default_rng(1)
+    fmt = "e4m3_16"
+    sources, keep = [], []
+    for i in range(2):
+        code = rng.integers(0, 16, size=(rows, cols)).astype(np.uint8)
+        scale = np.full((rows, cols // 16), 0x38 + 8 * i, dtype=np.uint8)
+        codes, tiles = (torch.from_numpy(v).cuda() for v in ref.pack(code, scale, fmt))
+        keep.append((codes, tiles))
+        sources.append(mc.Fp4Matrix(fmt, rows, cols, codes.data_ptr(), tiles.data_ptr()))
+    x = torch.zeros(rows, cols, device="cuda")
+    codes, scales, sizes = _buffers(mc, fmt, rows, cols, 1)
+    g = torch.zeros(40, device="cuda")
+    back = torch.zeros(40, rows, cols, device="cuda") if rows < 100 else None
+    torch.cuda.synchronize()
+    for i in range(40):
+        m = mc.Fp4Matrix(fmt, rows, cols, codes.data_ptr(), scales.data_ptr(), g.data_ptr() + 4 * i)
+        mc.fp4_dequantize(sources[i % 2], x.data_ptr(), "f32")
+        mc.fp4_tensor_scale(x.data_ptr(), "f32", rows, cols, g.data_ptr() + 4 * i)
+        mc.fp4_quantize(x.data_ptr(), "f32", m)
+        if back is not None:
+            mc.fp4_dequantize(m, back.data_ptr() + 4 * i * rows * cols, "f32")
+    torch.cuda.synchronize()
+    want = [float(np.float32(6.0 * (i + 1) / 2688.0)) for i in range(2)]  # the codes hold a 6, the scales are 1 or 2
+    assert g.tolist() == [want[i % 2] for i in range(40)]
+    if back is not None:
+        for i in range(2):
+            assert (back[i::2] == back[i]).all() and not torch.equal(back[0], back[1])
+
+
+@pytest.mark.gpu
 def test_more_values_than_32_bits_count(mc, ref):
     """Rows far behind the 2^31st value: sampled rows against the definition."""
     import torch
