@@ -49,6 +49,7 @@ struct Fp4GemmParams {
     int rows, cols, k;
     int k_blocks, k_blocks_per_split, splits;
     int swapped;  // 0: rows are C's rows; 1: rows are C's columns
+    int wide;     // the row operand's map is the four-dimensional one
 };
 
 __device__ __forceinline__ void store_c(void* c, int type, long long at, float v) {
@@ -75,30 +76,57 @@ __device__ __forceinline__ unsigned pack_half2(float lo, float hi, int type) {
     return d;
 }
 
+// 16 neighbouring values of a row, 16-byte aligned.
+__device__ __forceinline__ void store_row16(void* c, int type, long long at, const float (&f)[16]) {
+    if (type == MCD_TYPE_F32) {
+        auto* to = reinterpret_cast<float4*>(static_cast<float*>(c) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+    } else {
+        auto* to = reinterpret_cast<uint4*>(static_cast<unsigned short*>(c) + at);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float* q = f + 8 * j;
+            to[j] = make_uint4(pack_half2(q[0], q[1], type), pack_half2(q[2], q[3], type), pack_half2(q[4], q[5], type), pack_half2(q[6], q[7], type));
+        }
+    }
+}
+
 __device__ __forceinline__ float product_scale(const float* a, const float* b) {
     return (a != nullptr ? *a : 1.0f) * (b != nullptr ? *b : 1.0f);
 }
 
 // ------------------------------------------------------------------------------------------------ one CTA per tile
 //
-// 128 rows x kCols columns, K in blocks of 256 codes (128 bytes per tile row). Warp 0 brings tiles and scales into a ring
-// of stages, warp 1 issues copies of scales and multiplies, warps 2-5 drain one of two accumulators while the other is
-// being filled.
+// 128 rows x kCols columns, K in blocks of 256 codes (128 bytes per tile row), kBlocks of them per stage. Warp 0 brings
+// tiles and scales into a ring of stages, warp 1 issues copies of scales and multiplies, warps 2-5 drain one of two
+// accumulators while the other is being filled.
+//
+// What bounds it: few columns, that is few tokens, read the whole of the row operand once (16384 x 16384 E8M0_32 codes,
+// 143 MB: 41 to 50 us on different boxes; copying them to shared memory and nothing else took 33, contiguous or not, most
+// of the rest is the ramp of one wave of CTAs). Neither the multiplies nor the copies of scales are felt. A
+// stage therefore takes two or four K blocks, and one four-dimensional TMA box brings them in the order 8 rows x 128
+// bytes, the next 128 bytes of the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192: 16.0 us, 16.9 block by block). In shared memory the 1024-byte atoms of
+// a K block are then kBlocks apart, which is a stride of the operand descriptor. Matrices whose rows are no multiple of 8, or
+// whose row pitch is none of 128 bytes, go block by block (such a box could reach past the end of the last row).
 
 template <int kFormat, int kCols>
 struct Fp4Tile {
+    static constexpr int kBlocks = kCols <= 32 ? 4 : 2;
     static constexpr int kScaleTiles = kFormat == MCD_FP4_E8M0_32 ? 2 : 4;  // per K block
-    static constexpr int kRowBytes = kTileRows * 128;
+    static constexpr int kRowBytes = kTileRows * 128;                       // per K block, as the next two
     static constexpr int kColBytes = kCols * 128;
     static constexpr int kScaleBytes = kScaleTiles * kFp4TileBytes;
-    static constexpr int kStageBytes = kRowBytes + kColBytes + 2 * kScaleBytes;
-    static constexpr int kStages = std::min(10, 222000 / kStageBytes);
+    static constexpr int kStageBytes = kBlocks * (kRowBytes + kColBytes + 2 * kScaleBytes);
+    static constexpr int kStages = 221184 / kStageBytes;
     static constexpr int kBarrierBytes = 512;
-    static constexpr int kSmem = kStages * kStageBytes + 1024 + kBarrierBytes;
+    static constexpr int kTurnBytes = 4 * 32 * 17 * 4;  // see the epilogue
+    static constexpr int kSmem = kStages * kStageBytes + 1024 + kBarrierBytes + kTurnBytes;
     static constexpr int kAccColumns = kCols < 32 ? 32 : kCols;
     static constexpr int kScaleColumns = kScaleTiles * 4;
     static constexpr int kScaleBase = 2 * kAccColumns;
-    static_assert(kScaleBase + kStages * 2 * kScaleColumns <= 512, "TMEM columns");
+    static_assert(kStages >= 2, "a ring");
+    static_assert(kScaleBase + kStages * kBlocks * 2 * kScaleColumns <= 512, "TMEM columns");
     static_assert(kStages * 16 + 32 <= kBarrierBytes, "barriers");
 };
 
@@ -171,20 +199,28 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                 const int kb_end = min(p.k_blocks, kb_begin + p.k_blocks_per_split);
                 const unsigned char* row_scales = p.row_scales + rb * p.k_tiles * kFp4TileBytes;
                 const unsigned char* col_scales = p.col_scales + (cb * kCols >> 7) * p.k_tiles * kFp4TileBytes;
-                for (int kb = kb_begin; kb < kb_end; ++kb) {
+                for (int kb = kb_begin; kb < kb_end; kb += Tile::kBlocks) {
                     ok = mc_mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, MC_FP4_ERR_PRODUCER);
                     if (!ok) break;
                     const unsigned full = bar_full + 8 * stage;
                     const unsigned rows_dst = tiles_base + stage * Tile::kStageBytes;
-                    const unsigned cols_dst = rows_dst + Tile::kRowBytes;
-                    const unsigned scales_dst = cols_dst + Tile::kColBytes;
+                    const unsigned cols_dst = rows_dst + Tile::kBlocks * Tile::kRowBytes;
+                    const unsigned scales_dst = cols_dst + Tile::kBlocks * Tile::kColBytes;
+                    const int blocks = min(Tile::kBlocks, kb_end - kb);
                     const int kt = kb * Tile::kScaleTiles;
-                    const unsigned scale_bytes = static_cast<unsigned>(min(static_cast<long long>(Tile::kScaleTiles), p.k_tiles - kt)) * kFp4TileBytes;
-                    mc_mbar_expect_tx(full, Tile::kRowBytes + Tile::kColBytes + 2 * scale_bytes);
-                    mc_tma_load_2d(rows_dst, &map_rows, full, kb * 128, rb * kTileRows);
-                    mc_tma_load_2d(cols_dst, &map_cols, full, kb * 128, cb * kCols);
+                    const unsigned scale_bytes =
+                        static_cast<unsigned>(min(static_cast<long long>(blocks * Tile::kScaleTiles), p.k_tiles - kt)) * kFp4TileBytes;
+                    // a wide box counts whole, whatever of it lies outside the matrix
+                    mc_mbar_expect_tx(full, (p.wide ? Tile::kBlocks : blocks) * Tile::kRowBytes + blocks * Tile::kColBytes + 2 * scale_bytes);
+                    if (p.wide) {
+                        tma_load_4d(rows_dst, &map_rows, full, 0, 0, kb, rb * (kTileRows / 8));
+                    } else {
+                        for (int i = 0; i < blocks; ++i) mc_tma_load_2d(rows_dst + i * Tile::kRowBytes, &map_rows, full, (kb + i) * 128, rb * kTileRows);
+                    }
+                    for (int i = 0; i < blocks; ++i) mc_tma_load_2d(cols_dst + i * Tile::kColBytes, &map_cols, full, (kb + i) * 128, cb * kCols);
                     fp4_bulk_load(scales_dst, row_scales + static_cast<long long>(kt) * kFp4TileBytes, scale_bytes, full);
-                    fp4_bulk_load(scales_dst + Tile::kScaleBytes, col_scales + static_cast<long long>(kt) * kFp4TileBytes, scale_bytes, full);
+                    fp4_bulk_load(scales_dst + Tile::kBlocks * Tile::kScaleBytes, col_scales + static_cast<long long>(kt) * kFp4TileBytes, scale_bytes,
+                                  full);
                     ++issued;
                     if (++stage == stages) {
                         stage = 0;
@@ -226,35 +262,42 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned tmem_d = tmem + static_cast<unsigned>(acc * Tile::kAccColumns);
-                for (int kb = kb_begin; kb < kb_end; ++kb) {
+                for (int kb = kb_begin; kb < kb_end; kb += Tile::kBlocks) {
                     ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned rows_src = tiles_base + stage * Tile::kStageBytes;
-                    const unsigned cols_src = rows_src + Tile::kRowBytes;
-                    const unsigned scales_src = cols_src + Tile::kColBytes;
-                    const unsigned scale_r = tmem + Tile::kScaleBase + static_cast<unsigned>(stage * 2 * Tile::kScaleColumns);
-                    const unsigned scale_c = scale_r + Tile::kScaleColumns;
-                    const int left = p.k - kb * kFp4BlockK;
+                    const unsigned cols_src = rows_src + Tile::kBlocks * Tile::kRowBytes;
+                    const unsigned scales_src = cols_src + Tile::kBlocks * Tile::kColBytes;
+                    const unsigned scale_r = tmem + Tile::kScaleBase + static_cast<unsigned>(stage * Tile::kBlocks * 2 * Tile::kScaleColumns);
+                    const unsigned scale_c = scale_r + Tile::kBlocks * Tile::kScaleColumns;
                     // Behind the last column there are no scale tiles: those instructions are left out (the codes there are
                     // 0, but what lies in the scales' place could be a NaN).
-                    const int steps = min(kFp4BlockK / kFp4MmaK, (left + kFp4MmaK - 1) / kFp4MmaK);
+                    const int left = min(p.k, kb_end * kFp4BlockK) - kb * kFp4BlockK;
+                    const int all_steps = (left + kFp4MmaK - 1) / kFp4MmaK;
 #pragma unroll
-                    for (int t = 0; t < Tile::kScaleTiles; ++t) {
-                        if (t * (kFp4BlockK / kFp4MmaK / Tile::kScaleTiles) < steps) {
-                            fp4_scales_to_tmem<1>(scale_r + 4 * t, fp4_scale_desc(scales_src + t * kFp4TileBytes));
-                            fp4_scales_to_tmem<1>(scale_c + 4 * t, fp4_scale_desc(scales_src + Tile::kScaleBytes + t * kFp4TileBytes));
+                    for (int i = 0; i < Tile::kBlocks; ++i) {
+                        const int steps = min(kFp4BlockK / kFp4MmaK, all_steps - i * (kFp4BlockK / kFp4MmaK));
+#pragma unroll
+                        for (int t = 0; t < Tile::kScaleTiles; ++t) {
+                            const int tile = i * Tile::kScaleTiles + t;
+                            if (t * (kFp4BlockK / kFp4MmaK / Tile::kScaleTiles) < steps) {
+                                fp4_scales_to_tmem<1>(scale_r + 4 * tile, fp4_scale_desc(scales_src + tile * kFp4TileBytes));
+                                fp4_scales_to_tmem<1>(scale_c + 4 * tile,
+                                                      fp4_scale_desc(scales_src + (Tile::kBlocks * Tile::kScaleTiles + tile) * kFp4TileBytes));
+                            }
                         }
-                    }
-                    const unsigned long long desc_r = fp4_tile_desc(rows_src);
-                    const unsigned long long desc_c = fp4_tile_desc(cols_src);
+                        const unsigned long long desc_r = p.wide ? fp4_tile_desc(rows_src + i * 1024, Tile::kBlocks * 1024)
+                                                                 : fp4_tile_desc(rows_src + i * Tile::kRowBytes, 1024);
+                        const unsigned long long desc_c = fp4_tile_desc(cols_src + i * Tile::kColBytes, 1024);
 #pragma unroll
-                    for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
-                        if (ks < steps) {
-                            const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
-                            const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
-                            fp4_mma<kFormat, 1>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 4 * t,
-                                                (kb > kb_begin || ks > 0) ? 1u : 0u);
+                        for (int ks = 0; ks < kFp4BlockK / kFp4MmaK; ++ks) {
+                            if (ks < steps) {
+                                const int tile = i * Tile::kScaleTiles + (kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks);
+                                const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
+                                fp4_mma<kFormat, 1>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * tile, scale_c + 4 * tile,
+                                                    (kb > kb_begin || i > 0 || ks > 0) ? 1u : 0u);
+                            }
                         }
                     }
                     fp4_commit(bar_empty + 8 * stage);
@@ -272,6 +315,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
     } else {
         const int quarter = warp & 3;
         constexpr int kChunk = 16;
+        float* turn = reinterpret_cast<float*>(smem_raw + (tiles_base - mc_smem_addr(smem_raw)) + stages * Tile::kStageBytes + Tile::kBarrierBytes) + quarter * 32 * 17;
         const float alpha = product_scale(p.row_scale, p.col_scale);
         int acc = 0;
         unsigned acc_phase = 0;
@@ -291,19 +335,38 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
             const long long ld = partial ? n : p.ldc;
             const int type = partial ? MCD_TYPE_F32 : p.c_type;
             const float scale = partial ? 1.0f : alpha;
+            // rows of C that start on 16-byte boundaries leave in pieces of that size
+            const bool vec = !p.swapped && (reinterpret_cast<unsigned long long>(dst) & 15) == 0 && (ld & (type == MCD_TYPE_F32 ? 3 : 7)) == 0;
             for (int chunk = 0; chunk < kCols / kChunk; ++chunk) {
                 const int col0 = cb * kCols + chunk * kChunk;
                 if (col0 >= p.cols) break;
                 unsigned v[kChunk];
                 tmem_load16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + static_cast<unsigned>(acc * Tile::kAccColumns + chunk * kChunk), v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (row < p.rows) {
+                if (row < p.rows && vec && col0 + kChunk <= p.cols) {
+                    float f[kChunk];
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) {
-                        if (col0 + j < p.cols) {
-                            const long long at = p.swapped ? static_cast<long long>(col0 + j) * ld + row : static_cast<long long>(row) * ld + col0 + j;
-                            store_c(dst, type, at, __uint_as_float(v[j]) * scale);
+                    for (int j = 0; j < kChunk; ++j) f[j] = __uint_as_float(v[j]) * scale;
+                    store_row16(dst, type, static_cast<long long>(row) * ld + col0, f);
+                } else if (p.swapped) {
+                    if (row < p.rows) {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) {
+                            if (col0 + j < p.cols) store_c(dst, type, static_cast<long long>(col0 + j) * ld + row, __uint_as_float(v[j]) * scale);
                         }
+                    }
+                }
+                if (!p.swapped && !(vec && col0 + kChunk <= p.cols)) {
+                    // Rows of C that start anywhere: turned round in shared memory, so that half a warp writes a row's 16 values
+                    // (65536 x 100 of them, one thread a row: 77 us, this way 37).
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) turn[lane * 17 + j] = __uint_as_float(v[j]) * scale;
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = row - lane + 2 * i + (lane >> 4), c = col0 + (lane & 15);
+                        if (r < p.rows && c < p.cols) store_c(dst, type, static_cast<long long>(r) * ld + c, turn[(2 * i + (lane >> 4)) * 17 + (lane & 15)]);
                     }
                 }
             }
@@ -509,8 +572,8 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     const unsigned cols_src = rows_src + Pair::kRowBytes;
                     const unsigned scale_r = tmem + Pair::kScaleBase + static_cast<unsigned>(ready * Pair::kScaleColumns);
                     const unsigned scale_c = scale_r + Pair::kRowScaleColumns;
-                    const unsigned long long desc_r = fp4_tile_desc(rows_src);
-                    const unsigned long long desc_c = fp4_tile_desc(cols_src);
+                    const unsigned long long desc_r = fp4_tile_desc(rows_src, 1024);
+                    const unsigned long long desc_c = fp4_tile_desc(cols_src, 1024);
                     const int this_stage = stage;
                     if (++ready == Pair::kScaleBuffers) {
                         ready = 0;
@@ -600,7 +663,6 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16) + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
             const int row0 = rb * kPairTile + static_cast<int>(rank) * 128 + quarter * 32;
-            const int row = row0 + lane;
             // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
             // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
             auto chunk_at = [&](int i) { return acc ? i : 7 - i; };
@@ -643,11 +705,21 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                         __syncwarp();
                         if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
                     }
-                } else if (row < p.m) {
+                } else {
+                    // turned round in the staging buffer (the swizzle keeps both ways free of bank conflicts): a warp writes a row
+                    if (lane == 0) tma_store_wait_read<0>();
+                    __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        if (col0 + j < p.n) store_c(p.c, p.c_type, static_cast<long long>(row) * p.ldc + col0 + j, f[j]);
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(buffer + (lane * 32 + (j ^ lane)) * 4), "f"(f[j]) : "memory");
                     }
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < p.m; ++r) {
+                        float value;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value) : "r"(buffer + (r * 32 + (lane ^ r)) * 4) : "memory");
+                        if (col0 + lane < p.n) store_c(p.c, p.c_type, static_cast<long long>(row0 + r) * p.ldc + col0 + lane, value);
+                    }
+                    __syncwarp();
                 }
             };
             constexpr int kFirst = (Pair::kOverlapChunks + 1) / 2;  // shared chunks of the warps with half == 0
@@ -714,21 +786,27 @@ struct Plan {
     int per_split = 1;
 };
 
+// Up to 128 rows or columns of C: the one-CTA kernel, the shorter side as accumulator columns, so that the longer one fills
+// the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192: 19 us, 36 in
+// tiles of 128 x 128; 1024^3: 12 against 23; 512 x 512 x 4096, four tiles: 13 against 18 with K split).
+//
+// K is split where less than 60 CTAs would work: at one token an SM draws some 70 GB/s, so 64 of them take 8192 x 8192
+// codes in as good a time as 128 halves of them and a second launch that joins the halves (14 against 16 us).
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
     plan.per_split = plan.k_blocks;
-    plan.pairs = ((m + 255) / 256) * ((n + 255) / 256) >= 37;
+    plan.pairs = m > 128 && n > 128;
     if (plan.pairs) return plan;
-    plan.swapped = m <= 128;
+    plan.swapped = m <= n;
     const long long rows = plan.swapped ? n : m;
     const long long cols = plan.swapped ? m : n;
-    plan.tile_cols = !plan.swapped ? 128 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-    const long long tiles = ((rows + 127) / 128) * ((cols + plan.tile_cols - 1) / plan.tile_cols);
-    const int sms = 148;
-    int splits = 1;
-    if (tiles * 2 <= sms) splits = static_cast<int>(std::max<long long>(1, std::min<long long>(sms / tiles, plan.k_blocks / 4)));
-    plan.per_split = (plan.k_blocks + splits - 1) / splits;
+    plan.tile_cols = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
+    const long long tiles = (rows + 127) / 128;
+    constexpr int kSms = 148;
+    const int splits = tiles < 60 ? static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4))) : 1;
+    const int stage = plan.tile_cols <= 32 ? 4 : 2;  // K blocks of a stage
+    plan.per_split = ((plan.k_blocks + splits - 1) / splits + stage - 1) / stage * stage;
     plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
     return plan;
 }
@@ -743,6 +821,24 @@ int encode_codes(McTensorMap* map, const mcd_fp4_tensor& t, unsigned box_rows) {
     const cuuint32_t box[2] = {128, box_rows};
     const cuuint32_t elem_strides[2] = {1, 1};
     return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.codes, dims, strides,
+                                               box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled");
+}
+
+// Codes in atoms of 8 rows x 128 bytes; a box takes 16 such groups of rows and `blocks` neighbouring atoms of each, in the
+// order atom, neighbour, next group. Rows a multiple of 8, pitch one of 128: the box then never leaves the matrix unseen.
+bool can_be_wide(const mcd_fp4_tensor& t) { return t.rows % 8 == 0 && mcd_fp4_code_pitch(t.cols) % 128 == 0; }
+
+int encode_wide_codes(McTensorMap* map, const mcd_fp4_tensor& t, unsigned blocks) {
+    const DriverApi* drv = driver_api();
+    if (drv == nullptr) return fail("the CUDA driver API is unavailable");
+    const auto pitch = static_cast<cuuint64_t>(mcd_fp4_code_pitch(t.cols));
+    const cuuint64_t dims[4] = {128, 8, pitch / 128, static_cast<cuuint64_t>(t.rows / 8)};
+    const cuuint64_t strides[3] = {pitch, 128, 8 * pitch};
+    const cuuint32_t box[4] = {128, 8, blocks, kTileRows / 8};
+    const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+    return check_drv(drv->TensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, t.codes, dims, strides,
                                                box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
                      "cuTensorMapEncodeTiled");
@@ -915,7 +1011,8 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
     const mcd_fp4_tensor& on_rows = plan.swapped ? args->b : args->a;
     const mcd_fp4_tensor& on_cols = plan.swapped ? args->a : args->b;
     McTensorMap map_rows, map_cols;
-    if (int rc = encode_codes(&map_rows, on_rows, kTileRows)) return rc;
+    const bool wide = can_be_wide(on_rows);
+    if (int rc = wide ? encode_wide_codes(&map_rows, on_rows, plan.tile_cols <= 32 ? 4 : 2) : encode_codes(&map_rows, on_rows, kTileRows)) return rc;
     if (int rc = encode_codes(&map_cols, on_cols, static_cast<unsigned>(plan.tile_cols))) return rc;
     Fp4GemmParams p;
     p.row_scales = static_cast<const unsigned char*>(on_rows.scales);
@@ -935,6 +1032,7 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
     p.k_blocks_per_split = plan.per_split;
     p.splits = plan.splits;
     p.swapped = plan.swapped ? 1 : 0;
+    p.wide = wide ? 1 : 0;
     auto s = static_cast<cudaStream_t>(stream);
     const auto grid = static_cast<unsigned>(std::min<long long>(items, sm_count()));
     if (int rc = args->a.format == MCD_FP4_E8M0_32 ? launch_format<MCD_FP4_E8M0_32>(plan.tile_cols, map_rows, map_cols, p, grid, s)

@@ -11,9 +11,9 @@ namespace mcd {
 constexpr int kFp4BlockK = 256;
 constexpr int kFp4MmaK = 64;
 
-// K-major operand tile: rows of 128 bytes with the 128-byte swizzle, groups of 8 rows 1024 bytes apart.
-__device__ __forceinline__ unsigned long long fp4_tile_desc(unsigned addr) {
-    return static_cast<unsigned long long>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<unsigned long long>(1024 >> 4) << 32) |
+// K-major operand tile: rows of 128 bytes with the 128-byte swizzle, groups of 8 rows `apart` bytes from one another.
+__device__ __forceinline__ unsigned long long fp4_tile_desc(unsigned addr, unsigned apart) {
+    return static_cast<unsigned long long>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<unsigned long long>(apart >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
 }
 
@@ -108,6 +108,12 @@ __device__ __forceinline__ void tma_load_3d(unsigned smem_dst, const McTensorMap
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
         "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(unsigned smem_dst, const McTensorMap* map, unsigned bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
 }
 // One box out of shared memory; what lies outside the tensor is not written.

@@ -111,7 +111,7 @@ def _product(mc, a, b, dtype, ldc=None, offset=0, stream=0):
 @pytest.mark.parametrize("m, n, k", [
     (1, 1, 1), (1, 8, 31), (1, 128, 64), (2, 130, 65), (16, 128, 256), (17, 257, 257), (33, 64, 300), (64, 200, 96), (65, 129, 512),
     (128, 128, 128), (128, 300, 1000), (129, 128, 256), (200, 70, 33), (256, 256, 768), (300, 513, 321), (1, 300, 4096), (40, 100, 5000),
-    (513, 256, 1024), (512, 512, 2080), (700, 900, 640), (2100, 1300, 700), (1600, 1600, 2304), (10000, 257, 64), (2305, 2304, 1),
+    (513, 256, 1024), (512, 512, 2080), (700, 900, 640), (2100, 1300, 700), (1600, 1600, 2304), (10000, 257, 64), (2305, 2304, 1), (3000, 1, 128), (1000, 16, 3100), (700, 100, 257), (513, 128, 2048), (128, 128, 4096),
 ])
 def test_exact_data_gives_equal_results(mc, ref, fmt, m, n, k):
     rng = np.random.default_rng(m * 7 + n * 3 + k)
