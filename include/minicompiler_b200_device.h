@@ -345,7 +345,7 @@ MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
 
 /* ------------------------------------------------- mixture of experts, few tokens
  * A whole layer: for each of 1 .. MCD_MOE_MAX_TOKENS tokens
- *   l = R x (64-bit sums of the 16-bit products), p = softmax(l) over all experts,
+ *   l = R x (products of 16-bit values, exact in f32, summed to twice f32's precision), p = softmax(l) over all experts,
  *   the top_k experts by l, ties and NaN to the lowest index (a NaN counts as lower than every number),
  *   w_j = p of the j-th one (renormalize != 0: divided by their sum),
  *   y = sum_j w_j * D_j (silu(G_j x) * (U_j x)),   silu(v) = v / (1 + exp(-v)).
@@ -360,7 +360,8 @@ MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
  * The products accumulate in f32. x and silu(..) * (..) enter them with 11 significant bits after a power of two per token,
  * or per token and expert, that takes their largest magnitude below 2^15: nothing of a bf16 or f16 x is lost above 2^-29 of
  * the token's largest value. The experts' results are added in an order that the routing alone fixes: results do not
- * depend on scheduling. No wait, no status word; three launches. */
+ * depend on scheduling. Nothing in it waits, so there is no status word; three launches, four for more than 32 (token,
+ * expert) pairs. */
 #define MCD_MOE_MAX_TOKENS 64
 #define MCD_MOE_MAX_EXPERTS 512
 #define MCD_MOE_MAX_TOP_K 16

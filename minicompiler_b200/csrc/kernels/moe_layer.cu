@@ -3,12 +3,20 @@
 //
 //   l = R x;  p = softmax(l);  y = sum over the top_k experts e of w_e * D_e (silu(G_e x) * (U_e x))
 //
-// Few tokens meet many weights: every weight is used for the handful of tokens that chose its expert, so the time is
-// that of reading the chosen experts' weights once. Three launches, each a programmatic dependent of the one before it:
+// Few tokens meet many weights: every weight is used for the handful of tokens that chose its expert, so the floor is the
+// time of reading the chosen experts' weights once. Three launches, or four, each a programmatic dependent of the one
+// before it:
 //
-//   mc_moe_router  one cluster of 8 CTAs per token: logits in 64-bit sums, softmax, the top_k experts
-//   mc_moe_up      4-warp CTAs take (expert, 32 rows of G and the same 32 of U): h = silu(G x) * (U x), f32
+//   mc_moe_router  one cluster of 8 CTAs per token: logits in double-length sums, softmax, the top_k experts; x to f16
+//   mc_moe_up      8-warp CTAs take (expert, 32 or 64 rows of G and the same of U): h = silu(G x) * (U x), f16
+//   mc_moe_level   (many slots) h of a token and expert to one power of two
 //   mc_moe_down    a cluster of up to 8 CTAs takes 64 rows of y, its CTAs share the experts and add up what they found
+//
+// Where the time goes: for one token and 8 of 64 experts (26.7 MB of weights, 4 us to read) 25 us are the latencies of
+// three dependent launches - routing, first copies, one round of multiplies, joining, each a microsecond or two. For 32
+// tokens and 128 experts of 2048 x 768 (294 MB, 46 us) 105 us: 49 up, 40 down. The SMs then issue instructions on 2.3 of 4
+// slots; half of them are the multiplies' (22 per 512 codes and warp), the rest what every pass of an expert's rows over
+// its 2 tokens costs beside.
 //
 // The products: codes are small numbers that f16 holds exactly, so a warp turns 16 rows of codes into f16 fragments
 // (one conversion for two codes) and multiplies them with 8 tokens' values by mma.sync m16n8k16, f32 sums. That
@@ -54,26 +62,28 @@ constexpr int kMaxSlots = MCD_MOE_MAX_TOKENS * MCD_MOE_MAX_TOP_K;
 
 // How a CTA's warps divide their work: tiles of 16 rows, and halves of the columns of a round. With two halves there are
 // twice as many, shorter passes: for a few tokens, which could not occupy the SMs otherwise. With one, what a pass costs
-// beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns.
-template <int kHalves>
+// beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns. Two groups
+// of four warps go through passes of their own, each with its barrier: the down projection's form of that, whose CTAs
+// must not grow beyond 64 rows.
+template <int kHalves, int kGroups>
 struct Shape {
-    static constexpr int kTiles = kWarps / kHalves;
-    static constexpr int kRoundSteps = 4 / kHalves;  // per warp
+    static constexpr int kGroupWarps = kWarps / kGroups;
+    static constexpr int kGroupThreads = kGroupWarps * 32;
+    static constexpr int kTiles = kGroupWarps / kHalves;
+    static constexpr int kRoundSteps = kHalves * kGroups == 1 ? 4 : 2;  // per warp
     static constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
     static constexpr int kValueBytes = kTokenTile * kValuePitch;
-    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kThreads;  // of 8 values, per thread and round
+    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values, per thread and round
     static constexpr int kUpGroups = 16 / kTiles;  // groups of rows of G (and of U) in 128
 };
 
-// The down projection always works in two halves (whole rows left it 128 CTAs of 2048 rows' worth, 160 against 136 us for
-// 32 tokens of a layer of 128 experts).
 constexpr int kDownGroups = 2;  // groups of rows of y in 128
 constexpr int kDownRows = 128 / kDownGroups;
 constexpr int kDownPitch = kDownRows + 4;
 constexpr int kRouterCluster = 8;
 constexpr int kRouterThreads = 256;
-constexpr int kUpStages = 4, kDownStages = 3;  // depth of a warp's ring; the down projection keeps sums beside it
+constexpr int kUpStages = 4;  // depth of a warp's ring
 
 template <int kFormat>
 struct Stage {
@@ -173,13 +183,30 @@ __device__ __forceinline__ void add_products(float& sum, float& c, const uint4& 
     }
 }
 
+// The larger ones of two magnitudes (16-bit values without their signs compare as integers) and those of eight values.
+__device__ __forceinline__ unsigned packed_max(unsigned most, const uint4& v) {
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(w[i] & 0x7fff7fffu));
+    return most;
+}
+
+// The double-length sum of a warp's lanes.
+__device__ __forceinline__ double lanes_sum(const float (&sum)[2], const float (&c)[2]) {
+    const float whole = sum[0] + sum[1];
+    const bool finite = fabsf(whole) <= 3.402823466e38f;  // an infinite or NaN sum has no error to speak of
+    double total = finite ? (static_cast<double>(sum[0]) + sum[1]) + (static_cast<double>(c[0]) + c[1]) : static_cast<double>(whole);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    return total;
+}
+
 __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads) mc_moe_router(const MoeParams p) {
     // used in the cluster's first CTA
     __shared__ double logits[MCD_MOE_MAX_EXPERTS];
     __shared__ unsigned long long keys[MCD_MOE_MAX_EXPERTS];
     __shared__ int order[MCD_MOE_MAX_EXPERTS];
     __shared__ int best[MCD_MOE_MAX_TOP_K];
-    __shared__ unsigned warp_max[kRouterThreads / 32];
     __shared__ float warp_sum[kRouterThreads / 32];
     const int token = blockIdx.x / kRouterCluster;
     const unsigned rank = cluster_rank();
@@ -189,51 +216,46 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     const unsigned short* x = p.x + token * p.ldx;
     const unsigned logits_first = peer_address(smem_u32(logits), 0);
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    unsigned largest = 0;  // |x| as bits, packed 16-bit pairs: every warp sees all of x on its first expert
     bool started = false;
-
     for (int e = static_cast<int>(rank) * (kRouterThreads / 32) + warp; e < p.experts || !started; e += kRouterCluster * (kRouterThreads / 32)) {
-        double total = 0.0;
-        if (e < p.experts) {
-            const unsigned short* r = p.router + e * p.ld_router;
-            float sum[2] = {0.0f, 0.0f}, c[2] = {0.0f, 0.0f};
-            int at = lane * 8;
-            if (p.router_vec) {
-                for (; at + 768 + 8 <= p.d; at += 1024) {  // four loads of each row in flight
-                    uint4 a[4], b[4];
+        const unsigned short* r = p.router + min(e, p.experts - 1) * p.ld_router;
+        float sum[2] = {0.0f, 0.0f}, c[2] = {0.0f, 0.0f};
+        int at = lane * 8;
+        if (p.router_vec) {
+            for (; at + 768 + 8 <= p.d; at += 1024) {  // four loads of each row in flight
+                uint4 a[4], b[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        a[i] = *reinterpret_cast<const uint4*>(x + at + 256 * i);
-                        b[i] = __ldcs(reinterpret_cast<const uint4*>(r + at + 256 * i));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) add_products(sum[i & 1], c[i & 1], a[i], b[i], p.type);
+                for (int i = 0; i < 4; ++i) {
+                    a[i] = *reinterpret_cast<const uint4*>(x + at + 256 * i);
+                    b[i] = *reinterpret_cast<const uint4*>(r + at + 256 * i);
                 }
-                for (; at + 8 <= p.d; at += 256) {
-                    add_products(sum[0], c[0], *reinterpret_cast<const uint4*>(x + at), *reinterpret_cast<const uint4*>(r + at), p.type);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    add_products(sum[i & 1], c[i & 1], a[i], b[i], p.type);
+                    largest = packed_max(largest, a[i]);
                 }
             }
-            for (int k = (p.router_vec ? p.d / 8 * 8 : 0) + lane; k < p.d; k += 32) add_exactly(sum[0], c[0], value16(x[k], p.type) * value16(r[k], p.type));
-            // an infinite or NaN sum has no error to speak of
-            const float whole = sum[0] + sum[1];
-            const bool finite = fabsf(whole) <= 3.402823466e38f;
-            total = finite ? (static_cast<double>(sum[0]) + sum[1]) + (static_cast<double>(c[0]) + c[1]) : static_cast<double>(whole);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            for (; at + 8 <= p.d; at += 256) {
+                const uint4 a = *reinterpret_cast<const uint4*>(x + at);
+                add_products(sum[0], c[0], a, *reinterpret_cast<const uint4*>(r + at), p.type);
+                largest = packed_max(largest, a);
+            }
         }
+        for (int k = (p.router_vec ? p.d / 8 * 8 : 0) + lane; k < p.d; k += 32) {
+            add_exactly(sum[0], c[0], value16(x[k], p.type) * value16(r[k], p.type));
+            largest = packed_max(largest, make_uint4(x[k], 0, 0, 0));
+        }
+        const double total = lanes_sum(sum, c);
         if (!started) {  // the first CTA of the cluster runs before its shared memory is written
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             started = true;
         }
         if (e < p.experts && lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(total) : "memory");
     }
-    // Every CTA of the cluster finds the token's largest magnitude and brings its share of x to f16.
-    unsigned largest = 0;
-    for (int c = threadIdx.x; c < p.d; c += kRouterThreads) largest = max(largest, __float_as_uint(value16(x[c], p.type)) & 0x7fffffffu);
-    largest = __reduce_max_sync(0xffffffffu, largest);
-    if (lane == 0) warp_max[warp] = largest;
-    __syncthreads();
-    for (int w = 0; w < kRouterThreads / 32; ++w) largest = max(largest, warp_max[w]);
-    const float shift = power(shift_of(static_cast<int>(largest >> 23)));
+    // Every CTA of the cluster knows the token's largest magnitude and brings its share of x to f16.
+    largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));
+    const float shift = power(shift_of(static_cast<int>(__float_as_uint(value16(static_cast<unsigned short>(largest), p.type)) >> 23)));
     for (int c = static_cast<int>(rank) * kRouterThreads + static_cast<int>(threadIdx.x); c < p.d_pitch; c += kRouterCluster * kRouterThreads) {
         p.x16[token * static_cast<long long>(p.d_pitch) + c] = static_cast<unsigned short>(c < p.d ? pack_f16(value16(x[c], p.type) * shift, 0.0f) & 0xffffu : 0u);
     }
@@ -247,14 +269,20 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
 
     for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) keys[e] = sort_key(logits[e]);
     __syncthreads();
-    // An expert's place is the number of experts that come before it: the larger logit, ties to the lower index. Several
-    // threads share the comparisons of one expert where there are fewer than threads.
-    const int shares = max(1, kRouterThreads / p.experts);
-    for (int i = threadIdx.x; i < p.experts * shares; i += kRouterThreads) {
-        const int e = i % p.experts;
+    // An expert's place is the number of experts that come before it: the larger logit, ties to the lower index. Where there
+    // are fewer experts than threads, several share the comparisons of one.
+    int spread = 32 - __clz(p.experts - 1);  // experts in a power of two
+    if (p.experts == 1) spread = 0;
+    const int shares = max(1, kRouterThreads >> spread);
+    for (int i = threadIdx.x; (i & ((1 << spread) - 1)) < p.experts && i < (shares << spread); i += kRouterThreads) {
+        const int e = i & ((1 << spread) - 1), share = i >> spread;
         const unsigned long long key = keys[e];
         int before = 0;
-        for (int j = i / p.experts; j < p.experts; j += shares) before += keys[j] > key || (keys[j] == key && j < e) ? 1 : 0;
+#pragma unroll 8
+        for (int j = share; j < p.experts; j += shares) {
+            const unsigned long long other = keys[j];
+            before += other > key || (other == key && j < e) ? 1 : 0;
+        }
         if (before != 0) atomicAdd(&order[e], before);
     }
     __syncthreads();
@@ -538,13 +566,22 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 //   finish(piece)             the same in f16
 //   look(pass, here)          what a lane will need of its two columns, read before the multiplies
 //   done(pass, here, tile, side, acc)  a warp's sums, both halves of k
-template <int kFormat, int kHalves, int kStages, typename Work>
+template <int kFormat, int kHalves, int kGroups, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
-    using S = Shape<kHalves>;
+    using S = Shape<kHalves, kGroups>;
     constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kPieces = S::kPieces, kValuePitch = S::kValuePitch;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile = warp % kTiles, half = warp / kTiles;
-    unsigned char* ring = rings + warp * kStages * Stage<kFormat>::kBytes;
+    const int lane = threadIdx.x & 31, group = threadIdx.x / S::kGroupThreads;
+    const int thread = threadIdx.x % S::kGroupThreads;
+    const int tile = (thread >> 5) % kTiles, half = (thread >> 5) / kTiles;
+    unsigned char* ring = rings + (threadIdx.x >> 5) * kStages * Stage<kFormat>::kBytes;
+    values += group * 2 * S::kValueBytes;
+    auto sync = [&] {
+        if constexpr (kGroups == 1) {
+            __syncthreads();
+        } else {
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(S::kGroupThreads) : "memory");
+        }
+    };
     const unsigned ring_at = smem_u32(ring);
     const int steps = m.rounds * kRoundSteps;
 
@@ -588,7 +625,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         const int first = routing.start[value_pass.active] + value_pass.first;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int piece = i * kThreads + static_cast<int>(threadIdx.x);
+            const int piece = i * S::kGroupThreads + thread;
             const int n = piece / (kRoundK / 8);
             if (n < here) work.load(pieces[i], first + n, value_round * kRoundK + piece % (kRoundK / 8) * 8);
         }
@@ -598,7 +635,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         const int here = slots_of(value_pass);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int piece = i * kThreads + static_cast<int>(threadIdx.x);
+            const int piece = i * S::kGroupThreads + thread;
             const int n = piece / (kRoundK / 8);
             if (n < here) *reinterpret_cast<uint4*>(to + n * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16) = work.finish(pieces[i]);
         }
@@ -613,7 +650,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         const typename Work::Side side = work.look(at, slots_of(at));
 #pragma unroll 1
         for (; round < m.rounds; ++round) {
-            __syncthreads();  // this round's values are there, nobody reads the other buffer any more
+            sync();  // this round's values are there, nobody reads the other buffer any more
             load_values();
             if (round >= 0) {
 #pragma unroll 1
@@ -638,7 +675,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         for (int i = 0; i < 4; ++i) acc[i] = sums[0][i] + sums[1][i], sums[0][i] = sums[1][i] = 0.0f;
         if constexpr (kHalves == 2) {
             if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            __syncthreads();
+            sync();
             if (half == 0) {
                 const float4 other = halves[tile * 32 + lane];
                 acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
@@ -654,7 +691,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
 
 template <int kHalves>
 struct UpWork {
-    using S = Shape<kHalves>;
+    using S = Shape<kHalves, 1>;
     using Piece = uint4;
     const MoeParams& p;
     const Routing& routing;
@@ -749,10 +786,16 @@ struct UpWork {
 template <int kFormat>
 constexpr int ring_bytes(int stages) { return kWarps * stages * Stage<kFormat>::kBytes; }
 template <int kFormat, int kHalves>
-constexpr int kUpSmem = 2 * Shape<kHalves>::kValueBytes + ring_bytes<kFormat>(kUpStages);
-template <int kFormat>
+constexpr int kUpSmem = 2 * Shape<kHalves, 1>::kValueBytes + ring_bytes<kFormat>(kUpStages);
+// The down projection in one of two forms. kMany false: the halves of a round, all warps on one expert after the other, h as
+// mc_moe_up left it. kMany true: two groups of warps on experts of their own, h levelled before by mc_moe_level (32 tokens
+// of 128 experts of 2048 x 768: 40 us against 45), rings as deep as the sums beside them allow.
+template <bool kMany>
+using DownShape = Shape<kMany ? 1 : 2, kMany ? 2 : 1>;
+template <int kFormat, bool kMany, int kStages>
 constexpr int down_smem(int tokens) {
-    return tokens * kDownPitch * 4 + 2 * Shape<2>::kValueBytes + ring_bytes<kFormat>(kDownStages);
+    constexpr int groups = kMany ? 2 : 1;
+    return groups * (tokens * kDownPitch * 4 + 2 * DownShape<kMany>::kValueBytes) + ring_bytes<kFormat>(kStages);
 }
 
 template <int kFormat, int kHalves>
@@ -763,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     load_routing(routing, reinterpret_cast<int*>(smem), p);
     UpWork<kHalves> work(p, routing);
-    run_passes<kFormat, kHalves, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves>::kValueBytes, halves);
+    run_passes<kFormat, kHalves, 1, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves, 1>::kValueBytes, halves);
 }
 
 // Columns k .. k + 7 of h (k a multiple of 8) are two rows each of four of the tiles that h came from: their exponents.
@@ -800,7 +843,7 @@ __global__ void __launch_bounds__(128) mc_moe_level(const MoeParams p) {
 // kLevel: h lies as mc_moe_level left it, one power of two per slot; otherwise as mc_moe_up did, one per tile of 8 rows.
 template <bool kLevel>
 struct DownWork {
-    using S = Shape<2>;
+    using S = DownShape<kLevel>;
     struct Piece {
         uint4 raw;
         unsigned exponents;
@@ -884,38 +927,47 @@ struct DownWork {
     }
 };
 
-template <int kFormat, bool kLevel>
+template <int kFormat, bool kMany, int kStages>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
-    using S = Shape<2>;
+    using S = DownShape<kMany>;
+    constexpr int groups = kMany ? 2 : 1;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
     __shared__ float4 halves[kWarps / 2 * 32];
     unsigned char* values = smem;
-    unsigned char* rings = values + 2 * S::kValueBytes;
-    float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kDownStages));
+    unsigned char* rings = values + groups * 2 * S::kValueBytes;
+    float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kStages));  // [groups][tokens][kDownPitch]
+    const int group_sums = p.tokens * kDownPitch;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int group = blockIdx.x / cluster;
-    for (int i = threadIdx.x; i < p.tokens * kDownPitch; i += kThreads) sums[i] = 0.0f;
+    const int rows = blockIdx.x / cluster;  // which 64
+    const int mine = threadIdx.x / S::kGroupThreads;
+    for (int i = threadIdx.x; i < groups * group_sums; i += kThreads) sums[i] = 0.0f;
     load_routing(routing, reinterpret_cast<int*>(values), p);
-    DownWork<kLevel> work{p, routing, sums, group, rank, cluster};
-    run_passes<kFormat, 2, kDownStages>(work, p.down, routing, values, rings, halves);
+    DownWork<kMany> work{p, routing, sums + mine * group_sums, rows, rank * groups + mine, cluster * groups};
+    run_passes<kFormat, kMany ? 1 : 2, groups, kStages>(work, p.down, routing, values, rings, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
-    // Every CTA of the cluster finishes its share of the elements: the partial sums in rank order.
-    const unsigned mine = smem_u32(sums);
+    // Every CTA of the cluster finishes its share of the elements: the partial sums in the order of ranks and groups.
+    const unsigned sums_at = smem_u32(sums);
     const int count = p.tokens * kDownRows;
     for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < count; i += cluster * kThreads) {
         const int token = i / kDownRows, c = i - token * kDownRows;
-        const unsigned at = mine + static_cast<unsigned>(token * kDownPitch + c) * 4u;
+        const unsigned at = sums_at + static_cast<unsigned>(token * kDownPitch + c) * 4u;
         float v = 0.0f;
         for (int z = 0; z < cluster; ++z) {
-            float part;
-            if (cluster > 1) {
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(peer_address(at, static_cast<unsigned>(z))) : "memory");
-            } else {
-                part = sums[token * kDownPitch + c];
+#pragma unroll
+            for (int g = 0; g < groups; ++g) {
+                float part;
+                if (cluster > 1) {
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                 : "=f"(part)
+                                 : "r"(peer_address(at + static_cast<unsigned>(g * group_sums * 4), static_cast<unsigned>(z)))
+                                 : "memory");
+                } else {
+                    part = sums[g * group_sums + token * kDownPitch + c];
+                }
+                v += part;
             }
-            v += part;
         }
         const int r = work.row_in_y(c >> 4, c & 15);
         if (r < p.d) {
@@ -965,7 +1017,7 @@ int ready(PerDeviceOnce& once, Kernel kernel, int smem) {
 
 template <int kFormat, int kHalves>
 int launch_up(MoeParams p, int reached, cudaStream_t s) {
-    using S = Shape<kHalves>;
+    using S = Shape<kHalves, 1>;
     static PerDeviceOnce once;
     if (int rc = ready(once, mc_moe_up<kFormat, kHalves>, kUpSmem<kFormat, kHalves>)) return rc;
     p.gate_up.rounds = (p.d + S::kRoundK - 1) / S::kRoundK;
@@ -974,16 +1026,17 @@ int launch_up(MoeParams p, int reached, cudaStream_t s) {
     return launch(mc_moe_up<kFormat, kHalves>, grid, 1, kThreads, kUpSmem<kFormat, kHalves>, s, "mc_moe_up", p);
 }
 
-template <int kFormat, bool kLevel>
+template <int kFormat, bool kMany, int kStages>
 int launch_down(MoeParams p, int reached, cudaStream_t s) {
-    using S = Shape<2>;
+    using S = DownShape<kMany>;
     static PerDeviceOnce once;
-    if (int rc = ready(once, mc_moe_down<kFormat, kLevel>, down_smem<kFormat>(MCD_MOE_MAX_TOKENS))) return rc;
+    if (int rc = ready(once, mc_moe_down<kFormat, kMany, kStages>, down_smem<kFormat, kMany, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
     p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
     int cluster = 8;
     while (cluster > reached) cluster /= 2;
     const auto grid = static_cast<unsigned>((p.d + 127) / 128 * kDownGroups * cluster);
-    return launch(mc_moe_down<kFormat, kLevel>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat>(p.tokens), s, "mc_moe_down", p, cluster);
+    return launch(mc_moe_down<kFormat, kMany, kStages>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat, kMany, kStages>(p.tokens), s,
+                  "mc_moe_down", p, cluster);
 }
 
 template <int kFormat>
@@ -991,12 +1044,12 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     // The router's clusters are declared with the kernel.
     if (int rc = launch(mc_moe_router, static_cast<unsigned>(p.tokens * kRouterCluster), 1, kRouterThreads, 0, s, "mc_moe_router", p)) return rc;
     const int reached = std::min(p.experts, p.tokens * p.top_k);
-    const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2>::kTiles) > 4LL * sm_count();
+    const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2, 1>::kTiles) > 4LL * sm_count();
     if (int rc = many ? launch_up<kFormat, 1>(p, reached, s) : launch_up<kFormat, 2>(p, reached, s)) return rc;
     // A launch of its own for h pays where many CTAs would each level the same rows of it: 32 row groups for every 2048 of d.
-    if (p.tokens * p.top_k <= 32) return launch_down<kFormat, false>(p, reached, s);
+    if (p.tokens * p.top_k <= 32) return launch_down<kFormat, false, 3>(p, reached, s);
     if (int rc = launch(mc_moe_level, static_cast<unsigned>(p.tokens * p.top_k), 1, 128, 0, s, "mc_moe_level", p)) return rc;
-    return launch_down<kFormat, true>(p, reached, s);
+    return p.tokens <= 32 ? launch_down<kFormat, true, 3>(p, reached, s) : launch_down<kFormat, true, 2>(p, reached, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
