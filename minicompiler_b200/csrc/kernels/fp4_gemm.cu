@@ -10,7 +10,6 @@
 #include "minicompiler_b200_device.h"
 
 #include "device/driver_api.hpp"
-#include "device/per_device.hpp"
 #include "kernels/fp4_host.hpp"
 #include "kernels/fp4_mma.cuh"
 
@@ -103,12 +102,13 @@ __device__ __forceinline__ float product_scale(const float* a, const float* b) {
 // accumulators while the other is being filled.
 //
 // What bounds it: few columns, that is few tokens, read the whole of the row operand once (16384 x 16384 E8M0_32 codes,
-// 143 MB: 41 to 50 us on different boxes; copying them to shared memory and nothing else took 33, contiguous or not, most
-// of the rest is the ramp of one wave of CTAs). Neither the multiplies nor the copies of scales are felt. A
-// stage therefore takes two or four K blocks, and one four-dimensional TMA box brings them in the order 8 rows x 128
-// bytes, the next 128 bytes of the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192: 16.0 us, 16.9 block by block). In shared memory the 1024-byte atoms of
-// a K block are then kBlocks apart, which is a stride of the operand descriptor. Matrices whose rows are no multiple of 8, or
-// whose row pitch is none of 128 bytes, go block by block (such a box could reach past the end of the last row).
+// 143 MB: 41 to 50 us on different boxes; bringing them to shared memory and nothing else took 33, in one run or not, most
+// of the rest is the ramp of one wave of CTAs). Neither the multiplies nor the copies of scales are felt. A stage takes two
+// or four K blocks, and one four-dimensional TMA box brings them in the order 8 rows x 128 bytes, the next 128 bytes of
+// the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192: 16.0 us, 16.9 block by block). In shared memory the 1024-byte
+// atoms of a K block are then kBlocks apart, which is a stride of the operand descriptor. Matrices whose rows are no
+// multiple of 8, or whose row pitch is none of 128 bytes, go block by block (such a box could reach past the end of the
+// last row).
 
 template <int kFormat, int kCols>
 struct Fp4Tile {
@@ -400,7 +400,8 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
 //
 // Scales reach TMEM through registers: four warps of each CTA load them from shared memory and store them to their quarter
 // of the lanes, three K blocks ahead of the multiplies. Brought by tcgen05.cp they would stand in the tensor core's own
-// queue and cost it about 40 cycles per 512 bytes, six or twelve times per K block of 512 cycles (8192^3: 268 us against 202 with E8M0_32, 363 against 218 with E4M3_16).
+// queue and cost it about 40 cycles per 512 bytes, six or twelve times per K block of 512 cycles (8192^3: 268 us against
+// 202 with E8M0_32, 363 against 218 with E4M3_16).
 // A buffer is written again once the multiplies that read it have been committed.
 
 template <int kFormat>
@@ -761,17 +762,34 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
     }
 }
 
-// The K slices of every element in slice order, times the tensor scales.
+// The K slices of every element in slice order, times the tensor scales. kVec neighbours of a row per thread.
+template <int kVec>
 __global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ parts, int splits, long long m, long long n, const float* scale_a,
                                                    const float* scale_b, void* c, int c_type, long long ldc) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float alpha = product_scale(scale_a, scale_b);
     const long long count = m * n;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * 256) {
-        float sum = parts[i];
-        for (int z = 1; z < splits; ++z) sum += parts[z * count + i];
-        const long long r = i / n;
-        store_c(c, c_type, r * ldc + (i - r * n), sum * alpha);
+    const unsigned per_row = static_cast<unsigned>(n / kVec);
+    const long long r = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
+    if (r >= m) return;
+    for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < per_row; i += gridDim.x * 256) {
+        const float* from = parts + r * n + static_cast<long long>(i) * kVec;
+        float sum[kVec];
+        if constexpr (kVec == 4) {
+            float4 v = *reinterpret_cast<const float4*>(from);
+#pragma unroll 4
+            for (int z = 1; z < splits; ++z) {
+                const float4 w = *reinterpret_cast<const float4*>(from + z * count);
+                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+            }
+            sum[0] = v.x, sum[1] = v.y, sum[2] = v.z, sum[3] = v.w;
+        } else {
+            sum[0] = *from;
+            for (int z = 1; z < splits; ++z) sum[0] += from[z * count];
+        }
+        const long long at = r * ldc + static_cast<long long>(i) * kVec;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) store_c(c, c_type, at + j, sum[j] * alpha);
     }
 }
 
@@ -791,7 +809,8 @@ struct Plan {
 // tiles of 128 x 128; 1024^3: 12 against 23; 512 x 512 x 4096, four tiles: 13 against 18 with K split).
 //
 // K is split where less than 60 CTAs would work: at one token an SM draws some 70 GB/s, so 64 of them take 8192 x 8192
-// codes in as good a time as 128 halves of them and a second launch that joins the halves (14 against 16 us).
+// codes in as good a time as 128 halves of them and a second launch that joins the halves (14 against 16 us). With more than
+// 64 columns a CTA has twice as much to bring, and up to 74 tiles are halved (128 tokens, E4M3_16: 20 us, 23 whole).
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
@@ -804,7 +823,7 @@ Plan plan_for(long long m, long long n, long long k) {
     plan.tile_cols = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
     const long long tiles = (rows + 127) / 128;
     constexpr int kSms = 148;
-    const int splits = tiles < 60 ? static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4))) : 1;
+    const int splits = tiles < 60 || (plan.tile_cols == 128 && tiles <= kSms / 2) ? static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4))) : 1;
     const int stage = plan.tile_cols <= 32 ? 4 : 2;  // K blocks of a stage
     plan.per_split = ((plan.k_blocks + splits - 1) / splits + stage - 1) / stage * stage;
     plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
@@ -876,12 +895,12 @@ int encode_c(McTensorMap* map, void* c, int type, long long m, long long n, long
 }
 
 template <typename... Params, typename... Args>
-int launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, Args... args) {
+int launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, Args... args) {
     cudaLaunchAttribute attribute;
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid, 1, 1);
+    config.gridDim = grid;
     config.blockDim = dim3(threads, 1, 1);
     config.dynamicSmemBytes = smem;
     config.stream = s;
@@ -895,16 +914,8 @@ template <int kFormat, int kCols>
 int launch_one_cta(const McTensorMap& rows, const McTensorMap& cols, const Fp4GemmParams& p, unsigned grid, cudaStream_t s) {
     using Tile = Fp4Tile<kFormat, kCols>;
     static_assert(Tile::kSmem + 64 <= 227 * 1024, "shared memory");
-    static PerDeviceOnce configured;
-    int device = 0;
-    if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
-    if (configured.first_use(device)) {
-        if (int rc = check_rt(cudaFuncSetAttribute(mc_fp4_gemm<kFormat, kCols>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem),
-                              "cudaFuncSetAttribute(max dynamic shared memory)")) {
-            configured.forget(device);
-            return rc;
-        }
-    }
+    static SharedMemoryOnce once;
+    if (int rc = once.allow(mc_fp4_gemm<kFormat, kCols>, Tile::kSmem)) return rc;
     return launch_dependent(mc_fp4_gemm<kFormat, kCols>, grid, kOneCtaThreads, Tile::kSmem, s, "mc_fp4_gemm", rows, cols, p);
 }
 
@@ -922,16 +933,8 @@ template <int kFormat>
 int launch_pairs(const mcd_fp4_gemm_args* args, cudaStream_t s) {
     using Pair = Fp4Pair<kFormat>;
     static_assert(Pair::kSmem + 64 <= 227 * 1024, "shared memory");
-    static PerDeviceOnce configured;
-    int device = 0;
-    if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
-    if (configured.first_use(device)) {
-        if (int rc = check_rt(cudaFuncSetAttribute(mc_fp4_gemm_pair<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, Pair::kSmem),
-                              "cudaFuncSetAttribute(max dynamic shared memory)")) {
-            configured.forget(device);
-            return rc;
-        }
-    }
+    static SharedMemoryOnce once;
+    if (int rc = once.allow(mc_fp4_gemm_pair<kFormat>, Pair::kSmem)) return rc;
     McTensorMap rows, cols, row_scales, col_scales, c = {};
     if (int rc = encode_codes(&rows, args->a, 128)) return rc;
     if (int rc = encode_codes(&cols, args->b, 128)) return rc;
@@ -961,7 +964,10 @@ size_t plan_workspace(const Plan& plan, long long m, long long n) {
     return plan.splits > 1 ? static_cast<size_t>(plan.splits) * static_cast<size_t>(m) * static_cast<size_t>(n) * sizeof(float) : 0;
 }
 
-bool sized(const mcd_fp4_gemm_args* a) { return a != nullptr && a->a.rows > 0 && a->b.rows > 0 && a->a.cols > 0; }
+bool sized(const mcd_fp4_gemm_args* a) {
+    constexpr long long most = 2147483647LL;
+    return a != nullptr && a->a.rows > 0 && a->b.rows > 0 && a->a.cols > 0 && a->a.rows <= most && a->b.rows <= most && a->a.cols <= most;
+}
 
 }  // namespace
 
@@ -1040,7 +1046,10 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
         return rc;
     }
     if (plan.splits == 1) return 0;
-    const long long blocks = std::max<long long>(1, std::min<long long>((m * n + 255) / 256, 8LL * sm_count()));
-    return launch_dependent(mc_fp4_join, static_cast<unsigned>(blocks), 256, 0, s, "mc_fp4_join", static_cast<const float*>(p.workspace), plan.splits, m, n,
+    const bool vec = n % 4 == 0;
+    const long long per_row = vec ? n / 4 : n;
+    const auto join_rows = static_cast<unsigned>(std::min<long long>(m, 32768));
+    const dim3 join_grid(static_cast<unsigned>(std::min<long long>((per_row + 255) / 256, 1024)), join_rows, static_cast<unsigned>((m + join_rows - 1) / join_rows));
+    return launch_dependent(vec ? mc_fp4_join<4> : mc_fp4_join<1>, join_grid, 256, 0, s, "mc_fp4_join", static_cast<const float*>(p.workspace), plan.splits, m, n,
                             args->a.tensor_scale, args->b.tensor_scale, p.c, p.c_type, p.ldc);
 }

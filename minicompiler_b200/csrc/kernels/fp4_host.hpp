@@ -11,6 +11,7 @@
 #include <atomic>
 #include <cstdint>
 #include <initializer_list>
+#include <mutex>
 #include <string>
 
 namespace mcd {
@@ -35,6 +36,30 @@ inline int sm_count() {
     if (device >= 0 && device < 64) cached[device].store(sms, std::memory_order_relaxed);
     return sms;
 }
+
+// A kernel's opt-in to more than 48 KB of dynamic shared memory, once per device. Whoever comes while another thread is at
+// it waits for that to be done.
+class SharedMemoryOnce {
+public:
+    template <typename Kernel>
+    int allow(Kernel kernel, int bytes) {
+        int device = 0;
+        if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
+        std::lock_guard<std::mutex> lock(mutex_);
+        const bool kept = device >= 0 && device < 64;
+        if (kept && (done_ >> device & 1ull) != 0) return 0;
+        if (int rc = check_rt(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                              "cudaFuncSetAttribute(max dynamic shared memory)")) {
+            return rc;
+        }
+        if (kept) done_ |= 1ull << device;
+        return 0;
+    }
+
+private:
+    std::mutex mutex_;
+    unsigned long long done_ = 0;
+};
 
 // a * b * c <= limit, for non-negative numbers
 inline bool fits(long long a, long long b, long long c, long long limit) {

@@ -455,8 +455,9 @@ int rows_aligned(int type, const void* p, long long pitch) {
     return is_aligned(p, 32) && row % 32 == 0 ? 32 : is_aligned(p, 16) && row % 16 == 0 ? 16 : 0;
 }
 
-// Every launch is a programmatic dependent of what precedes it (each kernel says griddepcontrol.wait before its first access): a matrix of 8192 x 4096 f32 values and its scale, there and
-// back, takes 87 us instead of 93; a row of 2048 values, there and back and waited for, 8.2 instead of 10.3.
+// Every launch is a programmatic dependent of what precedes it (each kernel says griddepcontrol.wait before its first
+// access): a matrix of 8192 x 4096 f32 values and its scale, there and back, takes 87 us instead of 93; a row of 2048
+// values, there and back and waited for, 8.2 instead of 10.3.
 template <typename... Params, typename... Args>
 int launch(void (*kernel)(Params...), long long grid, unsigned threads, cudaStream_t s, const char* what, Args... args) {
     if (grid > 2147483647LL) return fail(std::string(what) + ": too many rows");
@@ -511,7 +512,7 @@ int tensor_scale_launch(const void* src, long long rows, long long cols, long lo
         vec = is_aligned(src, 32) ? 32 : is_aligned(src, 16) ? 16 : 0;
     }
     const long long units = rows * ((cols + kUnit - 1) / kUnit);
-    if (units <= 8192) {  // one per thread of a cluster
+    if (units <= 8192) {  // one per thread of a cluster; at four per thread (9 us) three launches on all SMs are as quick
         auto* kernel = vec == 32 ? mc_fp4_amax_one<T, 32> : vec == 16 ? mc_fp4_amax_one<T, 16> : mc_fp4_amax_one<T, 0>;
         return launch(kernel, 8LL * batch, 1024, s, "mc_fp4_amax_one", in, rows, cols, pitch, out);
     }

@@ -40,7 +40,6 @@
 #include "minicompiler_b200_device.h"
 
 #include "device/driver_api.hpp"
-#include "device/per_device.hpp"
 #include "kernels/fp4_format.cuh"
 #include "kernels/fp4_host.hpp"
 
@@ -75,7 +74,6 @@ struct Shape {
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
     static constexpr int kValueBytes = kTokenTile * kValuePitch;
     static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values, per thread and round
-    static constexpr int kUpGroups = 16 / kTiles;  // groups of rows of G (and of U) in 128
 };
 
 constexpr int kDownGroups = 2;  // groups of rows of y in 128
@@ -251,13 +249,16 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             started = true;
         }
-        if (e < p.experts && lane == 0) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(total) : "memory");
+        if (e < p.experts && lane == 0) {
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(logits_first + 8u * static_cast<unsigned>(e)), "d"(total) : "memory");
+        }
     }
     // Every CTA of the cluster knows the token's largest magnitude and brings its share of x to f16.
     largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));
     const float shift = power(shift_of(static_cast<int>(__float_as_uint(value16(static_cast<unsigned short>(largest), p.type)) >> 23)));
     for (int c = static_cast<int>(rank) * kRouterThreads + static_cast<int>(threadIdx.x); c < p.d_pitch; c += kRouterCluster * kRouterThreads) {
-        p.x16[token * static_cast<long long>(p.d_pitch) + c] = static_cast<unsigned short>(c < p.d ? pack_f16(value16(x[c], p.type) * shift, 0.0f) & 0xffffu : 0u);
+        const float v = c < p.d ? value16(x[c], p.type) * shift : 0.0f;
+        p.x16[token * static_cast<long long>(p.d_pitch) + c] = static_cast<unsigned short>(pack_f16(v, 0.0f) & 0xffffu);
     }
     if (rank == 0) {
         if (threadIdx.x == 0) p.x_shift[token] = shift;
@@ -567,7 +568,8 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 //   look(pass, here)          what a lane will need of its two columns, read before the multiplies
 //   done(pass, here, tile, side, acc)  a warp's sums, both halves of k
 template <int kFormat, int kHalves, int kGroups, int kStages, typename Work>
-__device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings, float4* halves) {
+__device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings,
+                                           float4* halves) {
     using S = Shape<kHalves, kGroups>;
     constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kPieces = S::kPieces, kValuePitch = S::kValuePitch;
     const int lane = threadIdx.x & 31, group = threadIdx.x / S::kGroupThreads;
@@ -637,7 +639,8 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * S::kGroupThreads + thread;
             const int n = piece / (kRoundK / 8);
-            if (n < here) *reinterpret_cast<uint4*>(to + n * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16) = work.finish(pieces[i]);
+            unsigned char* slot = to + n * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16;
+            if (n < here) *reinterpret_cast<uint4*>(slot) = work.finish(pieces[i]);
         }
         if (++value_round == m.rounds) {
             value_round = 0;
@@ -654,17 +657,18 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
             load_values();
             if (round >= 0) {
 #pragma unroll 1
-            for (int j = 0; j < kRoundSteps; ++j) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-                __syncwarp();
-                copy_next();  // into the slot of the step before, which all lanes have left
-                const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
-                if (s < m.stages) {
-                    multiply_step<kFormat, kValuePitch>(ring + slot * Stage<kFormat>::kBytes, values + buffer * S::kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
+                for (int j = 0; j < kRoundSteps; ++j) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                    __syncwarp();
+                    copy_next();  // into the slot of the step before, which all lanes have left
+                    const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
+                    if (s < m.stages) {
+                        multiply_step<kFormat, kValuePitch>(ring + slot * Stage<kFormat>::kBytes,
+                                                            values + buffer * S::kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
+                    }
+                    copies_end();
+                    if (++slot == kStages) slot = 0;
                 }
-                copies_end();
-                if (++slot == kStages) slot = 0;
-            }
             }
             buffer ^= 1;
             store_values(values + buffer * S::kValueBytes);
@@ -695,7 +699,8 @@ struct UpWork {
     using Piece = uint4;
     const MoeParams& p;
     const Routing& routing;
-    int groups;                    // of rows of an expert
+    static constexpr int kGroupsOf128 = 16 / S::kTiles;  // groups of rows of G (and of U) in 128
+    int groups;                                          // of rows of an expert
     int skip_active, skip_groups;  // gridDim.x items further on
 
     __device__ __forceinline__ UpWork(const MoeParams& params, const Routing& r) : p(params), routing(r), groups(params.f_groups / S::kTiles) {
@@ -719,7 +724,7 @@ struct UpWork {
     }
     // Rows that share 32 bytes of scales: two neighbours in each of the four groups of 32 of a 128-row tile.
     __device__ __forceinline__ int row_in_f(const Pass& pass, int tile, int g) const {
-        return pass.group / S::kUpGroups * 128 + 32 * (g >> 1) + 2 * S::kTiles * (pass.group % S::kUpGroups) + 2 * tile + (g & 1);
+        return pass.group / kGroupsOf128 * 128 + 32 * (g >> 1) + 2 * S::kTiles * (pass.group % kGroupsOf128) + 2 * tile + (g & 1);
     }
     // Rows 0 .. 7 of a tile are G's, 8 .. 15 the same of U.
     template <typename Rows>
@@ -1005,21 +1010,11 @@ int launch(void (*kernel)(Params...), unsigned grid, unsigned cluster, unsigned 
     return check_rt(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
 
-template <typename Kernel>
-int ready(PerDeviceOnce& once, Kernel kernel, int smem) {
-    int device = 0;
-    if (int rc = check_rt(cudaGetDevice(&device), "cudaGetDevice")) return rc;
-    if (!once.first_use(device)) return 0;
-    const int rc = check_rt(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(max dynamic shared memory)");
-    if (rc != 0) once.forget(device);
-    return rc;
-}
-
 template <int kFormat, int kHalves>
 int launch_up(MoeParams p, int reached, cudaStream_t s) {
     using S = Shape<kHalves, 1>;
-    static PerDeviceOnce once;
-    if (int rc = ready(once, mc_moe_up<kFormat, kHalves>, kUpSmem<kFormat, kHalves>)) return rc;
+    static SharedMemoryOnce once;
+    if (int rc = once.allow(mc_moe_up<kFormat, kHalves>, kUpSmem<kFormat, kHalves>)) return rc;
     p.gate_up.rounds = (p.d + S::kRoundK - 1) / S::kRoundK;
     const long long items = static_cast<long long>(reached) * (p.f_groups / S::kTiles);
     const auto grid = static_cast<unsigned>(std::min<long long>(items, 2LL * sm_count()));
@@ -1029,8 +1024,8 @@ int launch_up(MoeParams p, int reached, cudaStream_t s) {
 template <int kFormat, bool kMany, int kStages>
 int launch_down(MoeParams p, int reached, cudaStream_t s) {
     using S = DownShape<kMany>;
-    static PerDeviceOnce once;
-    if (int rc = ready(once, mc_moe_down<kFormat, kMany, kStages>, down_smem<kFormat, kMany, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
+    static SharedMemoryOnce once;
+    if (int rc = once.allow(mc_moe_down<kFormat, kMany, kStages>, down_smem<kFormat, kMany, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
     p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
     int cluster = 8;
     while (cluster > reached) cluster /= 2;

@@ -15,7 +15,8 @@ E4M3 = np.array([(b & 7) * 2.0 ** -9 if b < 8 else (1 + (b & 7) / 8.0) * 2.0 ** 
 
 
 def f32(x):
-    return np.asarray(x, dtype=np.float32).astype(np.float64)
+    with np.errstate(over="ignore"):
+        return np.asarray(x, dtype=np.float32).astype(np.float64)
 
 
 def nearest_even(x, table):
