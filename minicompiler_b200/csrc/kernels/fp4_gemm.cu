@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kTileRows = 128;   // TMEM lanes
 constexpr int kRaster = 16;      // row tiles per band of work items
+constexpr int kMaxCluster = 8;   // K slices that a cluster adds up
 
 struct Fp4GemmParams {
     // "rows" is the operand on the 128 TMEM lanes, "columns" the one whose rows are accumulator columns
@@ -47,8 +48,9 @@ struct Fp4GemmParams {
     int c_type;
     int rows, cols, k;
     int k_blocks, k_blocks_per_split, splits;
-    int swapped;  // 0: rows are C's rows; 1: rows are C's columns
-    int wide;     // the row operand's map is the four-dimensional one
+    int swapped;    // 0: rows are C's rows; 1: rows are C's columns
+    int wide;       // the row operand's map is the four-dimensional one
+    int clustered;  // the K slices of a tile are the CTAs of a cluster, one item per CTA, and are added up there
 };
 
 __device__ __forceinline__ void store_c(void* c, int type, long long at, float v) {
@@ -102,7 +104,7 @@ __device__ __forceinline__ float product_scale(const float* a, const float* b) {
 // accumulators while the other is being filled.
 //
 // What bounds it: few columns, that is few tokens, read the whole of the row operand once (16384 x 16384 E8M0_32 codes,
-// 143 MB: 41 to 50 us on different boxes; bringing them to shared memory and nothing else took 33, in one run or not, most
+// 143 MB: 41 to 50 us on different machines; bringing them to shared memory and nothing else took 33, in one run or not, most
 // of the rest is the ramp of one wave of CTAs). Neither the multiplies nor the copies of scales are felt. A stage takes two
 // or four K blocks, and one four-dimensional TMA box brings them in the order 8 rows x 128 bytes, the next 128 bytes of
 // the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192: 16.0 us, 16.9 block by block). In shared memory the 1024-byte
@@ -330,6 +332,22 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = rb * kTileRows + quarter * 32 + lane;
+            if (kCols <= 32 && p.clustered) {
+                // This CTA's multiplies are done, and with them its ring: the slice goes there, column by column.
+                for (int chunk = 0; chunk < kCols / kChunk; ++chunk) {
+                    unsigned v[kChunk];
+                    tmem_load16(tmem + (static_cast<unsigned>(quarter * 32) << 16) + static_cast<unsigned>(chunk * kChunk), v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(tiles_base + static_cast<unsigned>((chunk * kChunk + j) * kTileRows + quarter * 32 + lane) * 4u),
+                                     "r"(v[j])
+                                     : "memory");
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                break;
+            }
             const bool partial = p.splits > 1;
             void* dst = partial ? static_cast<void*>(p.workspace + split * m * n) : p.c;
             const long long ld = partial ? n : p.ldc;
@@ -378,6 +396,41 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
         }
     }
 
+    if (kCols <= 32 && p.clustered) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // Every CTA finishes the columns whose number is its rank modulo the cluster: slices in their order.
+        int rb, cb, rank;
+        fp4_decode_item(blockIdx.x, tiles_r, tiles_c, p.splits, rb, cb, rank);
+        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const int valid = min(kCols, p.cols - cb * kCols);
+        for (int i = threadIdx.x;; i += kOneCtaThreads) {
+            const int c = rank + i / kTileRows * p.splits, r = i % kTileRows;
+            if (c >= valid) break;
+            const int row = rb * kTileRows + r, col = cb * kCols + c;
+            if (row >= p.rows) continue;
+            const unsigned at = tiles_base + static_cast<unsigned>(c * kTileRows + r) * 4u;
+            float part[kMaxCluster];
+#pragma unroll
+            for (int z = 0; z < kMaxCluster; ++z) {
+                part[z] = 0.0f;
+                if (z < p.splits) {
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[z]) : "r"(cluster_address(at, static_cast<unsigned>(z))) : "memory");
+                }
+            }
+            float sum = part[0];
+#pragma unroll
+            for (int z = 1; z < kMaxCluster; ++z) {
+                if (z < p.splits) sum += part[z];
+            }
+            store_c(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row : static_cast<long long>(row) * p.ldc + col, sum * alpha);
+        }
+        // shared memory stays until the last of the cluster has read it
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -802,15 +855,20 @@ struct Plan {
     int splits = 1;
     int k_blocks = 1;
     int per_split = 1;
+    bool clustered = false;  // the slices of a tile meet in a cluster's shared memory
 };
 
 // Up to 128 rows or columns of C: the one-CTA kernel, the shorter side as accumulator columns, so that the longer one fills
 // the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192: 19 us, 36 in
 // tiles of 128 x 128; 1024^3: 12 against 23; 512 x 512 x 4096, four tiles: 13 against 18 with K split).
 //
-// K is split where less than 60 CTAs would work: at one token an SM draws some 70 GB/s, so 64 of them take 8192 x 8192
-// codes in as good a time as 128 halves of them and a second launch that joins the halves (14 against 16 us). With more than
-// 64 columns a CTA has twice as much to bring, and up to 74 tiles are halved (128 tokens, E4M3_16: 20 us, 23 whole).
+// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. With up to 32 accumulator
+// columns two to eight slices are the CTAs of one cluster, which adds them up from shared memory (one token, 8192 x 8192:
+// 11 us, 14 whole; 2048 x 2048: 8 us, 10.5 with a second launch that joins), as many as find SMs all at once: eight of 14
+// tiles, four of 32, three of 42. A second wave costs more than the slices give (32 tokens, 8192 columns of K, 16 tiles:
+// 8.7 us in clusters of four, 14 in clusters of eight; 34 tiles: 10.8 in threes, 16 in fours). Wider accumulators (128
+// tokens, 8192 x 8192: 18 us, 23 in a cluster) and the few tiles of a K that wants more than 24 slices go through the
+// workspace.
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
@@ -823,10 +881,20 @@ Plan plan_for(long long m, long long n, long long k) {
     plan.tile_cols = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
     const long long tiles = (rows + 127) / 128;
     constexpr int kSms = 148;
-    const int splits = tiles < 60 || (plan.tile_cols == 128 && tiles <= kSms / 2) ? static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4))) : 1;
     const int stage = plan.tile_cols <= 32 ? 4 : 2;  // K blocks of a stage
-    plan.per_split = ((plan.k_blocks + splits - 1) / splits + stage - 1) / stage * stage;
-    plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
+    auto split = [&](int splits) {
+        plan.per_split = ((plan.k_blocks + splits - 1) / splits + stage - 1) / stage * stage;
+        plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
+    };
+    const int most = static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4)));
+    if (plan.tile_cols > 32 || most > 3 * kMaxCluster) {
+        if (tiles < 60 || (plan.tile_cols == 128 && tiles <= kSms / 2)) split(most);
+        return plan;
+    }
+    auto fits = [&](int slices, int sms) { return slices <= most && tiles * slices <= sms; };
+    const int splits = fits(8, 112) ? 8 : fits(4, 128) ? 4 : fits(3, 128) ? 3 : fits(2, kSms) ? 2 : 1;
+    split(splits);
+    plan.clustered = plan.splits > 1;
     return plan;
 }
 
@@ -895,17 +963,21 @@ int encode_c(McTensorMap* map, void* c, int type, long long m, long long n, long
 }
 
 template <typename... Params, typename... Args>
-int launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, Args... args) {
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+int launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned cluster, unsigned threads, size_t smem, cudaStream_t s, const char* what, Args... args) {
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
     config.blockDim = dim3(threads, 1, 1);
     config.dynamicSmemBytes = smem;
     config.stream = s;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return check_rt(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
@@ -916,7 +988,7 @@ int launch_one_cta(const McTensorMap& rows, const McTensorMap& cols, const Fp4Ge
     static_assert(Tile::kSmem + 64 <= 227 * 1024, "shared memory");
     static SharedMemoryOnce once;
     if (int rc = once.allow(mc_fp4_gemm<kFormat, kCols>, Tile::kSmem)) return rc;
-    return launch_dependent(mc_fp4_gemm<kFormat, kCols>, grid, kOneCtaThreads, Tile::kSmem, s, "mc_fp4_gemm", rows, cols, p);
+    return launch_dependent(mc_fp4_gemm<kFormat, kCols>, grid, p.clustered ? p.splits : 1, kOneCtaThreads, Tile::kSmem, s, "mc_fp4_gemm", rows, cols, p);
 }
 
 template <int kFormat>
@@ -957,11 +1029,11 @@ int launch_pairs(const mcd_fp4_gemm_args* args, cudaStream_t s) {
     }
     const long long tiles = ((args->a.rows + kPairTile - 1) / kPairTile) * ((args->b.rows + kPairTile - 1) / kPairTile);
     const auto grid = 2 * static_cast<unsigned>(std::min<long long>(tiles, sm_count() / 2));
-    return launch_dependent(mc_fp4_gemm_pair<kFormat>, grid, kPairThreads, Pair::kSmem, s, "mc_fp4_gemm_pair", rows, cols, row_scales, col_scales, c, p);
+    return launch_dependent(mc_fp4_gemm_pair<kFormat>, grid, 1, kPairThreads, Pair::kSmem, s, "mc_fp4_gemm_pair", rows, cols, row_scales, col_scales, c, p);
 }
 
 size_t plan_workspace(const Plan& plan, long long m, long long n) {
-    return plan.splits > 1 ? static_cast<size_t>(plan.splits) * static_cast<size_t>(m) * static_cast<size_t>(n) * sizeof(float) : 0;
+    return plan.splits > 1 && !plan.clustered ? static_cast<size_t>(plan.splits) * static_cast<size_t>(m) * static_cast<size_t>(n) * sizeof(float) : 0;
 }
 
 bool sized(const mcd_fp4_gemm_args* a) {
@@ -978,7 +1050,8 @@ extern "C" size_t mcd_fp4_gemm_workspace(const mcd_fp4_gemm_args* args) {
 
 extern "C" int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args) {
     if (!sized(args)) return 0;
-    return plan_for(args->a.rows, args->b.rows, args->a.cols).splits > 1 ? 2 : 1;
+    const Plan plan = plan_for(args->a.rows, args->b.rows, args->a.cols);
+    return plan.splits > 1 && !plan.clustered ? 2 : 1;
 }
 
 extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
@@ -1039,17 +1112,18 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
     p.splits = plan.splits;
     p.swapped = plan.swapped ? 1 : 0;
     p.wide = wide ? 1 : 0;
+    p.clustered = plan.clustered ? 1 : 0;
     auto s = static_cast<cudaStream_t>(stream);
-    const auto grid = static_cast<unsigned>(std::min<long long>(items, sm_count()));
+    const auto grid = static_cast<unsigned>(plan.clustered ? items : std::min<long long>(items, sm_count()));
     if (int rc = args->a.format == MCD_FP4_E8M0_32 ? launch_format<MCD_FP4_E8M0_32>(plan.tile_cols, map_rows, map_cols, p, grid, s)
                                                    : launch_format<MCD_FP4_E4M3_16>(plan.tile_cols, map_rows, map_cols, p, grid, s)) {
         return rc;
     }
-    if (plan.splits == 1) return 0;
+    if (plan.splits == 1 || plan.clustered) return 0;
     const bool vec = n % 4 == 0;
     const long long per_row = vec ? n / 4 : n;
     const auto join_rows = static_cast<unsigned>(std::min<long long>(m, 32768));
     const dim3 join_grid(static_cast<unsigned>(std::min<long long>((per_row + 255) / 256, 1024)), join_rows, static_cast<unsigned>((m + join_rows - 1) / join_rows));
-    return launch_dependent(vec ? mc_fp4_join<4> : mc_fp4_join<1>, join_grid, 256, 0, s, "mc_fp4_join", static_cast<const float*>(p.workspace), plan.splits, m, n,
+    return launch_dependent(vec ? mc_fp4_join<4> : mc_fp4_join<1>, join_grid, 1, 256, 0, s, "mc_fp4_join", static_cast<const float*>(p.workspace), plan.splits, m, n,
                             args->a.tensor_scale, args->b.tensor_scale, p.c, p.c_type, p.ldc);
 }
