@@ -107,7 +107,7 @@ __device__ __forceinline__ float product_scale(const float* a, const float* b) {
 // 143 MB: 41 to 50 us on different machines; bringing them to shared memory and nothing else took 33, in one run or not, most
 // of the rest is the ramp of one wave of CTAs). Neither the multiplies nor the copies of scales are felt. A stage takes two
 // or four K blocks, and one four-dimensional TMA box brings them in the order 8 rows x 128 bytes, the next 128 bytes of
-// the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192: 16.0 us, 16.9 block by block). In shared memory the 1024-byte
+// the same rows, ..., the next 8 rows (64 tokens, 8192 x 8192, K whole: 16.0 us, 16.9 block by block). In shared memory the 1024-byte
 // atoms of a K block are then kBlocks apart, which is a stride of the operand descriptor. Matrices whose rows are no
 // multiple of 8, or whose row pitch is none of 128 bytes, go block by block (such a box could reach past the end of the
 // last row).
@@ -332,7 +332,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = rb * kTileRows + quarter * 32 + lane;
-            if (kCols <= 32 && p.clustered) {
+            if (p.clustered) {
                 // This CTA's multiplies are done, and with them its ring: the slice goes there, column by column.
                 for (int chunk = 0; chunk < kCols / kChunk; ++chunk) {
                     unsigned v[kChunk];
@@ -396,35 +396,65 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
         }
     }
 
-    if (kCols <= 32 && p.clustered) {
+    if (p.clustered) {
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        // Every CTA finishes the columns whose number is its rank modulo the cluster: slices in their order.
+        // Every CTA finishes its share of the columns, four rows of a column per thread: slices in their order.
         int rb, cb, rank;
         fp4_decode_item(blockIdx.x, tiles_r, tiles_c, p.splits, rb, cb, rank);
         const float alpha = product_scale(p.row_scale, p.col_scale);
         const int valid = min(kCols, p.cols - cb * kCols);
-        for (int i = threadIdx.x;; i += kOneCtaThreads) {
-            const int c = rank + i / kTileRows * p.splits, r = i % kTileRows;
-            if (c >= valid) break;
-            const int row = rb * kTileRows + r, col = cb * kCols + c;
-            if (row >= p.rows) continue;
-            const unsigned at = tiles_base + static_cast<unsigned>(c * kTileRows + r) * 4u;
-            float part[kMaxCluster];
+        const int share = (valid + p.splits - 1) / p.splits;
+        const int first = rank * share;
+        const int quads = max(0, min(share, valid - first)) * (kTileRows / 4);
+        const int bytes = p.c_type == MCD_TYPE_F32 ? 4 : 2;
+        const bool vec = p.swapped && ((reinterpret_cast<unsigned long long>(p.c) | static_cast<unsigned long long>(p.ldc * bytes)) & (4 * bytes - 1)) == 0;
+        constexpr int kAtOnce = 2;  // quads per thread and turn
+        for (int base = threadIdx.x; base < quads; base += kAtOnce * kOneCtaThreads) {
+            float4 part[kAtOnce][kMaxCluster];
 #pragma unroll
-            for (int z = 0; z < kMaxCluster; ++z) {
-                part[z] = 0.0f;
-                if (z < p.splits) {
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[z]) : "r"(cluster_address(at, static_cast<unsigned>(z))) : "memory");
+            for (int u = 0; u < kAtOnce; ++u) {
+                const unsigned at = tiles_base + static_cast<unsigned>(first * (kTileRows / 4) + min(base + u * kOneCtaThreads, quads - 1)) * 16u;
+#pragma unroll
+                for (int z = 0; z < kMaxCluster; ++z) {
+                    if (z < p.splits) {
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(part[u][z].x), "=f"(part[u][z].y), "=f"(part[u][z].z), "=f"(part[u][z].w)
+                                     : "r"(cluster_address(at, static_cast<unsigned>(z)))
+                                     : "memory");
+                    }
                 }
             }
-            float sum = part[0];
 #pragma unroll
-            for (int z = 1; z < kMaxCluster; ++z) {
-                if (z < p.splits) sum += part[z];
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int q = base + u * kOneCtaThreads;
+                const int row = rb * kTileRows + q % (kTileRows / 4) * 4, col = cb * kCols + first + q / (kTileRows / 4);
+                if (q >= quads || row >= p.rows) continue;
+                float sum[4] = {part[u][0].x, part[u][0].y, part[u][0].z, part[u][0].w};
+#pragma unroll
+                for (int z = 1; z < kMaxCluster; ++z) {
+                    if (z < p.splits) sum[0] += part[u][z].x, sum[1] += part[u][z].y, sum[2] += part[u][z].z, sum[3] += part[u][z].w;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] *= alpha;
+                if (vec && row + 4 <= p.rows) {
+                    const long long to = static_cast<long long>(col) * p.ldc + row;
+                    if (p.c_type == MCD_TYPE_F32) {
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.c) + to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                    } else {
+                        *reinterpret_cast<uint2*>(static_cast<unsigned short*>(p.c) + to) =
+                            make_uint2(pack_half2(sum[0], sum[1], p.c_type), pack_half2(sum[2], sum[3], p.c_type));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (row + j < p.rows) {
+                            store_c(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row + j : static_cast<long long>(row + j) * p.ldc + col, sum[j]);
+                        }
+                    }
+                }
             }
-            store_c(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row : static_cast<long long>(row) * p.ldc + col, sum * alpha);
         }
         // shared memory stays until the last of the cluster has read it
         __syncwarp();
@@ -862,13 +892,13 @@ struct Plan {
 // the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192: 19 us, 36 in
 // tiles of 128 x 128; 1024^3: 12 against 23; 512 x 512 x 4096, four tiles: 13 against 18 with K split).
 //
-// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. With up to 32 accumulator
-// columns two to eight slices are the CTAs of one cluster, which adds them up from shared memory (one token, 8192 x 8192:
-// 11 us, 14 whole; 2048 x 2048: 8 us, 10.5 with a second launch that joins), as many as find SMs all at once: eight of 14
-// tiles, four of 32, three of 42. A second wave costs more than the slices give (32 tokens, 8192 columns of K, 16 tiles:
-// 8.7 us in clusters of four, 14 in clusters of eight; 34 tiles: 10.8 in threes, 16 in fours). Wider accumulators (128
-// tokens, 8192 x 8192: 18 us, 23 in a cluster) and the few tiles of a K that wants more than 24 slices go through the
-// workspace.
+// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. Two to eight slices are
+// the CTAs of one cluster, which adds them up from shared memory, as many as find SMs all at once: eight of 14 tiles, four
+// of 32, three of 42 (one token, 8192 x 8192: 11 us, 14 whole; 128 tokens: 14, 18 through a workspace and a second launch;
+// 2048 x 2048: 8 and 10.5). A second wave costs more than the slices give (32 tokens, 8192 columns of K, 16 tiles: 8.7 us in
+// clusters of four, 14 in clusters of eight; 34 tiles: 10.8 in threes, 16 in fours). A long K with few tiles has too few
+// CTAs that way and goes through the workspace (128 rows, one token, K 131072: 21 us, 24 in a cluster; two to four times
+// 128 rows: 16, 25; up to 65536 the cluster takes as long or less).
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
@@ -887,8 +917,8 @@ Plan plan_for(long long m, long long n, long long k) {
         plan.splits = (plan.k_blocks + plan.per_split - 1) / plan.per_split;
     };
     const int most = static_cast<int>(std::max<long long>(1, std::min<long long>(kSms / tiles, plan.k_blocks / 4)));
-    if (plan.tile_cols > 32 || most > 3 * kMaxCluster) {
-        if (tiles < 60 || (plan.tile_cols == 128 && tiles <= kSms / 2)) split(most);
+    if (tiles <= 6 && plan.k_blocks > 256) {
+        split(most);
         return plan;
     }
     auto fits = [&](int slices, int sms) { return slices <= most && tiles * slices <= sms; };
