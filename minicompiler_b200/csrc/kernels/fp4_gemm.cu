@@ -381,10 +381,18 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) turn[lane * 17 + j] = __uint_as_float(v[j]) * scale;
                     __syncwarp();
+                    const int c = col0 + (lane & 15);
+                    const int first = row - lane + (lane >> 4);
+#pragma unroll 1
+                    for (int i = 0; i < 16; i += 8) {
+                        float value[8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = row - lane + 2 * i + (lane >> 4), c = col0 + (lane & 15);
-                        if (r < p.rows && c < p.cols) store_c(dst, type, static_cast<long long>(r) * ld + c, turn[(2 * i + (lane >> 4)) * 17 + (lane & 15)]);
+                        for (int j = 0; j < 8; ++j) value[j] = turn[(2 * (i + j) + (lane >> 4)) * 17 + (lane & 15)];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = first + 2 * (i + j);
+                            if (r < p.rows && c < p.cols) store_c(dst, type, static_cast<long long>(r) * ld + c, value[j]);
+                        }
                     }
                 }
             }
@@ -509,6 +517,90 @@ struct Fp4Pair {
     static_assert(kScaleBuffers * kScaleColumns <= kOverlap, "TMEM columns");
 };
 
+// A lane's 32 values, the row `lane` of a box of 32 x 32, to shared memory as a TMA store wants them: rows of 128 bytes (f32,
+// 128-byte swizzle) or of 64 (16 bits, 64-byte swizzle).
+__device__ __forceinline__ void stage_row(unsigned at, const unsigned (&v)[32], float alpha, int type) {
+    unsigned lane = threadIdx.x & 31;
+    asm volatile("" : "+r"(lane));  // addresses made here and not kept: nothing of this is worth registers between tiles
+    float f[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
+    if (type == MCD_TYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((j ^ (lane & 7)) << 4)), "f"(f[4 * j]), "f"(f[4 * j + 1]),
+                         "f"(f[4 * j + 2]), "f"(f[4 * j + 3])
+                         : "memory");
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                         "r"(pack_half2(f[8 * j], f[8 * j + 1], type)), "r"(pack_half2(f[8 * j + 2], f[8 * j + 3], type)),
+                         "r"(pack_half2(f[8 * j + 4], f[8 * j + 5], type)), "r"(pack_half2(f[8 * j + 6], f[8 * j + 7], type))
+                         : "memory");
+        }
+    }
+}
+
+// Such a box to rows of C that start anywhere: a warp writes a row, or, where all 16-bit rows start on words, two of them.
+// `rows` and `cols` of the box exist. Instructions are what this costs, so eight rows are read ahead of their stores, and
+// the addresses in shared memory are constants beside two of the lane's (37728 x 1883 of bf16, K 128, 142 MB of C: 60 us,
+// 51 for 1884 columns; TMA takes 38 for 1888).
+__device__ __forceinline__ void store_box(unsigned at, void* c, int type, long long first, long long ldc, int rows, int cols) {
+    int lane = static_cast<int>(threadIdx.x & 31);
+    asm volatile("" : "+r"(lane));  // addresses made here and not kept: nothing of this is worth registers between tiles
+    if (type == MCD_TYPE_F32) {
+        float* to = static_cast<float*>(c) + first + lane;
+        const int mine = lane < cols ? rows : 0;
+#pragma unroll
+        for (int r = 0; r < 32; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[j]) : "r"(at + ((((lane >> 2) ^ j) << 4) + (lane & 3) * 4) + (r + j) * 128) : "memory");
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j, to += ldc) {
+                if (r + j < mine) *to = v[j];
+            }
+        }
+        return;
+    }
+    unsigned short* to = static_cast<unsigned short*>(c) + first;
+    if (cols >= 32 && ((reinterpret_cast<unsigned long long>(to) >> 1 | static_cast<unsigned long long>(ldc)) & 1) == 0) {
+        const int i = lane & 15, mine = rows - (lane >> 4);
+        to += (lane >> 4) * ldc + 2 * i;
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+            unsigned v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[j]) : "r"(at + (lane >> 4) * 64 + (((i >> 2) ^ (j & 3)) << 4) + (i & 3) * 4 + (k + j) * 128) : "memory");
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j, to += 2 * ldc) {
+                if (2 * (k + j) < mine) *reinterpret_cast<unsigned*>(to) = v[j];
+            }
+        }
+        return;
+    }
+    to += lane;
+    const int mine = lane < cols ? rows : 0;
+#pragma unroll
+    for (int r = 0; r < 32; r += 8) {
+        unsigned short v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[j]) : "r"(at + (((lane >> 3) ^ ((j >> 1) & 3)) << 4) + (lane & 7) * 2 + (r + j) * 64) : "memory");
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j, to += ldc) {
+            if (r + j < mine) *to = v[j];
+        }
+    }
+}
+
 constexpr int kPairThreads = 64 + 8 * 32 + 4 * 32;
 constexpr int kPairTile = 256;
 
@@ -520,7 +612,7 @@ struct Fp4PairParams {
     long long ldc;
     int c_type;
     int m, n, k, k_blocks;
-    int by_tma;  // C leaves as TMA boxes; otherwise (alignment) straight from registers
+    int by_tma;  // C leaves as TMA boxes; otherwise (alignment) row by row
 };
 
 template <int kFormat>
@@ -750,83 +842,70 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
             // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
             // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
             auto chunk_at = [&](int i) { return acc ? i : 7 - i; };
-            auto finish = [&](unsigned* v, int chunk) {
-                const int col0 = cb * kPairTile + chunk * 32;
-                if (col0 >= p.n) return;  // warp-uniform
-                float f[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
-                // A box that reaches over the last column is not left to TMA, which cuts rows off at 16 bytes: what lies behind
-                // C's columns inside ldc is not ours.
-                if (p.by_tma && col0 + 32 <= p.n) {
-                    // 32 x 32 boxes through this warp's staging buffer: rows of 128 bytes (f32, 128-byte swizzle) or of 64
-                    // (16 bits, 64-byte swizzle; two boxes take turns in the buffer's halves)
-                    if (p.c_type == MCD_TYPE_F32) {
-                        if (lane == 0) tma_store_wait_read<0>();
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + ((j ^ (lane & 7)) << 4)), "f"(f[4 * j]),
-                                         "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3])
-                                         : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) tma_store_2d(&map_c, buffer, col0, row0);
-                    } else {
-                        const unsigned at = buffer + (turn & 1u) * 2048u;
-                        ++turn;
-                        if (lane == 0) tma_store_wait_read<1>();
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
-                                         "r"(pack_half2(f[8 * j], f[8 * j + 1], p.c_type)), "r"(pack_half2(f[8 * j + 2], f[8 * j + 3], p.c_type)),
-                                         "r"(pack_half2(f[8 * j + 4], f[8 * j + 5], p.c_type)), "r"(pack_half2(f[8 * j + 6], f[8 * j + 7], p.c_type))
-                                         : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
-                    }
-                } else {
-                    // turned round in the staging buffer (the swizzle keeps both ways free of bank conflicts): a warp writes a row
-                    if (lane == 0) tma_store_wait_read<0>();
+            // Boxes that reach over the last column are not left to TMA, which cuts rows off at 16 bytes: what lies behind C's
+            // columns inside ldc is not ours.
+            if (!p.by_tma || (p.n % 32 != 0 && (cb + 1) * kPairTile > p.n)) {
+                if (lane == 0) tma_store_wait_read<0>();
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const int chunk = chunk_at(2 * i + half), col0 = cb * kPairTile + chunk * 32;
+                    unsigned w[32];
+                    tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(buffer + (lane * 32 + (j ^ lane)) * 4), "f"(f[j]) : "memory");
-                    }
+                    if (i == 3 && lane == 0) mbar_arrive_cluster(acc_empty);
+                    if (col0 >= p.n || row0 >= p.m) continue;  // warp-uniform
+                    stage_row(buffer, w, alpha, p.c_type);
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < p.m; ++r) {
-                        float value;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value) : "r"(buffer + (r * 32 + (lane ^ r)) * 4) : "memory");
-                        if (col0 + lane < p.n) store_c(p.c, p.c_type, static_cast<long long>(row0 + r) * p.ldc + col0 + lane, value);
-                    }
+                    store_box(buffer, p.c, p.c_type, static_cast<long long>(row0) * p.ldc + col0, p.ldc, p.m - row0, p.n - col0);
                     __syncwarp();
                 }
+                acc ^= 1;
+                continue;
+            }
+            auto finish = [&](const unsigned (&v)[32], int chunk) {
+                const int col0 = cb * kPairTile + chunk * 32;
+                if (col0 >= p.n) return;  // warp-uniform
+                // boxes of 16 bits take turns in the halves of this warp's buffer
+                unsigned at = buffer;
+                if (p.c_type == MCD_TYPE_F32) {
+                    if (lane == 0) tma_store_wait_read<0>();
+                } else {
+                    at += (turn & 1u) * 2048u;
+                    ++turn;
+                    if (lane == 0) tma_store_wait_read<1>();
+                }
+                __syncwarp();
+                stage_row(at, v, alpha, p.c_type);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
             };
+            // The shared chunks are read before anything else; where a warp has three of them, the first leaves meanwhile (three
+            // in registers spill).
             constexpr int kFirst = (Pair::kOverlapChunks + 1) / 2;  // shared chunks of the warps with half == 0
-            unsigned v[kFirst][32];
+            unsigned v[2][32];
 #pragma unroll
             for (int i = 0; i < kFirst; ++i) {
-                if (2 * i + half < Pair::kOverlapChunks) tmem_load32(lanes + static_cast<unsigned>(chunk_at(2 * i + half) * 32), v[i]);
+                if (i == 2) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    finish(v[0], chunk_at(half));
+                }
+                if (2 * i + half < Pair::kOverlapChunks) tmem_load32(lanes + static_cast<unsigned>(chunk_at(2 * i + half) * 32), v[i & 1]);
             }
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_empty);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = kFirst == 3 ? 1 : 0; i < 4; ++i) {
                 const int order = 2 * i + half;
-                if (i < kFirst && order < Pair::kOverlapChunks) {
-                    finish(v[i < kFirst ? i : 0], chunk_at(order));
-                } else {
-                    unsigned w[32];
-                    tmem_load32(lanes + static_cast<unsigned>(chunk_at(order) * 32), w);
+                if (order >= Pair::kOverlapChunks) {
+                    tmem_load32(lanes + static_cast<unsigned>(chunk_at(order) * 32), v[i & 1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    finish(w, chunk_at(order));
                 }
+                finish(v[i & 1], chunk_at(order));
             }
             acc ^= 1;
         }

@@ -150,7 +150,8 @@ def test_normal_data_within_the_bound(mc, ref, fmt, dtype, m, n, k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
 @pytest.mark.parametrize("m, n, ldc, offset", [(20, 100, 101, 1), (20, 100, 104, 8), (200, 100, 131, 3), (300, 256, 264, 16), (200, 128, 128, 1), (2100, 1300, 1301, 1),
-                                               (2100, 1300, 1304, 16), (2100, 1300, 1304, 1)])
+                                               (2100, 1300, 1304, 16), (2100, 1300, 1304, 1), (1537, 1285, 1286, 2),
+                                               (1537, 1285, 1285, 0), (1537, 1285, 1286, 3), (700, 1100, 1104, 8)])
 def test_only_c_is_written(mc, ref, dtype, m, n, ldc, offset):
     rng = np.random.default_rng(ldc)
     a, b = _exact_operand(mc, ref, rng, m, 96, "e8m0_32"), _exact_operand(mc, ref, rng, n, 96, "e8m0_32")
