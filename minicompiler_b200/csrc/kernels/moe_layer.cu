@@ -9,8 +9,8 @@
 //
 //   mc_moe_router  one cluster of 8 CTAs per token: logits in double-length sums, softmax, the top_k experts; x to f16
 //   mc_moe_up      8-warp CTAs take (expert, 32 or 64 rows of G and the same of U): h = silu(G x) * (U x), f16
-//   mc_moe_level   (many slots) h of a token and expert to one power of two
-//   mc_moe_down    a cluster of up to 8 CTAs takes 64 rows of y, its CTAs share the experts and add up what they found
+//   mc_moe_level   (where many CTAs read it) h of a token and expert to one power of two
+//   mc_moe_down    a cluster of up to 8 CTAs takes 64 or 32 rows of y, its CTAs share the experts and add up what they found
 //
 // Where the time goes: for one token and 8 of 64 experts (26.7 MB of weights, 4 us to read) 25 us are the latencies of
 // three dependent launches - routing, first copies, one round of multiplies, joining, each a microsecond or two. For 32
@@ -61,24 +61,21 @@ constexpr int kMaxSlots = MCD_MOE_MAX_TOKENS * MCD_MOE_MAX_TOP_K;
 
 // How a CTA's warps divide their work: tiles of 16 rows, and halves of the columns of a round. With two halves there are
 // twice as many, shorter passes: for a few tokens, which could not occupy the SMs otherwise. With one, what a pass costs
-// beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns. Two groups
-// of four warps go through passes of their own, each with its barrier: the down projection's form of that, whose CTAs
-// must not grow beyond 64 rows.
+// beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns. Groups of
+// four or of two warps go through passes of their own, each with its barrier: the down projection's form of that, whose
+// CTAs must not grow beyond 64 rows.
 template <int kHalves, int kGroups>
 struct Shape {
     static constexpr int kGroupWarps = kWarps / kGroups;
     static constexpr int kGroupThreads = kGroupWarps * 32;
     static constexpr int kTiles = kGroupWarps / kHalves;
-    static constexpr int kRoundSteps = kHalves * kGroups == 1 ? 4 : 2;  // per warp
+    static constexpr int kRoundSteps = kHalves * kGroups == 1 ? 4 : kGroups == 4 ? 1 : 2;  // per warp
     static constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
     static constexpr int kValueBytes = kTokenTile * kValuePitch;
     static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values, per thread and round
 };
 
-constexpr int kDownGroups = 2;  // groups of rows of y in 128
-constexpr int kDownRows = 128 / kDownGroups;
-constexpr int kDownPitch = kDownRows + 4;
 constexpr int kRouterCluster = 8;
 constexpr int kRouterThreads = 256;
 constexpr int kUpStages = 4;  // depth of a warp's ring
@@ -803,15 +800,21 @@ template <int kFormat>
 constexpr int ring_bytes(int stages) { return kWarps * stages * Stage<kFormat>::kBytes; }
 template <int kFormat, int kHalves>
 constexpr int kUpSmem = 2 * Shape<kHalves, 1>::kValueBytes + ring_bytes<kFormat>(kUpStages);
-// The down projection in one of two forms. kMany false: the halves of a round, all warps on one expert after the other, h as
-// mc_moe_up left it. kMany true: two groups of warps on experts of their own, h levelled before by mc_moe_level (32 tokens
-// of 128 experts of 2048 x 768: 40 us against 45), rings as deep as the sums beside them allow.
-template <bool kMany>
-using DownShape = Shape<kMany ? 1 : 2, kMany ? 2 : 1>;
-template <int kFormat, bool kMany, int kStages>
+// The down projection in one of three forms, by groups of warps. One group: the halves of a round, all warps on one expert after the
+// other, h as mc_moe_up left it. Two groups on experts of their own, h levelled before by mc_moe_level (32 tokens of 128
+// experts of 2048 x 768: 40 us against 45), rings as deep as the sums beside them allow. Four, of two warps and 32 rows of y,
+// for few rows of y, which leave SMs without work otherwise (the layer, 64 tokens, 8 of 64 experts of 1024 x 1024: 86 us
+// against 101; 32 tokens, 1024 x 512: 44 against 48; 4 tokens, 1024 x 1024: 37 against 40). Eight of one warp were slower
+// throughout: nothing is shared among rows then.
+template <int kGroups>
+struct DownShape : Shape<kGroups == 1 ? 2 : 1, kGroups> {
+    static constexpr int kRows = DownShape::kTiles * 16;
+    static constexpr int kRowGroups = 128 / kRows;  // in 128 rows of y
+    static constexpr int kPitch = kRows + 4;
+};
+template <int kFormat, int kGroups, int kStages>
 constexpr int down_smem(int tokens) {
-    constexpr int groups = kMany ? 2 : 1;
-    return groups * (tokens * kDownPitch * 4 + 2 * DownShape<kMany>::kValueBytes) + ring_bytes<kFormat>(kStages);
+    return kGroups * (tokens * DownShape<kGroups>::kPitch * 4 + 2 * DownShape<kGroups>::kValueBytes) + ring_bytes<kFormat>(kStages);
 }
 
 template <int kFormat, int kHalves>
@@ -856,10 +859,11 @@ __global__ void __launch_bounds__(128) mc_moe_level(const MoeParams p) {
     }
 }
 
-// kLevel: h lies as mc_moe_level left it, one power of two per slot; otherwise as mc_moe_up did, one per tile of 8 rows.
-template <bool kLevel>
+// One group: h lies as mc_moe_up left it, one power of two per tile of 8 rows; several: as mc_moe_level did, one per slot.
+template <int kGroups>
 struct DownWork {
-    using S = DownShape<kLevel>;
+    using S = DownShape<kGroups>;
+    static constexpr bool kLevel = kGroups > 1;
     struct Piece {
         uint4 raw;
         unsigned exponents;
@@ -867,7 +871,7 @@ struct DownWork {
     };
     const MoeParams& p;
     const Routing& routing;
-    float* sums;  // [tokens][kDownPitch]
+    float* sums;  // [tokens][kPitch]
     int group;    // of rows of y: their share of each group of 32 of a 128-row tile
     int first, step;
 
@@ -886,7 +890,7 @@ struct DownWork {
     }
     // Row i of a tile: four neighbours in each group of 32, so that a warp uses 64 of 128 bytes of scales, the tile beside it the rest.
     __device__ __forceinline__ int row_in_y(int tile, int i) const {
-        return group / kDownGroups * 128 + 32 * (i >> 2) + 4 * S::kTiles * (group % kDownGroups) + 4 * tile + (i & 3);
+        return group / S::kRowGroups * 128 + 32 * (i >> 2) + 4 * S::kTiles * (group % S::kRowGroups) + 4 * tile + (i & 3);
     }
     template <typename Rows>
     __device__ __forceinline__ void aim(Rows& rows, const Pass& pass, int tile) const {
@@ -935,7 +939,7 @@ struct DownWork {
         for (int j = 0; j < 2; ++j) {
             if (2 * t + j < here) {
                 // this warp's 16 columns; nobody else adds to them
-                float* sum = sums + side.token[j] * kDownPitch + tile * 16;
+                float* sum = sums + side.token[j] * S::kPitch + tile * 16;
                 sum[g] += side.weight[j] * (acc[j] * side.back[j]);
                 sum[g + 8] += side.weight[j] * (acc[2 + j] * side.back[j]);
             }
@@ -943,32 +947,31 @@ struct DownWork {
     }
 };
 
-template <int kFormat, bool kMany, int kStages>
+template <int kFormat, int groups, int kStages>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
-    using S = DownShape<kMany>;
-    constexpr int groups = kMany ? 2 : 1;
+    using S = DownShape<groups>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
     __shared__ float4 halves[kWarps / 2 * 32];
     unsigned char* values = smem;
     unsigned char* rings = values + groups * 2 * S::kValueBytes;
-    float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kStages));  // [groups][tokens][kDownPitch]
-    const int group_sums = p.tokens * kDownPitch;
+    float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kStages));  // [groups][tokens][kPitch]
+    const int group_sums = p.tokens * S::kPitch;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int rows = blockIdx.x / cluster;  // which 64
+    const int rows = blockIdx.x / cluster;  // which 64 or 32
     const int mine = threadIdx.x / S::kGroupThreads;
     for (int i = threadIdx.x; i < groups * group_sums; i += kThreads) sums[i] = 0.0f;
     load_routing(routing, reinterpret_cast<int*>(values), p);
-    DownWork<kMany> work{p, routing, sums + mine * group_sums, rows, rank * groups + mine, cluster * groups};
-    run_passes<kFormat, kMany ? 1 : 2, groups, kStages>(work, p.down, routing, values, rings, halves);
+    DownWork<groups> work{p, routing, sums + mine * group_sums, rows, rank * groups + mine, cluster * groups};
+    run_passes<kFormat, groups == 1 ? 2 : 1, groups, kStages>(work, p.down, routing, values, rings, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
     // Every CTA of the cluster finishes its share of the elements: the partial sums in the order of ranks and groups.
     const unsigned sums_at = smem_u32(sums);
-    const int count = p.tokens * kDownRows;
+    const int count = p.tokens * S::kRows;
     for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < count; i += cluster * kThreads) {
-        const int token = i / kDownRows, c = i - token * kDownRows;
-        const unsigned at = sums_at + static_cast<unsigned>(token * kDownPitch + c) * 4u;
+        const int token = i / S::kRows, c = i - token * S::kRows;
+        const unsigned at = sums_at + static_cast<unsigned>(token * S::kPitch + c) * 4u;
         float v = 0.0f;
         for (int z = 0; z < cluster; ++z) {
 #pragma unroll
@@ -980,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, in
                                  : "r"(peer_address(at + static_cast<unsigned>(g * group_sums * 4), static_cast<unsigned>(z)))
                                  : "memory");
                 } else {
-                    part = sums[g * group_sums + token * kDownPitch + c];
+                    part = sums[g * group_sums + token * S::kPitch + c];
                 }
                 v += part;
             }
@@ -1032,16 +1035,17 @@ int launch_up(MoeParams p, int reached, cudaStream_t s) {
     return launch(mc_moe_up<kFormat, kHalves>, grid, 1, kThreads, kUpSmem<kFormat, kHalves>, s, "mc_moe_up", p);
 }
 
-template <int kFormat, bool kMany, int kStages>
+template <int kFormat, int kGroups, int kStages>
 int launch_down(MoeParams p, int reached, cudaStream_t s) {
-    using S = DownShape<kMany>;
+    using S = DownShape<kGroups>;
+    static_assert(down_smem<kFormat, kGroups, kStages>(MCD_MOE_MAX_TOKENS) + 10 * 1024 <= 227 * 1024, "shared memory");
     static SharedMemoryOnce once;
-    if (int rc = once.allow(mc_moe_down<kFormat, kMany, kStages>, down_smem<kFormat, kMany, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
+    if (int rc = once.allow(mc_moe_down<kFormat, kGroups, kStages>, down_smem<kFormat, kGroups, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
     p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
     int cluster = 8;
     while (cluster > reached) cluster /= 2;
-    const auto grid = static_cast<unsigned>((p.d + 127) / 128 * kDownGroups * cluster);
-    return launch(mc_moe_down<kFormat, kMany, kStages>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat, kMany, kStages>(p.tokens), s,
+    const auto grid = static_cast<unsigned>((p.d + 127) / 128 * S::kRowGroups * cluster);
+    return launch(mc_moe_down<kFormat, kGroups, kStages>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat, kGroups, kStages>(p.tokens), s,
                   "mc_moe_down", p, cluster);
 }
 
@@ -1052,10 +1056,13 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     const int reached = std::min(p.experts, p.tokens * p.top_k);
     const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2, 1>::kTiles) > 4LL * sm_count();
     if (int rc = many ? launch_up<kFormat, 1>(p, reached, s) : launch_up<kFormat, 2>(p, reached, s)) return rc;
+    // Four groups per CTA where their clusters find SMs all at once, two CTAs on each, and there are experts for the groups.
+    const bool spread = p.d <= 1024 && reached >= 24;
     // A launch of its own for h pays where many CTAs would each level the same rows of it: 32 row groups for every 2048 of d.
-    if (p.tokens * p.top_k <= 32) return launch_down<kFormat, false, 3>(p, reached, s);
+    if (p.tokens * p.top_k <= 32 && !spread) return launch_down<kFormat, 1, 3>(p, reached, s);
     if (int rc = launch(mc_moe_level, static_cast<unsigned>(p.tokens * p.top_k), 1, 128, 0, s, "mc_moe_level", p)) return rc;
-    return p.tokens <= 32 ? launch_down<kFormat, true, 3>(p, reached, s) : launch_down<kFormat, true, 2>(p, reached, s);
+    if (spread) return p.tokens <= 32 ? launch_down<kFormat, 4, 3>(p, reached, s) : launch_down<kFormat, 4, 2>(p, reached, s);
+    return p.tokens <= 32 ? launch_down<kFormat, 2, 3>(p, reached, s) : launch_down<kFormat, 2, 2>(p, reached, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }

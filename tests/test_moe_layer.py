@@ -191,7 +191,8 @@ class Problem:
 @pytest.mark.parametrize("tokens, experts, top_k, d, f", [
     (1, 1, 1, 32, 32), (1, 4, 2, 64, 96), (1, 8, 8, 256, 128), (2, 5, 1, 33, 17), (3, 16, 4, 130, 77), (7, 13, 3, 300, 721), (9, 40, 6, 512, 260),
     (16, 8, 2, 129, 128), (33, 6, 3, 96, 40), (64, 4, 4, 64, 64), (64, 64, 16, 96, 48), (1, 512, 16, 40, 24), (5, 8, 2, 1100, 1300),
-    (40, 100, 6, 200, 260), (64, 90, 12, 97, 770), (21, 200, 9, 540, 390),
+    (40, 100, 6, 200, 260), (64, 90, 12, 97, 770), (21, 200, 9, 540, 390), (20, 12, 5, 300, 200), (9, 40, 6, 1100, 260), (6, 30, 5, 1024, 300),
+    (3, 63, 8, 448, 700), (37, 40, 8, 1030, 140),
 ])
 def test_layer(mc, ref, fmt, dtype, tokens, experts, top_k, d, f):
     Problem(mc, ref, fmt=fmt, dtype=dtype, tokens=tokens, experts=experts, top_k=top_k, d=d, f=f, renormalize=tokens % 2 == 1, seed=d + f).check()
