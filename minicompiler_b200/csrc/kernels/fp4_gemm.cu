@@ -93,6 +93,22 @@ __device__ __forceinline__ void store_row16(void* c, int type, long long at, con
     }
 }
 
+// Four values at `at`, `at + step`, ...; step 1 and `vec`: aligned for one store. `left` of them exist.
+__device__ __forceinline__ void store_quad(void* c, int type, long long at, long long step, const float (&f)[4], bool vec, int left) {
+    if (vec && left >= 4) {
+        if (type == MCD_TYPE_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(c) + at) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+            *reinterpret_cast<uint2*>(static_cast<unsigned short*>(c) + at) = make_uint2(pack_half2(f[0], f[1], type), pack_half2(f[2], f[3], type));
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j < left) store_c(c, type, at + j * step, f[j]);
+    }
+}
+
 __device__ __forceinline__ float product_scale(const float* a, const float* b) {
     return (a != nullptr ? *a : 1.0f) * (b != nullptr ? *b : 1.0f);
 }
@@ -446,22 +462,8 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sum[j] *= alpha;
-                if (vec && row + 4 <= p.rows) {
-                    const long long to = static_cast<long long>(col) * p.ldc + row;
-                    if (p.c_type == MCD_TYPE_F32) {
-                        *reinterpret_cast<float4*>(static_cast<float*>(p.c) + to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-                    } else {
-                        *reinterpret_cast<uint2*>(static_cast<unsigned short*>(p.c) + to) =
-                            make_uint2(pack_half2(sum[0], sum[1], p.c_type), pack_half2(sum[2], sum[3], p.c_type));
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (row + j < p.rows) {
-                            store_c(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row + j : static_cast<long long>(row + j) * p.ldc + col, sum[j]);
-                        }
-                    }
-                }
+                store_quad(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row : static_cast<long long>(row) * p.ldc + col,
+                           p.swapped ? 1 : p.ldc, sum, vec, p.rows - row);
             }
         }
         // shared memory stays until the last of the cluster has read it
@@ -480,7 +482,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
 
 // --------------------------------------------------------------------------------------------- an SM pair per tile
 //
-// A cluster of two CTAs owns 256 x 256 of C: each stages its own 128 rows of A, its own 128 of the 256 rows of B, the
+// Two CTAs of a cluster own 256 x 256 of C, or a slice of K of it (see the rule at the host side): each stages its own 128 rows of A, its own 128 of the 256 rows of B, the
 // scales of its rows of A and of all 256 rows of B; the leader's cta_group::2 instructions read both CTAs' shared memory
 // and leave each CTA's 128 rows in its TMEM.
 //
@@ -603,6 +605,8 @@ __device__ __forceinline__ void store_box(unsigned at, void* c, int type, long l
 
 constexpr int kPairThreads = 64 + 8 * 32 + 4 * 32;
 constexpr int kPairTile = 256;
+constexpr int kMaxPairSplits = 4;
+constexpr int kSlicePitch = 1040;  // 256 sums of a row, and 16 bytes that spread rows over the banks
 
 struct Fp4PairParams {
     const float* row_scale;
@@ -612,11 +616,12 @@ struct Fp4PairParams {
     long long ldc;
     int c_type;
     int m, n, k, k_blocks;
+    int splits, k_blocks_per_split;
     int by_tma;  // C leaves as TMA boxes; otherwise (alignment) row by row
 };
 
-template <int kFormat>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+template <int kFormat, bool kSplit>
+__global__ void __launch_bounds__(kPairThreads, 1)
 mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_constant__ McTensorMap map_cols,
                  const __grid_constant__ McTensorMap map_row_scales, const __grid_constant__ McTensorMap map_col_scales,
                  const __grid_constant__ McTensorMap map_c, const Fp4PairParams p) {
@@ -635,10 +640,15 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
     volatile int* abort_flag = &abort_storage;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    unsigned rank;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    unsigned cluster_rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(cluster_rank));
+    const unsigned rank = cluster_rank & 1u, pair_first = kSplit ? cluster_rank & ~1u : 0u;
     const bool leader = rank == 0;
-    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    // Split: a cluster has one tile, its pairs a slice of K each.
+    const int pairs = kSplit ? 2 * p.splits : 2;
+    const int cluster = blockIdx.x / pairs, clusters = gridDim.x / pairs;
+    const int kb_begin = kSplit ? static_cast<int>(cluster_rank >> 1) * p.k_blocks_per_split : 0;
+    const int kb_end = kSplit ? min(p.k_blocks, kb_begin + p.k_blocks_per_split) : p.k_blocks;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tiles_r = (p.m + kPairTile - 1) / kPairTile;
@@ -678,10 +688,10 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                 int rb, cb, split;
                 fp4_decode_item(item, tiles_r, tiles_c, 1, rb, cb, split);
                 const int row_tile = 2 * rb + static_cast<int>(rank);
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
                     ok = mc_mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, MC_FP4_ERR_PRODUCER);
                     if (!ok) break;
-                    const unsigned full = cluster_address(bar_full + 8 * stage, 0);
+                    const unsigned full = cluster_address(bar_full + 8 * stage, pair_first);
                     const unsigned rows_dst = tiles_base + stage * Pair::kStageBytes;
                     const unsigned cols_dst = rows_dst + Pair::kRowBytes;
                     const unsigned row_scales_dst = cols_dst + Pair::kColBytes;
@@ -737,7 +747,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                 empty_phase ^= 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned tmem_d = tmem + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                for (int kb = kb_begin; kb < kb_end; ++kb) {
                     if (!seen) {
                         ok = mc_mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_MMA) &&
                              mc_mbar_wait(bar_ready + 8 * ready, ready_phase, abort_flag, p.status, MC_FP4_ERR_MMA);
@@ -767,12 +777,12 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                         const int t = kFormat == MCD_FP4_E8M0_32 ? ks >> 1 : ks;
                         const unsigned which = kFormat == MCD_FP4_E8M0_32 && (ks & 1) ? kFp4UpperScales : 0u;
                         fp4_mma<kFormat, 2>(tmem_d, desc_r + 2 * ks, desc_c + 2 * ks, idesc | which, scale_r + 4 * t, scale_c + 8 * t,
-                                            (kb > 0 || ks > 0) ? 1u : 0u);
+                                            (kb > kb_begin || ks > 0) ? 1u : 0u);
                     }
-                    fp4_commit_pair(bar_empty + 8 * this_stage);
+                    fp4_commit_pair(bar_empty + 8 * this_stage, pair_first);
                 }
                 if (!ok) break;
-                fp4_commit_pair(bar_acc_full);
+                fp4_commit_pair(bar_acc_full, pair_first);
                 acc ^= 1;
             }
         }
@@ -780,12 +790,12 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         // Scales from shared memory to the 32 TMEM lanes of this warp, the same in every quarter: lane r takes the 16 bytes
         // of rows r, r + 32, r + 64, r + 96 of a tile as four columns.
         const unsigned tmem_lanes = tmem + (static_cast<unsigned>((warp & 3) * 32) << 16) + Pair::kScaleBase;
-        const unsigned bar_leader = cluster_address(bar_ready, 0);
+        const unsigned bar_leader = cluster_address(bar_ready, pair_first);
         int stage = 0, done_stage = 0, ready = 0, number = 0;
         unsigned phase = 0, done_phase = 0;
         bool ok = true;
         for (int item = cluster; ok && item < items; item += clusters) {
-            for (int kb = 0; kb < p.k_blocks; ++kb) {
+            for (int kb = kb_begin; kb < kb_end; ++kb) {
                 ok = mc_mbar_wait(bar_scales + 8 * stage, phase, abort_flag, p.status, MC_FP4_ERR_SCALES);
                 const unsigned src = tiles_base + stage * Pair::kStageBytes + Pair::kTileBytes + static_cast<unsigned>(lane * 16);
                 const unsigned dst = tmem_lanes + static_cast<unsigned>(ready * Pair::kScaleColumns);
@@ -825,7 +835,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         const int half = (warp - 2) >> 2;
         const unsigned buffer = staging + static_cast<unsigned>(warp - 2) * Pair::kStagingPerWarp;
         const float alpha = product_scale(p.row_scale, p.col_scale);
-        const unsigned acc_empty = cluster_address(bar_acc_empty, 0);
+        const unsigned acc_empty = cluster_address(bar_acc_empty, pair_first);
         int acc = 0;
         unsigned full_phase = 0, turn = 0;
         bool ok = true;
@@ -838,6 +848,25 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
             full_phase ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16) + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
+            if constexpr (kSplit) {
+                // The multiplies of this slice are done, and with them the ring: the slice goes there, row by row.
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const int chunk = 4 * half + i;
+                    unsigned w[32];
+                    tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const unsigned to = tiles_base + static_cast<unsigned>((quarter * 32 + lane) * kSlicePitch + chunk * 128);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16 * j), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]),
+                                     "r"(w[4 * j + 3])
+                                     : "memory");
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                break;
+            }
             const int row0 = rb * kPairTile + static_cast<int>(rank) * 128 + quarter * 32;
             // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
             // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
@@ -915,6 +944,50 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (kSplit) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // Every CTA finishes its share of the columns of its 128 rows, four neighbours per thread: slices in their order.
+        int rb, cb, split;
+        fp4_decode_item(cluster, tiles_r, tiles_c, 1, rb, cb, split);
+        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const int share = kPairTile / p.splits, first = static_cast<int>(cluster_rank >> 1) * share;
+        const int per_row = share / 4;
+        const int bytes = p.c_type == MCD_TYPE_F32 ? 4 : 2;
+        const bool vec = ((reinterpret_cast<unsigned long long>(p.c) | static_cast<unsigned long long>(p.ldc * bytes)) & (4 * bytes - 1)) == 0;
+        constexpr int kAtOnce = 2;  // quads per thread and turn
+        for (int base = threadIdx.x; base < 128 * per_row; base += kAtOnce * kPairThreads) {
+            float4 part[kAtOnce][kMaxPairSplits];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int q = min(base + u * kPairThreads, 128 * per_row - 1);
+                const unsigned at = tiles_base + static_cast<unsigned>(q / per_row * kSlicePitch + (first + q % per_row * 4) * 4);
+#pragma unroll
+                for (int z = 0; z < kMaxPairSplits; ++z) {
+                    if (z < p.splits) {
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(part[u][z].x), "=f"(part[u][z].y), "=f"(part[u][z].z), "=f"(part[u][z].w)
+                                     : "r"(cluster_address(at, 2u * static_cast<unsigned>(z) + rank))
+                                     : "memory");
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int q = base + u * kPairThreads;
+                const int row = rb * kPairTile + static_cast<int>(rank) * 128 + q / per_row, col = cb * kPairTile + first + q % per_row * 4;
+                if (q >= 128 * per_row || row >= p.m || col >= p.n) continue;
+                float sum[4] = {part[u][0].x, part[u][0].y, part[u][0].z, part[u][0].w};
+#pragma unroll
+                for (int z = 1; z < kMaxPairSplits; ++z) {
+                    if (z < p.splits) sum[0] += part[u][z].x, sum[1] += part[u][z].y, sum[2] += part[u][z].z, sum[3] += part[u][z].w;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] *= alpha;
+                store_quad(p.c, p.c_type, static_cast<long long>(row) * p.ldc + col, 1, sum, vec, p.n - col);
+            }
+        }
+    }
     // neither CTA gives up its shared memory or TMEM while the other may still use it
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -968,22 +1041,31 @@ struct Plan {
 };
 
 // Up to 128 rows or columns of C: the one-CTA kernel, the shorter side as accumulator columns, so that the longer one fills
-// the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192: 19 us, 36 in
-// tiles of 128 x 128; 1024^3: 12 against 23; 512 x 512 x 4096, four tiles: 13 against 18 with K split).
+// the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192 unsplit: 18 us, 36 in
+// tiles of 128 x 128; 1024^3: 12 against 23).
 //
-// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. Two to eight slices are
-// the CTAs of one cluster, which adds them up from shared memory, as many as find SMs all at once: eight of 14 tiles, four
-// of 32, three of 42 (one token, 8192 x 8192: 11 us, 14 whole; 128 tokens: 14, 18 through a workspace and a second launch;
-// 2048 x 2048: 8 and 10.5). A second wave costs more than the slices give (32 tokens, 8192 columns of K, 16 tiles: 8.7 us in
-// clusters of four, 14 in clusters of eight; 34 tiles: 10.8 in threes, 16 in fours). A long K with few tiles has too few
-// CTAs that way and goes through the workspace (128 rows, one token, K 131072: 21 us, 24 in a cluster; two to four times
-// 128 rows: 16, 25; up to 65536 the cluster takes as long or less).
+// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. The slices of a tile are
+// CTAs, or pairs, of one cluster, which adds them up from shared memory, as many as find SMs all at once: eight CTAs for 14
+// tiles, four for 32, three for 42.
+//   One CTA per slice: one token, 8192 x 8192: 11 us, 14 whole; 128 tokens: 14, 18 through a workspace and a second launch;
+//     2048 x 2048: 8 and 10.5. A second wave costs more than the slices give (32 tokens, 8192 columns of K, 16 tiles:
+//     8.7 us in clusters of four, 14 in clusters of eight; 34 tiles: 10.8 in threes, 16 in fours). A long K with few tiles
+//     has too few CTAs that way and goes through the workspace (128 rows, one token, K 131072: 21 us, 24 in a cluster; two
+//     to four times 128 rows: 16, 25; up to 65536 the cluster takes as long or less).
+//   Pairs: 512 x 512 x 8192, four slices: 12 us, 16 whole; 256 x 8192 x 8192, two: 16 against 18; x 16384: 24 against 32. At
+//     K 4096 joining takes what the slices give.
 Plan plan_for(long long m, long long n, long long k) {
     Plan plan;
     plan.k_blocks = static_cast<int>((k + kFp4BlockK - 1) / kFp4BlockK);
     plan.per_split = plan.k_blocks;
     plan.pairs = m > 128 && n > 128;
-    if (plan.pairs) return plan;
+    if (plan.pairs) {
+        const long long pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+        if (plan.k_blocks >= 24) plan.splits = pair_tiles <= 14 ? 4 : pair_tiles <= 32 ? 2 : 1;
+        plan.per_split = (plan.k_blocks + plan.splits - 1) / plan.splits;
+        plan.clustered = plan.splits > 1;
+        return plan;
+    }
     plan.swapped = m <= n;
     const long long rows = plan.swapped ? n : m;
     const long long cols = plan.swapped ? m : n;
@@ -1110,12 +1192,13 @@ int launch_format(int tile_cols, const McTensorMap& rows, const McTensorMap& col
     }
 }
 
-template <int kFormat>
-int launch_pairs(const mcd_fp4_gemm_args* args, cudaStream_t s) {
+template <int kFormat, bool kSplit>
+int launch_pairs(const mcd_fp4_gemm_args* args, const Plan& plan, cudaStream_t s) {
     using Pair = Fp4Pair<kFormat>;
     static_assert(Pair::kSmem + 64 <= 227 * 1024, "shared memory");
+    static_assert(128 * kSlicePitch <= Pair::kStages * Pair::kStageBytes, "a slice fits into the ring");
     static SharedMemoryOnce once;
-    if (int rc = once.allow(mc_fp4_gemm_pair<kFormat>, Pair::kSmem)) return rc;
+    if (int rc = once.allow(mc_fp4_gemm_pair<kFormat, kSplit>, Pair::kSmem)) return rc;
     McTensorMap rows, cols, row_scales, col_scales, c = {};
     if (int rc = encode_codes(&rows, args->a, 128)) return rc;
     if (int rc = encode_codes(&cols, args->b, 128)) return rc;
@@ -1132,13 +1215,16 @@ int launch_pairs(const mcd_fp4_gemm_args* args, cudaStream_t s) {
     p.n = static_cast<int>(args->b.rows);
     p.k = static_cast<int>(args->a.cols);
     p.k_blocks = (p.k + kFp4BlockK - 1) / kFp4BlockK;
+    p.splits = plan.splits;
+    p.k_blocks_per_split = plan.per_split;
     p.by_tma = is_aligned(args->c, 16) && args->ldc % (args->c_type == MCD_TYPE_F32 ? 4 : 8) == 0;
     if (p.by_tma) {
         if (int rc = encode_c(&c, args->c, args->c_type, p.m, p.n, args->ldc)) return rc;
     }
     const long long tiles = ((args->a.rows + kPairTile - 1) / kPairTile) * ((args->b.rows + kPairTile - 1) / kPairTile);
-    const auto grid = 2 * static_cast<unsigned>(std::min<long long>(tiles, sm_count() / 2));
-    return launch_dependent(mc_fp4_gemm_pair<kFormat>, grid, 1, kPairThreads, Pair::kSmem, s, "mc_fp4_gemm_pair", rows, cols, row_scales, col_scales, c, p);
+    const unsigned cluster = 2 * static_cast<unsigned>(plan.splits);
+    const auto grid = cluster * static_cast<unsigned>(kSplit ? tiles : std::min<long long>(tiles, sm_count() / 2));
+    return launch_dependent(mc_fp4_gemm_pair<kFormat, kSplit>, grid, cluster, kPairThreads, Pair::kSmem, s, "mc_fp4_gemm_pair", rows, cols, row_scales, col_scales, c, p);
 }
 
 size_t plan_workspace(const Plan& plan, long long m, long long n) {
@@ -1194,7 +1280,10 @@ extern "C" int mcd_fp4_gemm(const mcd_fp4_gemm_args* args, void* stream) {
     }
     if (plan.pairs) {
         auto on = static_cast<cudaStream_t>(stream);
-        return args->a.format == MCD_FP4_E8M0_32 ? launch_pairs<MCD_FP4_E8M0_32>(args, on) : launch_pairs<MCD_FP4_E4M3_16>(args, on);
+        if (args->a.format == MCD_FP4_E8M0_32) {
+            return plan.splits > 1 ? launch_pairs<MCD_FP4_E8M0_32, true>(args, plan, on) : launch_pairs<MCD_FP4_E8M0_32, false>(args, plan, on);
+        }
+        return plan.splits > 1 ? launch_pairs<MCD_FP4_E4M3_16, true>(args, plan, on) : launch_pairs<MCD_FP4_E4M3_16, false>(args, plan, on);
     }
     const mcd_fp4_tensor& on_rows = plan.swapped ? args->b : args->a;
     const mcd_fp4_tensor& on_cols = plan.swapped ? args->a : args->b;

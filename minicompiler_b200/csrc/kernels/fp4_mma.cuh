@@ -69,10 +69,10 @@ __device__ __forceinline__ void fp4_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// The same for an SM pair: arrives on the barrier at this offset in both CTAs.
-__device__ __forceinline__ void fp4_commit_pair(unsigned bar) {
+// The same for an SM pair, the CTAs `first` and `first` + 1 of the cluster: arrives on the barrier at this offset in both.
+__device__ __forceinline__ void fp4_commit_pair(unsigned bar, unsigned first) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                 "h"(static_cast<unsigned short>(3))
+                 "h"(static_cast<unsigned short>(3u << first))
                  : "memory");
 }
 

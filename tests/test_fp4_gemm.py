@@ -111,7 +111,8 @@ def _product(mc, a, b, dtype, ldc=None, offset=0, stream=0):
 @pytest.mark.parametrize("m, n, k", [
     (1, 1, 1), (1, 8, 31), (1, 128, 64), (2, 130, 65), (16, 128, 256), (17, 257, 257), (33, 64, 300), (64, 200, 96), (65, 129, 512),
     (128, 128, 128), (128, 300, 1000), (129, 128, 256), (200, 70, 33), (256, 256, 768), (300, 513, 321), (1, 300, 4096), (40, 100, 5000),
-    (513, 256, 1024), (512, 512, 2080), (700, 900, 640), (2100, 1300, 700), (1600, 1600, 2304), (10000, 257, 64), (2305, 2304, 1), (3000, 1, 128), (1000, 16, 3100), (700, 100, 257), (513, 128, 2048), (128, 128, 4096), (3, 200, 66000), (70, 650, 66000), (90, 16, 33000), (100, 4300, 1700), (5000, 120, 1100), (17, 2000, 2100), (5, 9000, 2048), (70, 1030, 4100), (1200, 20, 9000), (20, 1201, 9000),
+    (513, 256, 1024), (512, 512, 2080), (700, 900, 640), (2100, 1300, 700), (1600, 1600, 2304), (10000, 257, 64), (2305, 2304, 1), (3000, 1, 128), (1000, 16, 3100), (700, 100, 257), (513, 128, 2048), (128, 128, 4096), (3, 200, 66000), (70, 650, 66000), (90, 16, 33000), (100, 4300, 1700), (5000, 120, 1100), (17, 2000, 2100), (5, 9000, 2048), (70, 1030, 4100), (1200, 20, 9000), (20, 1201, 9000), (300, 513, 6200), (200, 1000, 7777), (1000, 700, 8200), (1500, 1600, 6500),
+    (257, 8100, 6145),
 ])
 def test_exact_data_gives_equal_results(mc, ref, fmt, m, n, k):
     rng = np.random.default_rng(m * 7 + n * 3 + k)
@@ -162,6 +163,19 @@ def test_only_c_is_written(mc, ref, dtype, m, n, ldc, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+@pytest.mark.parametrize("m, n, ldc, offset", [(20, 300, 301, 1), (20, 300, 304, 8), (300, 20, 21, 1), (300, 500, 501, 1), (300, 500, 504, 8), (300, 501, 504, 16),
+                                               (300, 500, 502, 2), (257, 4100, 4103, 3)])
+def test_slices_of_k_write_c_and_nothing_else(mc, ref, dtype, m, n, ldc, offset):
+    rng = np.random.default_rng(ldc)
+    a, b = _exact_operand(mc, ref, rng, m, 6200, "e8m0_32"), _exact_operand(mc, ref, rng, n, 6200, "e8m0_32")
+    got, around = _product(mc, a, b, dtype, ldc=ldc, offset=offset)
+    assert around
+    want = a.values @ b.values.T
+    assert (np.abs(got - want) <= (0 if dtype == "f32" else STEP[dtype]) * np.abs(want)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("m, n", [(5, 40), (200, 300)])
 def test_a_nan_scale_reaches_its_row_and_no_other(mc, ref, fmt, m, n):
@@ -179,7 +193,7 @@ def test_a_nan_scale_reaches_its_row_and_no_other(mc, ref, fmt, m, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m, n, k", [(3, 256, 8192), (3, 256, 70000), (100, 1300, 2600), (700, 600, 512)])
+@pytest.mark.parametrize("m, n, k", [(3, 256, 8192), (3, 256, 70000), (100, 1300, 2600), (700, 600, 512), (300, 600, 7000)])
 def test_the_same_bits_every_time_and_in_a_replayed_graph(mc, ref, m, n, k):
     import torch
 
