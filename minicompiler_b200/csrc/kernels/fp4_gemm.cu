@@ -4,8 +4,9 @@
 //
 //   sum over k of (a b) = sum over blocks of s_a s_b * (sum over the block of code_a code_b)
 //
-// An instruction covers 64 columns of k; the scales it needs lie in TMEM, brought there from shared memory by
-// tcgen05.cp, which the tensor core executes in order with the multiplies behind it.
+// An instruction covers 64 columns of k; the scales it needs lie in TMEM, brought there from shared memory. One CTA per
+// tile: by tcgen05.cp, which the tensor core executes in order with the multiplies behind it. SM pairs, which multiply
+// without a pause: by warps of their own.
 
 #include "minicompiler_b200_device.h"
 
