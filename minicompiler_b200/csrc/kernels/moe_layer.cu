@@ -8,8 +8,8 @@
 // before it:
 //
 //   mc_moe_router  one cluster of 8 CTAs per token: logits in double-length sums, softmax, the top_k experts; x to f16
-//   mc_moe_up      8-warp CTAs take (expert, 32 or 64 rows of G and the same of U): h = silu(G x) * (U x), f16
-//   mc_moe_level   (where many CTAs read it) h of a token and expert to one power of two
+//   mc_moe_up      8-warp CTAs take (expert, 32 or 64 rows of G and the same of U): h = silu(G x) * (U x), f32
+//   mc_moe_level   (where many CTAs read it) h to the two f16 numbers that the down projection multiplies
 //   mc_moe_down    a cluster of up to 8 CTAs takes 64 or 32 rows of y, its CTAs share the experts and add up what they found
 //
 // Where the time goes: for one token and 8 of 64 experts (26.7 MB of weights, 4 us to read) 25 us are the latencies of
@@ -27,9 +27,10 @@
 // code * scale is exact in f16 (6 bits, 2^-10 .. 2688), so the codes are scaled before the multiply.
 //
 // x and h come to f16 as well, after a power of two that takes the largest magnitude to [2^14, 2^15): one per token for x,
-// and for h one per token, expert and 8 rows (those of one warp's tile, which knows them without asking anybody); the
-// down projection brings them to the power of the largest. 11 bits are kept of values down to 2^-29 of the largest: bf16
-// and f16 inputs lose nothing above that, h is rounded to 11 bits.
+// one per token and expert for h. 11 bits are kept of x's values down to 2^-29 of the largest, so bf16 and f16 inputs lose
+// nothing above that. h has the 24 bits of f32 and enters as two f16 numbers, hi and what it leaves times 2^11, which
+// keep 22 of them: columns 2 s and 2 s + 1 of a multiply are those of slot s. A multiply has 8 columns and an expert rarely
+// more than four tokens, so the second number mostly takes columns that would be empty.
 //
 // How the weights stream: a CTA has 8 warps, four tiles of 16 rows by two halves of k. Every warp keeps a ring of its own
 // in shared memory filled by 16-byte cp.async, three steps of 256 columns ahead of the multiplies and across the ends of
@@ -73,7 +74,7 @@ struct Shape {
     static constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
     static constexpr int kValueBytes = kTokenTile * kValuePitch;
-    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values, per thread and round
+    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values of a column, per thread and round
 };
 
 constexpr int kRouterCluster = 8;
@@ -112,11 +113,10 @@ struct MoeParams {
     // workspace
     int* chosen;              // [tokens * top_k]
     float* weights;           // [tokens * top_k]
-    int* h_max;               // [tokens * top_k]: the largest of h_exponent
+    int* h_max;               // [tokens * top_k]: f32 exponent of the largest |h|
     float* x_shift;           // [tokens]: the power of two that x is multiplied with
     unsigned short* x16;      // [tokens][d_pitch]: x in f16 after that
-    unsigned char* h_exponent;  // [tokens * top_k][f_groups]: f32 exponent of the largest |h| among a tile's rows
-    unsigned short* h;        // [tokens * top_k][f_pitch]: f16 after shift_for of that exponent
+    uint4* h;                 // [tokens * top_k][f_pitch / 8][2]: 8 values in f32; mc_moe_level: 8 hi, then 8 lo in f16
 };
 
 __device__ __forceinline__ float value16(unsigned short v, int type) {
@@ -423,7 +423,7 @@ __device__ __forceinline__ void load_routing(Routing& r, int* scratch, const Moe
     __syncthreads();
 }
 
-// What a CTA works through: rows of an expert against up to 8 of its slots.
+// What a CTA works through: rows of an expert against up to 8 (up) or 4 (down, two columns each) of its slots.
 struct Pass {
     int active;  // which of the active experts
     int group;   // of rows (up only)
@@ -571,15 +571,17 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 // The two projections differ in what a pass is, where values come from and what becomes of the sums; Work supplies these:
 //   begin(pass), next(pass)   the CTA's first pass, the one after: false when there is none
 //   aim(rows, pass, tile)     point the stream at the warp's rows
+//   kParts                    columns of a multiply that a slot takes
 //   load(piece, n, k)         8 values of slot n (of all slots) from column k on, as they lie in memory
-//   finish(piece)             the same in f16
+//   finish(piece, columns)    the same in f16, for each of its columns
 //   look(pass, here)          what a lane will need of its two columns, read before the multiplies
 //   done(pass, here, tile, side, acc)  a warp's sums, both halves of k
 template <int kFormat, int kHalves, int kGroups, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings,
                                            float4* halves) {
     using S = Shape<kHalves, kGroups>;
-    constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kPieces = S::kPieces, kValuePitch = S::kValuePitch;
+    constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kValuePitch = S::kValuePitch;
+    constexpr int kParts = Work::kParts, kPieces = S::kPieces / kParts;
     const int lane = threadIdx.x & 31, group = threadIdx.x / S::kGroupThreads;
     const int thread = threadIdx.x % S::kGroupThreads;
     const int tile = (thread >> 5) % kTiles, half = (thread >> 5) / kTiles;
@@ -628,7 +630,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
     bool value_more = true;
     int value_round = 0;
     typename Work::Piece pieces[kPieces];
-    auto slots_of = [&](const Pass& pass) { return min(kTokenTile, routing.start[pass.active + 1] - routing.start[pass.active] - pass.first); };
+    auto slots_of = [&](const Pass& pass) { return min(Work::kSlots, routing.start[pass.active + 1] - routing.start[pass.active] - pass.first); };
     auto load_values = [&] {
         if (!value_more) return;
         const int here = slots_of(value_pass);
@@ -647,8 +649,12 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         for (int i = 0; i < kPieces; ++i) {
             const int piece = i * S::kGroupThreads + thread;
             const int n = piece / (kRoundK / 8);
-            unsigned char* slot = to + n * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16;
-            if (n < here) *reinterpret_cast<uint4*>(slot) = work.finish(pieces[i]);
+            unsigned char* slot = to + n * kParts * kValuePitch + value_piece<kFormat>(piece % (kRoundK / 8) * 8) * 16;
+            if (n >= here) continue;
+            uint4 columns[kParts];
+            work.finish(pieces[i], columns);
+#pragma unroll
+            for (int c = 0; c < kParts; ++c) *reinterpret_cast<uint4*>(slot + c * kValuePitch) = columns[c];
         }
         if (++value_round == m.rounds) {
             value_round = 0;
@@ -705,6 +711,7 @@ template <int kHalves>
 struct UpWork {
     using S = Shape<kHalves, 1>;
     using Piece = uint4;
+    static constexpr int kParts = 1, kSlots = kTokenTile;
     const MoeParams& p;
     const Routing& routing;
     static constexpr int kGroupsOf128 = 16 / S::kTiles;  // groups of rows of G (and of U) in 128
@@ -722,7 +729,7 @@ struct UpWork {
         return pass.active < routing.num_active;
     }
     __device__ __forceinline__ bool next(Pass& pass) const {
-        pass.first += kTokenTile;
+        pass.first += kSlots;
         if (pass.first < routing.start[pass.active + 1] - routing.start[pass.active]) return true;
         pass.first = 0;
         pass.active += skip_active;
@@ -751,7 +758,7 @@ struct UpWork {
         piece = make_uint4(0, 0, 0, 0);
         if (k < p.d_pitch) piece = *reinterpret_cast<const uint4*>(p.x16 + routing.tokens[n] * static_cast<long long>(p.d_pitch) + k);
     }
-    __device__ __forceinline__ uint4 finish(const Piece& piece) const { return piece; }
+    __device__ __forceinline__ void finish(const Piece& piece, uint4 (&columns)[1]) const { columns[0] = piece; }
     struct Side {
         float back[2];  // undoes x's shift, times the expert's tensor scale
         int slot[2];
@@ -785,12 +792,8 @@ struct UpWork {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
             if (n < here) {
-                const float shifted = h * power(shift_of(e));
-                if (r < p.f_pitch) p.h[static_cast<long long>(slot) * p.f_pitch + r] = static_cast<unsigned short>(pack_f16(shifted, 0.0f) & 0xffffu);
-                if (g == 0) {
-                    p.h_exponent[static_cast<long long>(slot) * p.f_groups + pass.group * S::kTiles + tile] = static_cast<unsigned char>(e);
-                    atomicMax(p.h_max + slot, e);
-                }
+                if (r < p.f_pitch) reinterpret_cast<float*>(p.h)[static_cast<long long>(slot) * p.f_pitch + r] = h;
+                if (g == 0) atomicMax(p.h_max + slot, e);
             }
         }
     }
@@ -828,23 +831,21 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     run_passes<kFormat, kHalves, 1, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves, 1>::kValueBytes, halves);
 }
 
-// Columns k .. k + 7 of h (k a multiple of 8) are two rows each of four of the tiles that h came from: their exponents.
-__device__ __forceinline__ unsigned exponents_at(const MoeParams& p, int slot, int k) {
-    return *reinterpret_cast<const unsigned*>(p.h_exponent + static_cast<long long>(slot) * p.f_groups + (k >> 7) * 16 + ((k >> 3) & 3) * 4);
-}
-
-// Eight values of h brought from their tiles' powers of two to that of the slot's largest.
-__device__ __forceinline__ uint4 levelled(const uint4& raw, unsigned exponents, int largest) {
-    const int to = shift_of(largest);
-    unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+// Eight values of h after the power of two of their slot's largest: hi, the nearest f16, and lo, 2^11 times what hi leaves, at
+// most 2^14. An infinite hi (beside a value that is infinite or NaN nothing is shifted) leaves nothing.
+__device__ __forceinline__ void split(const uint4& first, const uint4& second, int largest, uint4 (&columns)[2]) {
+    const unsigned w[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
+    const float to = power(shift_of(largest));
+    unsigned hi[4], lo[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        // 2^(to - from) as f16, at most 1 (what came from a smaller largest is multiplied up less); below 2^-24 it is 0
-        const int down = shift_of(static_cast<int>((exponents >> (8 * j)) & 0xffu)) - to;
-        const unsigned factor = down <= 0 ? 0x3c00u : down <= 14 ? static_cast<unsigned>(15 - down) << 10 : down <= 24 ? 1u << (24 - down) : 0u;
-        w[j] = mul_f16x2(w[j], factor | factor << 16);
+        const float a = __uint_as_float(w[2 * j]) * to, b = __uint_as_float(w[2 * j + 1]) * to;
+        hi[j] = pack_f16(a, b);
+        const float ha = f16_lo(hi[j]), hb = f16_hi(hi[j]);
+        lo[j] = pack_f16(fabsf(ha) <= 65504.0f ? (a - ha) * 2048.0f : 0.0f, fabsf(hb) <= 65504.0f ? (b - hb) * 2048.0f : 0.0f);
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    columns[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    columns[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 // All of h, in place.
@@ -852,21 +853,24 @@ __global__ void __launch_bounds__(128) mc_moe_level(const MoeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int slot = blockIdx.x;
-    const int largest = p.h_max[slot];
-    for (int k = threadIdx.x * 8; k < p.f_pitch; k += 128 * 8) {
-        auto* at = reinterpret_cast<uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
-        *at = levelled(*at, exponents_at(p, slot, k), largest);
+    const int largest = p.h_max[slot], eights = p.f_pitch / 8;
+    for (int i = threadIdx.x; i < eights; i += 128) {
+        uint4* at = p.h + 2 * (static_cast<long long>(slot) * eights + i);
+        uint4 columns[2];
+        split(at[0], at[1], largest, columns);
+        at[0] = columns[0];
+        at[1] = columns[1];
     }
 }
 
-// One group: h lies as mc_moe_up left it, one power of two per tile of 8 rows; several: as mc_moe_level did, one per slot.
+// One group: h lies as mc_moe_up left it, in f32; several: as mc_moe_level did, as the two f16 numbers.
 template <int kGroups>
 struct DownWork {
     using S = DownShape<kGroups>;
     static constexpr bool kLevel = kGroups > 1;
+    static constexpr int kParts = 2, kSlots = kTokenTile / 2;
     struct Piece {
-        uint4 raw;
-        unsigned exponents;
+        uint4 raw[2];
         int largest;
     };
     const MoeParams& p;
@@ -882,7 +886,7 @@ struct DownWork {
         return pass.active < routing.num_active;
     }
     __device__ __forceinline__ bool next(Pass& pass) const {
-        pass.first += kTokenTile;
+        pass.first += kSlots;
         if (pass.first < routing.start[pass.active + 1] - routing.start[pass.active]) return true;
         pass.first = 0;
         pass.active += step;
@@ -904,45 +908,46 @@ struct DownWork {
     }
     __device__ __forceinline__ void load(Piece& piece, int n, int k) const {
         const int slot = routing.slots[n];
-        piece.raw = make_uint4(0, 0, 0, 0);
-        piece.exponents = 0;
+        piece.raw[0] = piece.raw[1] = make_uint4(0, 0, 0, 0);
         if (!kLevel) piece.largest = p.h_max[slot];
         if (k < p.f_pitch) {
-            piece.raw = *reinterpret_cast<const uint4*>(p.h + static_cast<long long>(slot) * p.f_pitch + k);
-            if (!kLevel) piece.exponents = exponents_at(p, slot, k);
+            const uint4* at = p.h + 2 * (static_cast<long long>(slot) * (p.f_pitch / 8) + k / 8);
+            piece.raw[0] = at[0];
+            piece.raw[1] = at[1];
         }
     }
-    __device__ __forceinline__ uint4 finish(const Piece& piece) const { return kLevel ? piece.raw : levelled(piece.raw, piece.exponents, piece.largest); }
-    struct Side {
-        float back[2];    // undoes h's shift, times the expert's tensor scale
-        float weight[2];
-        int token[2];
-    };
-    __device__ __forceinline__ Side look(const Pass& pass, int here) const {
-        Side side;
-        const int first_slot = routing.start[pass.active] + pass.first;
-        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.active]] : 1.0f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int at = first_slot + min(static_cast<int>(threadIdx.x & 3) * 2 + j, here - 1);
-            const int slot = routing.slots[at];
-            side.back[j] = power(-shift_of(p.h_max[slot])) * scale;
-            side.weight[j] = p.weights[slot];
-            side.token[j] = routing.tokens[at];
+    __device__ __forceinline__ void finish(const Piece& piece, uint4 (&columns)[2]) const {
+        if (kLevel) {
+            columns[0] = piece.raw[0];
+            columns[1] = piece.raw[1];
+        } else {
+            split(piece.raw[0], piece.raw[1], piece.largest, columns);
         }
+    }
+    struct Side {
+        float back;    // undoes h's shift, times the expert's tensor scale
+        float weight;
+        int token;
+    };
+    // A lane's two columns are the two of one slot.
+    __device__ __forceinline__ Side look(const Pass& pass, int here) const {
+        const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.active]] : 1.0f;
+        const int at = routing.start[pass.active] + pass.first + min(static_cast<int>(threadIdx.x & 3), here - 1);
+        const int slot = routing.slots[at];
+        Side side;
+        side.back = power(-shift_of(p.h_max[slot])) * scale;
+        side.weight = p.weights[slot];
+        side.token = routing.tokens[at];
         return side;
     }
     __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[4]) const {
         const int lane = threadIdx.x & 31;
         const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (2 * t + j < here) {
-                // this warp's 16 columns; nobody else adds to them
-                float* sum = sums + side.token[j] * S::kPitch + tile * 16;
-                sum[g] += side.weight[j] * (acc[j] * side.back[j]);
-                sum[g + 8] += side.weight[j] * (acc[2 + j] * side.back[j]);
-            }
+        if (t < here) {
+            // this warp's 16 columns; nobody else adds to them
+            float* sum = sums + side.token * S::kPitch + tile * 16;
+            sum[g] += side.weight * (fmaf(acc[1], 0x1p-11f, acc[0]) * side.back);
+            sum[g + 8] += side.weight * (fmaf(acc[3], 0x1p-11f, acc[2]) * side.back);
         }
     }
 };
@@ -1090,7 +1095,7 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
 extern "C" size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f) {
     if (tokens < 1 || tokens > MCD_MOE_MAX_TOKENS || experts < 1 || top_k < 1 || top_k > MCD_MOE_MAX_TOP_K || d < 1 || f < 1) return 0;
     const size_t slots = static_cast<size_t>(tokens) * static_cast<size_t>(top_k);
-    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + rounded(slots * f_groups(f)) + rounded(slots * in_eights(f) * 2) +
+    return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + slots * in_eights(f) * 4 +
            rounded(static_cast<size_t>(tokens) * in_eights(d) * 2);
 }
 
@@ -1158,9 +1163,8 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     p.weights = reinterpret_cast<float*>(at += rounded(slots * 4));
     p.h_max = reinterpret_cast<int*>(at += rounded(slots * 4));
     p.x_shift = reinterpret_cast<float*>(at += rounded(slots * 4));
-    p.h_exponent = at += rounded(static_cast<size_t>(args->tokens) * 4);
-    p.h = reinterpret_cast<unsigned short*>(at += rounded(slots * f_groups(f)));
-    p.x16 = reinterpret_cast<unsigned short*>(at += rounded(slots * in_eights(f) * 2));
+    p.h = reinterpret_cast<uint4*>(at += rounded(static_cast<size_t>(args->tokens) * 4));
+    p.x16 = reinterpret_cast<unsigned short*>(at += slots * in_eights(f) * 4);
     auto s = static_cast<cudaStream_t>(stream);
     return gu.format == MCD_FP4_E8M0_32 ? launch_layer<MCD_FP4_E8M0_32>(p, s) : launch_layer<MCD_FP4_E4M3_16>(p, s);
 }

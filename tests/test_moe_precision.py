@@ -1,0 +1,95 @@
+"""How exact the mixture-of-experts layer is, where the coarse bounds of test_moe_layer.py would not show it.
+
+h = silu(G x) * (U x) enters the down projection as two f16 numbers: hi, its nearest, and what hi leaves, rounded in turn:
+22 bits, 2^-22 of a value, and not less than 2^-36 after the shift that takes the largest of a token and expert to
+[2^14, 2^15), 2^-50 of that one. The rest is f32: sums of n terms off by n 2^-23 of their terms' magnitudes, silu by 8 steps."""
+
+import numpy as np
+import pytest
+
+from test_moe_layer import FORMATS, STEP, U, Problem, ref  # noqa: F401  (ref: the fixture)
+
+
+class Tight(Problem):
+    """The same layer held to a bound in which h has 22 bits."""
+
+    def _expected(self):
+        x, d, f = self.x64, self.d, self.f
+        logits = x @ self.router64.T
+        chosen = np.stack([np.lexsort((np.arange(self.experts), -l))[: self.top_k] for l in logits])
+        p = np.exp(logits - logits.max(axis=1, keepdims=True))
+        weights = np.take_along_axis(p / p.sum(axis=1, keepdims=True), chosen, axis=1)
+        if self.renormalize:
+            weights = weights / weights.sum(axis=1, keepdims=True)
+        y, bound = np.zeros((self.tokens, d)), np.zeros((self.tokens, d))
+        for t in range(self.tokens):
+            size = np.zeros(d)
+            for j in range(self.top_k):
+                gu, dn = self.values[0][chosen[t, j]], self.values[1][chosen[t, j]]
+                z, z_err = gu @ x[t], (d + 4) * U * (np.abs(gu) @ np.abs(x[t]))
+                gate, up = z[:f], z[f:]
+                small = np.exp(-np.abs(gate))
+                sig = np.where(gate >= 0, 1, small) / (1 + small)
+                h = gate * sig * up
+                h_err = 1.1 * z_err[:f] * (np.abs(up) + z_err[f:]) + np.abs(gate * sig) * z_err[f:] + 8 * U * np.abs(h)
+                h_err += 2.0 ** -22 * (np.abs(h) + h_err) + 2.0 ** -50 * (np.abs(h) + h_err).max()
+                o, o_size = dn @ h, np.abs(dn) @ (np.abs(h) + h_err)
+                o_err = np.abs(dn) @ h_err + (2 * f + 4) * U * o_size  # twice the terms: hi and what it leaves
+                y[t] += weights[t, j] * o
+                bound[t] += weights[t, j] * (o_err + 32 * U * np.abs(o))
+                size += weights[t, j] * (np.abs(o) + o_err)
+            bound[t] += (self.top_k + 8) * U * size
+        return y, bound + STEP[self.dtype] * (np.abs(y) + bound) + 2.0 ** -25, chosen, weights
+
+
+def _differences(f, d, fmt, seed):
+    """A `spoil` that makes a down projection's row the difference of two of h's values: codes 1 and -1 under scales of 1.
+
+    The values are of like size, so what is left of them shows how many bits they had."""
+    rng = np.random.default_rng(seed)
+    pairs = np.stack([rng.permutation(f)[:2] for _ in range(d)])
+
+    def spoil(matrix, expert, code, scale):
+        if matrix == 1:
+            code[:] = 0
+            code[np.arange(d), pairs[:, 0]] = 2
+            code[np.arange(d), pairs[:, 1]] = 10
+            scale[:] = 127 if fmt == "e8m0_32" else 0x38
+        else:
+            # rows of U repeat those of G, and all rows are nearly one another's: h's values lie close together
+            code[f:] = code[:f]
+            scale[f:] = scale[:f]
+            code[:] = code[0]
+            scale[:] = scale[0]
+            flip = rng.integers(0, code.shape[1], size=2 * f)
+            code[np.arange(2 * f), flip] = (code[np.arange(2 * f), flip] + 1) % 8
+
+    return spoil
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("tokens, experts, top_k, d, f", [(1, 1, 1, 64, 40), (1, 6, 2, 48, 300), (5, 7, 3, 96, 33), (9, 2, 1, 64, 48), (20, 4, 2, 1100, 72),
+                                                          (40, 30, 5, 64, 140), (64, 3, 3, 80, 64)])
+def test_h_has_more_bits_than_f16(mc, ref, fmt, dtype, tokens, experts, top_k, d, f):  # noqa: F811
+    p = Tight(mc, ref, fmt=fmt, dtype=dtype, tokens=tokens, experts=experts, top_k=top_k, d=d, f=f, seed=d, spoil=_differences(f, d, fmt, 5))
+    got = p.run()
+    y, bound, chosen, _ = p.expected()
+    assert np.array_equal(p.chosen.cpu().numpy(), chosen)
+    assert (np.abs(got - y) <= bound).all(), float((np.abs(got - y) / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens, experts, top_k, d, f", [(1, 4, 2, 640, 96), (7, 13, 3, 300, 721), (64, 4, 4, 64, 64), (33, 6, 3, 96, 40), (40, 100, 6, 200, 260),
+                                                          (20, 12, 5, 300, 200), (9, 40, 6, 1100, 260), (64, 90, 12, 97, 770)])
+def test_the_layer_is_as_exact_as_its_result_type(mc, ref, fmt, tokens, experts, top_k, d, f):  # noqa: F811
+    """In the norm the error is that of rounding y alone. An error spread evenly over half a step 2^-11 of a binade has the mean
+    square 2^-22 / 3; over mantissas m of density 1 / m the mean of m^2 is 1.5 / ln 2. A third on top for the sample's spread."""
+    p = Tight(mc, ref, fmt=fmt, dtype="f16", tokens=tokens, experts=experts, top_k=top_k, d=d, f=f, seed=f)
+    got = p.run()
+    y, bound, chosen, _ = p.expected()
+    assert np.array_equal(p.chosen.cpu().numpy(), chosen)
+    assert (np.abs(got - y) <= bound).all()
+    assert np.linalg.norm(got - y) <= 1.3 * STEP["f16"] * (np.log(2) / 4.5) ** 0.5 * np.linalg.norm(y)
