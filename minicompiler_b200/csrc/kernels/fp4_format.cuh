@@ -91,6 +91,18 @@ __device__ __forceinline__ float e8m0_decode(unsigned byte) {
     return __uint_as_float(bits);
 }
 
+// A value times a * b, where a * b need not be a number that f32 holds well although the result is: one factor where it is,
+// otherwise a and b one behind the other. They then lie on the same side of 1, so that the way there leaves f32 only where
+// the result does.
+struct TwoFactors {
+    float first, second;
+    __device__ __forceinline__ float times(float v) const { return v * first * second; }
+};
+__device__ __forceinline__ TwoFactors two_factors(float a, float b) {
+    const float both = a * b;
+    return fabsf(both) >= 1.17549435e-38f && fabsf(both) <= 3.402823466e38f ? TwoFactors{both, 1.0f} : TwoFactors{a, b};
+}
+
 #endif
 
 }  // namespace mcd

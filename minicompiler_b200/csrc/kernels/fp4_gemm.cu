@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 using namespace mcd;
 
@@ -110,8 +111,8 @@ __device__ __forceinline__ void store_quad(void* c, int type, long long at, long
     }
 }
 
-__device__ __forceinline__ float product_scale(const float* a, const float* b) {
-    return (a != nullptr ? *a : 1.0f) * (b != nullptr ? *b : 1.0f);
+__device__ __forceinline__ TwoFactors product_scale(const float* a, const float* b) {
+    return two_factors(a != nullptr ? *a : 1.0f, b != nullptr ? *b : 1.0f);
 }
 
 // ------------------------------------------------------------------------------------------------ one CTA per tile
@@ -335,7 +336,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
         const int quarter = warp & 3;
         constexpr int kChunk = 16;
         float* turn = reinterpret_cast<float*>(smem_raw + (tiles_base - mc_smem_addr(smem_raw)) + stages * Tile::kStageBytes + Tile::kBarrierBytes) + quarter * 32 * 17;
-        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const TwoFactors alpha = product_scale(p.row_scale, p.col_scale);
         int acc = 0;
         unsigned acc_phase = 0;
         bool ok = true;
@@ -369,7 +370,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
             void* dst = partial ? static_cast<void*>(p.workspace + split * m * n) : p.c;
             const long long ld = partial ? n : p.ldc;
             const int type = partial ? MCD_TYPE_F32 : p.c_type;
-            const float scale = partial ? 1.0f : alpha;
+            const TwoFactors scale = partial ? TwoFactors{1.0f, 1.0f} : alpha;
             // rows of C that start on 16-byte boundaries leave in pieces of that size
             const bool vec = !p.swapped && (reinterpret_cast<unsigned long long>(dst) & 15) == 0 && (ld & (type == MCD_TYPE_F32 ? 3 : 7)) == 0;
             for (int chunk = 0; chunk < kCols / kChunk; ++chunk) {
@@ -381,13 +382,13 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                 if (row < p.rows && vec && col0 + kChunk <= p.cols) {
                     float f[kChunk];
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) f[j] = __uint_as_float(v[j]) * scale;
+                    for (int j = 0; j < kChunk; ++j) f[j] = scale.times(__uint_as_float(v[j]));
                     store_row16(dst, type, static_cast<long long>(row) * ld + col0, f);
                 } else if (p.swapped) {
                     if (row < p.rows) {
 #pragma unroll
                         for (int j = 0; j < kChunk; ++j) {
-                            if (col0 + j < p.cols) store_c(dst, type, static_cast<long long>(col0 + j) * ld + row, __uint_as_float(v[j]) * scale);
+                            if (col0 + j < p.cols) store_c(dst, type, static_cast<long long>(col0 + j) * ld + row, scale.times(__uint_as_float(v[j])));
                         }
                     }
                 }
@@ -396,7 +397,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                     // (65536 x 100 of them, one thread a row: 77 us, this way 37).
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) turn[lane * 17 + j] = __uint_as_float(v[j]) * scale;
+                    for (int j = 0; j < kChunk; ++j) turn[lane * 17 + j] = scale.times(__uint_as_float(v[j]));
                     __syncwarp();
                     const int c = col0 + (lane & 15);
                     const int first = row - lane + (lane >> 4);
@@ -428,7 +429,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
         // Every CTA finishes its share of the columns, four rows of a column per thread: slices in their order.
         int rb, cb, rank;
         fp4_decode_item(blockIdx.x, tiles_r, tiles_c, p.splits, rb, cb, rank);
-        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const TwoFactors alpha = product_scale(p.row_scale, p.col_scale);
         const int valid = min(kCols, p.cols - cb * kCols);
         const int share = (valid + p.splits - 1) / p.splits;
         const int first = rank * share;
@@ -462,7 +463,7 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                     if (z < p.splits) sum[0] += part[u][z].x, sum[1] += part[u][z].y, sum[2] += part[u][z].z, sum[3] += part[u][z].w;
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[j] *= alpha;
+                for (int j = 0; j < 4; ++j) sum[j] = alpha.times(sum[j]);
                 store_quad(p.c, p.c_type, p.swapped ? static_cast<long long>(col) * p.ldc + row : static_cast<long long>(row) * p.ldc + col,
                            p.swapped ? 1 : p.ldc, sum, vec, p.rows - row);
             }
@@ -521,13 +522,14 @@ struct Fp4Pair {
 };
 
 // A lane's 32 values, the row `lane` of a box of 32 x 32, to shared memory as a TMA store wants them: rows of 128 bytes (f32,
-// 128-byte swizzle) or of 64 (16 bits, 64-byte swizzle).
-__device__ __forceinline__ void stage_row(unsigned at, const unsigned (&v)[32], float alpha, int type) {
+// 128-byte swizzle) or of 64 (16 bits, 64-byte swizzle). kBoth: times both factors of alpha, otherwise the second is 1.
+template <bool kBoth>
+__device__ __forceinline__ void stage_row(unsigned at, const unsigned (&v)[32], const TwoFactors& alpha, int type) {
     unsigned lane = threadIdx.x & 31;
     asm volatile("" : "+r"(lane));  // addresses made here and not kept: nothing of this is worth registers between tiles
     float f[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
+    for (int j = 0; j < 32; ++j) f[j] = kBoth ? alpha.times(__uint_as_float(v[j])) : __uint_as_float(v[j]) * alpha.first;
     if (type == MCD_TYPE_F32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -835,109 +837,119 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         const int quarter = warp & 3;
         const int half = (warp - 2) >> 2;
         const unsigned buffer = staging + static_cast<unsigned>(warp - 2) * Pair::kStagingPerWarp;
-        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const TwoFactors alpha = product_scale(p.row_scale, p.col_scale);
         const unsigned acc_empty = cluster_address(bar_acc_empty, pair_first);
-        int acc = 0;
-        unsigned full_phase = 0, turn = 0;
-        bool ok = true;
-        for (int item = cluster; ok && item < items; item += clusters) {
-            int rb, cb, split;
-            fp4_decode_item(item, tiles_r, tiles_c, 1, rb, cb, split);
-            ok = mc_mbar_wait(bar_acc_full, full_phase, abort_flag, p.status, MC_FP4_ERR_EPILOGUE);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            full_phase ^= 1u;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16) + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
-            if constexpr (kSplit) {
-                // The multiplies of this slice are done, and with them the ring: the slice goes there, row by row.
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    const int chunk = 4 * half + i;
-                    unsigned w[32];
-                    tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const unsigned to = tiles_base + static_cast<unsigned>((quarter * 32 + lane) * kSlicePitch + chunk * 128);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16 * j), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]),
-                                     "r"(w[4 * j + 3])
-                                     : "memory");
+        // Written once for each number of factors: 32 multiplications more per row of a chunk are felt where K is short (65536 x
+        // 2048 x 256: 61 us instead of 56), and so is a branch around them (59).
+        auto epilogue = [&](auto two) {
+            constexpr bool kBoth = decltype(two)::value;
+            int acc = 0;
+            unsigned full_phase = 0, turn = 0;
+            bool ok = true;
+            for (int item = cluster; ok && item < items; item += clusters) {
+                int rb, cb, split;
+                fp4_decode_item(item, tiles_r, tiles_c, 1, rb, cb, split);
+                ok = mc_mbar_wait(bar_acc_full, full_phase, abort_flag, p.status, MC_FP4_ERR_EPILOGUE);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                full_phase ^= 1u;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned lanes = tmem + (static_cast<unsigned>(quarter * 32) << 16) + (acc ? static_cast<unsigned>(256 - Pair::kOverlap) : 0u);
+                if constexpr (kSplit) {
+                    // The multiplies of this slice are done, and with them the ring: the slice goes there, row by row.
+    #pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const int chunk = 4 * half + i;
+                        unsigned w[32];
+                        tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        const unsigned to = tiles_base + static_cast<unsigned>((quarter * 32 + lane) * kSlicePitch + chunk * 128);
+    #pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16 * j), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]),
+                                         "r"(w[4 * j + 3])
+                                         : "memory");
+                        }
                     }
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                break;
-            }
-            const int row0 = rb * kPairTile + static_cast<int>(rank) * 128 + quarter * 32;
-            // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
-            // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
-            auto chunk_at = [&](int i) { return acc ? i : 7 - i; };
-            // Boxes that reach over the last column are not left to TMA, which cuts rows off at 16 bytes: what lies behind C's
-            // columns inside ldc is not ours.
-            if (!p.by_tma || (p.n % 32 != 0 && (cb + 1) * kPairTile > p.n)) {
-                if (lane == 0) tma_store_wait_read<0>();
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    const int chunk = chunk_at(2 * i + half), col0 = cb * kPairTile + chunk * 32;
-                    unsigned w[32];
-                    tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    break;
+                }
+                const int row0 = rb * kPairTile + static_cast<int>(rank) * 128 + quarter * 32;
+                // Chunks of 32 columns in the order in which they are wanted back: the shared ones lie at the end of the first
+                // accumulator and at the beginning of the second. The two warps of a lane quarter take turns.
+                auto chunk_at = [&](int i) { return acc ? i : 7 - i; };
+                // Boxes that reach over the last column are not left to TMA, which cuts rows off at 16 bytes: what lies behind C's
+                // columns inside ldc is not ours.
+                if (!p.by_tma || (p.n % 32 != 0 && (cb + 1) * kPairTile > p.n)) {
+                    if (lane == 0) tma_store_wait_read<0>();
+    #pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const int chunk = chunk_at(2 * i + half), col0 = cb * kPairTile + chunk * 32;
+                        unsigned w[32];
+                        tmem_load32(lanes + static_cast<unsigned>(chunk * 32), w);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (i == 3 && lane == 0) mbar_arrive_cluster(acc_empty);
+                        if (col0 >= p.n || row0 >= p.m) continue;  // warp-uniform
+                        stage_row<kBoth>(buffer, w, alpha, p.c_type);
+                        __syncwarp();
+                        store_box(buffer, p.c, p.c_type, static_cast<long long>(row0) * p.ldc + col0, p.ldc, p.m - row0, p.n - col0);
+                        __syncwarp();
+                    }
+                    acc ^= 1;
+                    continue;
+                }
+                auto finish = [&](const unsigned (&v)[32], int chunk) {
+                    const int col0 = cb * kPairTile + chunk * 32;
+                    if (col0 >= p.n) return;  // warp-uniform
+                    // boxes of 16 bits take turns in the halves of this warp's buffer
+                    unsigned at = buffer;
+                    if (p.c_type == MCD_TYPE_F32) {
+                        if (lane == 0) tma_store_wait_read<0>();
+                    } else {
+                        at += (turn & 1u) * 2048u;
+                        ++turn;
+                        if (lane == 0) tma_store_wait_read<1>();
+                    }
                     __syncwarp();
-                    if (i == 3 && lane == 0) mbar_arrive_cluster(acc_empty);
-                    if (col0 >= p.n || row0 >= p.m) continue;  // warp-uniform
-                    stage_row(buffer, w, alpha, p.c_type);
+                    stage_row<kBoth>(at, v, alpha, p.c_type);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    store_box(buffer, p.c, p.c_type, static_cast<long long>(row0) * p.ldc + col0, p.ldc, p.m - row0, p.n - col0);
-                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
+                };
+                // The shared chunks are read before anything else; where a warp has three of them, the first leaves meanwhile (three
+                // in registers spill).
+                constexpr int kFirst = (Pair::kOverlapChunks + 1) / 2;  // shared chunks of the warps with half == 0
+                unsigned v[2][32];
+    #pragma unroll
+                for (int i = 0; i < kFirst; ++i) {
+                    if (i == 2) {
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        finish(v[0], chunk_at(half));
+                    }
+                    if (2 * i + half < Pair::kOverlapChunks) tmem_load32(lanes + static_cast<unsigned>(chunk_at(2 * i + half) * 32), v[i & 1]);
+                }
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc_empty);
+    #pragma unroll
+                for (int i = kFirst == 3 ? 1 : 0; i < 4; ++i) {
+                    const int order = 2 * i + half;
+                    if (order >= Pair::kOverlapChunks) {
+                        tmem_load32(lanes + static_cast<unsigned>(chunk_at(order) * 32), v[i & 1]);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    }
+                    finish(v[i & 1], chunk_at(order));
                 }
                 acc ^= 1;
-                continue;
             }
-            auto finish = [&](const unsigned (&v)[32], int chunk) {
-                const int col0 = cb * kPairTile + chunk * 32;
-                if (col0 >= p.n) return;  // warp-uniform
-                // boxes of 16 bits take turns in the halves of this warp's buffer
-                unsigned at = buffer;
-                if (p.c_type == MCD_TYPE_F32) {
-                    if (lane == 0) tma_store_wait_read<0>();
-                } else {
-                    at += (turn & 1u) * 2048u;
-                    ++turn;
-                    if (lane == 0) tma_store_wait_read<1>();
-                }
-                __syncwarp();
-                stage_row(at, v, alpha, p.c_type);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) tma_store_2d(&map_c, at, col0, row0);
-            };
-            // The shared chunks are read before anything else; where a warp has three of them, the first leaves meanwhile (three
-            // in registers spill).
-            constexpr int kFirst = (Pair::kOverlapChunks + 1) / 2;  // shared chunks of the warps with half == 0
-            unsigned v[2][32];
-#pragma unroll
-            for (int i = 0; i < kFirst; ++i) {
-                if (i == 2) {
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    finish(v[0], chunk_at(half));
-                }
-                if (2 * i + half < Pair::kOverlapChunks) tmem_load32(lanes + static_cast<unsigned>(chunk_at(2 * i + half) * 32), v[i & 1]);
-            }
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty);
-#pragma unroll
-            for (int i = kFirst == 3 ? 1 : 0; i < 4; ++i) {
-                const int order = 2 * i + half;
-                if (order >= Pair::kOverlapChunks) {
-                    tmem_load32(lanes + static_cast<unsigned>(chunk_at(order) * 32), v[i & 1]);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                }
-                finish(v[i & 1], chunk_at(order));
-            }
-            acc ^= 1;
+        };
+        if (alpha.second == 1.0f) {
+            epilogue(std::false_type{});
+        } else {
+            epilogue(std::true_type{});
         }
         if (lane == 0) tma_store_wait_read<0>();
     }
@@ -951,7 +963,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
         // Every CTA finishes its share of the columns of its 128 rows, four neighbours per thread: slices in their order.
         int rb, cb, split;
         fp4_decode_item(cluster, tiles_r, tiles_c, 1, rb, cb, split);
-        const float alpha = product_scale(p.row_scale, p.col_scale);
+        const TwoFactors alpha = product_scale(p.row_scale, p.col_scale);
         const int share = kPairTile / p.splits, first = static_cast<int>(cluster_rank >> 1) * share;
         const int per_row = share / 4;
         const int bytes = p.c_type == MCD_TYPE_F32 ? 4 : 2;
@@ -984,7 +996,7 @@ mc_fp4_gemm_pair(const __grid_constant__ McTensorMap map_rows, const __grid_cons
                     if (z < p.splits) sum[0] += part[u][z].x, sum[1] += part[u][z].y, sum[2] += part[u][z].z, sum[3] += part[u][z].w;
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[j] *= alpha;
+                for (int j = 0; j < 4; ++j) sum[j] = alpha.times(sum[j]);
                 store_quad(p.c, p.c_type, static_cast<long long>(row) * p.ldc + col, 1, sum, vec, p.n - col);
             }
         }
@@ -1003,7 +1015,7 @@ template <int kVec>
 __global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ parts, int splits, long long m, long long n, const float* scale_a,
                                                    const float* scale_b, void* c, int c_type, long long ldc) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float alpha = product_scale(scale_a, scale_b);
+    const TwoFactors alpha = product_scale(scale_a, scale_b);
     const long long count = m * n;
     const unsigned per_row = static_cast<unsigned>(n / kVec);
     const long long r = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
@@ -1025,7 +1037,7 @@ __global__ void __launch_bounds__(256) mc_fp4_join(const float* __restrict__ par
         }
         const long long at = r * ldc + static_cast<long long>(i) * kVec;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) store_c(c, c_type, at + j, sum[j] * alpha);
+        for (int j = 0; j < kVec; ++j) store_c(c, c_type, at + j, alpha.times(sum[j]));
     }
 }
 

@@ -303,3 +303,44 @@ def test_host_memory_is_refused(mc):
     with pytest.raises(mc.McError, match="not device memory"):
         mc.Fp4Gemm(a, b, dev.data_ptr() + 32768, "f32").enqueue()
     torch.cuda.synchronize()
+
+
+def _far_operand(mc, ref, rng, rows, k, byte, g, zero=None):
+    """Codes under one block scale and a tensor scale g; row `zero` has codes 0."""
+    code = rng.integers(0, 16, size=(rows, k)).astype(np.uint8)
+    if zero is not None:
+        code[zero] = 0
+    return Operand(mc, ref, code, np.full((rows, -(-k // 16)), byte, dtype=np.uint8), "e4m3_16", g)
+
+
+# one CTA per tile whole, in a cluster, through the workspace; SM pairs whole and in slices
+FORMS = [(5, 40, 200), (3, 256, 8192), (3, 256, 66000), (300, 513, 321), (300, 501, 6400)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", FORMS)
+@pytest.mark.parametrize("ga, gb, byte", [(2.0 ** -75, 2.0 ** -75, 0x78), (2.0 ** -120, 2.0 ** -20, 0x78), (2.0 ** 64, 2.0 ** 64, 0x01), (2.0 ** 100, 2.0 ** 35, 0x01),
+                                          (2.0 ** -100, 2.0 ** 100, 0x38), (2.0 ** 100, 2.0 ** -100, 0x38), (2.0 ** -130, 2.0 ** 5, 0x78)])
+def test_tensor_scales_whose_product_leaves_f32(mc, ref, m, n, k, ga, gb, byte):
+    """Powers of two, and sums that f32 holds exactly: so does C, although g_a g_b need not. 0x78 is 2^8, 0x01 2^-9."""
+    rng = np.random.default_rng(k)
+    a, b = _far_operand(mc, ref, rng, m, k, byte, ga, zero=1), _far_operand(mc, ref, rng, n, k, byte, gb)
+    want = a.values @ b.values.T
+    want = np.where(np.abs(want) < 2.0 ** 128, want, np.copysign(np.inf, want))
+    assert np.isfinite(want).any() and np.count_nonzero(want) > want.size / 2
+    got, around = _product(mc, a, b, "f32")
+    assert around
+    assert np.array_equal(got, want)
+    assert (got[1] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", FORMS)
+@pytest.mark.parametrize("ga, gb, byte", [(1.37 * 2.0 ** -70, 1.71 * 2.0 ** -70, 0x78), (1.9 * 2.0 ** -118, 1.3 * 2.0 ** -20, 0x78)])
+def test_tensor_scales_whose_product_is_subnormal(mc, ref, m, n, k, ga, gb, byte):
+    """The sums are exact; each scale is a rounding of 2^-24, and where C is subnormal one of half of f32's smallest number."""
+    rng = np.random.default_rng(k + 1)
+    a, b = _far_operand(mc, ref, rng, m, k, byte, ga), _far_operand(mc, ref, rng, n, k, byte, gb)
+    want = a.values @ b.values.T
+    got, _ = _product(mc, a, b, "f32")
+    assert (np.abs(got - want) <= 2.01 * 2.0 ** -24 * np.abs(want) + 2.0 ** -149).all()
