@@ -357,3 +357,47 @@ def test_more_values_than_32_bits_count(mc, ref):
         want_codes, _ = ref.pack(code, scale_bytes, "e8m0_32")
         assert np.array_equal(codes[: sizes.codes_bytes].view(rows, -1)[r].cpu().numpy(), want_codes[0])
         assert np.array_equal(back[r].double().cpu().numpy(), ref.values(code, scale_bytes, "e8m0_32")[0])
+
+
+def _rounded_once(x, dtype):
+    """64-bit x to the nearest f16 or bf16, ties to even, subnormals included; past the end infinity."""
+    digits, lowest, most = {"f16": (11, -24, 65504.0), "bf16": (8, -133, float(2 - 2.0 ** -7) * 2.0 ** 127), "f32": (24, -149, float(np.finfo(np.float32).max))}[dtype]
+    step = np.exp2(np.maximum(np.frexp(x)[1] - digits, lowest).astype(np.float64))
+    r = np.rint(x / step) * step
+    return np.where(np.abs(r) > most, np.copysign(np.inf, r), r)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "f16"))
+@pytest.mark.parametrize("cols", (2016, 2015))
+def test_values_read_back_are_rounded_once(mc, ref, dtype, cols):
+    """code * scale * g has 6 + 24 bits, which 64-bit numbers hold: what is read back is its nearest, however near a tie it lies."""
+    import torch
+
+    rng = np.random.default_rng(8)
+    # every code under every scale, for tensor scales of any size
+    g = np.exp2(rng.uniform(-24, 3, 60)).astype(np.float32)
+    g = np.concatenate([g, np.exp2(rng.uniform(-149, 127, 60)).astype(np.float32), np.float32(1) + np.arange(1, 41).astype(np.float32) * np.float32(2.0 ** -23),
+                        np.arange(1, 20, dtype=np.float32) * np.float32(2.0 ** -149), np.float32([2.0 ** -126, 3.4e38])])
+    # scales that take a product as near to a tie of the result's type as f32 lets them: the f32 product lies on the tie
+    digits, lowest = {"f32": (24, -149), "bf16": (8, -133), "f16": (11, -24)}[dtype]
+    exponent = np.concatenate([rng.integers(-10, 11, 150), rng.integers(lowest - 2, lowest + digits, 100)])
+    tie = (2.0 ** (digits - 1) + rng.integers(0, 2 ** (digits - 1), 250) + 0.5) * np.exp2(np.maximum(exponent - digits + 1.0, lowest))
+    g = np.concatenate([g, (tie / rng.choice([1.125, 1.25, 1.375, 1.5, 1.625, 1.75, 1.875, 2.25, 2.625], 250)).astype(np.float32)])
+    g = g[g > 0]
+    code = np.tile(np.arange(16, dtype=np.uint8), 126)[None, :cols]
+    scale = np.minimum(np.arange(126, dtype=np.uint8), 0x7E)[None]
+    codes, tiles = ref.pack(code, scale, "e4m3_16")
+    batch = len(g)
+    dev = [torch.from_numpy(np.repeat(v[None], batch, axis=0)).cuda() for v in (codes, tiles)] + [torch.from_numpy(g).cuda()]
+    m = mc.Fp4Matrix("e4m3_16", 1, cols, dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), batch)
+    out = torch.empty(batch, cols, dtype=_torch_dtype(dtype), device="cuda")
+    torch.cuda.synchronize()
+    mc.fp4_dequantize(m, out.data_ptr(), dtype)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    want = np.stack([_rounded_once(ref.values(code, scale, "e4m3_16", float(v))[0], dtype) for v in g])
+    if dtype != "f32":
+        twice = np.stack([_rounded_once(_rounded_once(ref.values(code, scale, "e4m3_16", float(v))[0], "f32"), dtype) for v in g])
+        assert (twice != want).sum() > 200  # what two roundings would give is told apart
+    assert np.array_equal(got, want), int((got != want).sum())
