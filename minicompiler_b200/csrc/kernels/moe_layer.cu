@@ -707,6 +707,14 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
 
 // -------------------------------------------------------------------------------------------------------- up and down
 
+// v / (1 + exp(-v)) * up. With e = exp(-|v| / 2) that is v / (1 + e^2) * up, and for negative v times e^2, which is taken in two
+// halves: nothing on the way leaves f32's range unless the result does, however large `up` is.
+__device__ __forceinline__ float silu_times(float v, float up) {
+    const float e = expf(-0.5f * fabsf(v));
+    const float part = v < 0.0f ? e : 1.0f;
+    return __fdividef(v * part, fmaf(e, e, 1.0f)) * (up * part);  // a divisor of 1 to 2
+}
+
 template <int kHalves>
 struct UpWork {
     using S = Shape<kHalves, 1>;
@@ -786,7 +794,7 @@ struct UpWork {
             float h = 0.0f;
             if (n < here && r < p.f) {
                 const float gate = acc[j] * side.back[j], up = acc[2 + j] * side.back[j];
-                h = __fdividef(gate, 1.0f + expf(-gate)) * up;
+                h = silu_times(gate, up);
             }
             int e = static_cast<int>((__float_as_uint(h) >> 23) & 0xffu);
 #pragma unroll

@@ -39,7 +39,8 @@ class Tight(Problem):
                 bound[t] += weights[t, j] * (o_err + 32 * U * np.abs(o))
                 size += weights[t, j] * (np.abs(o) + o_err)
             bound[t] += (self.top_k + 8) * U * size
-        return y, bound + STEP[self.dtype] * (np.abs(y) + bound) + 2.0 ** -25, chosen, weights
+        smallest = {"f16": 2.0 ** -25, "bf16": 2.0 ** -134}[self.dtype]  # half a step of the subnormal numbers
+        return y, bound + STEP[self.dtype] * (np.abs(y) + bound) + smallest, chosen, weights
 
 
 def _differences(f, d, fmt, seed):
@@ -93,3 +94,49 @@ def test_the_layer_is_as_exact_as_its_result_type(mc, ref, fmt, tokens, experts,
     assert np.array_equal(p.chosen.cpu().numpy(), chosen)
     assert (np.abs(got - y) <= bound).all()
     assert np.linalg.norm(got - y) <= 1.3 * STEP["f16"] * (np.log(2) / 4.5) ** 0.5 * np.linalg.norm(y)
+
+
+def _silu_problem(mc, ref, gates, up_exponent):
+    """One expert whose h is silu(gate) * 2^up_exponent for each of the gates (sums of two numbers of a block), x of ones."""
+    f, d = len(gates), 32
+
+    def spoil(matrix, expert, code, scale):
+        code[:] = 0
+        if matrix == 1:
+            code[:f] = 2 * np.eye(f, dtype=np.uint8)  # y[i] = h[i]
+            scale[:] = 127
+        else:
+            for i, (first, second, e) in enumerate(gates):  # -(first + second) * 2^e, first and second magnitudes of the code
+                code[i, :2] = 8 + np.searchsorted(ref.MAGNITUDES, [first, second])
+                scale[i] = 127 + e
+            code[f:, 0] = 2
+            scale[f:] = 127 + up_exponent
+
+    x = np.zeros((1, d))
+    x[0, :2] = 1.0
+    return Problem(mc, ref, fmt="e8m0_32", dtype="bf16", tokens=1, experts=1, top_k=1, d=d, f=f, x=x, spoil=spoil)
+
+
+@pytest.mark.gpu
+def test_silu_of_very_negative_gates(mc, ref):  # noqa: F811
+    """silu(v) goes to 0 like v e^v: 1 + e^-v leaves f32 at -88.7 and a fast division gives up at -87.3, but times 2^100 the values
+    are ordinary numbers down to v = -150. bf16 rounds by 2^-8 of a value at most, the rest is far below."""
+    gates = [(3, 2, 4), (4, 1.5, 4), (4, 0, 0), (6, 0, 4), (6, 0.5, 4), (6, 1, 4), (6, 1.5, 4), (6, 2, 4), (6, 3, 4), (1, 0, 0), (0, 0, 0)]
+    gate = np.array([-(a + b) * 2.0 ** e for a, b, e in gates])
+    want = gate / (1 + np.exp(-gate)) * 2.0 ** 100
+    # values below 2^-50 of the largest of the token and expert are not kept; the large ones are in a layer of their own
+    for part in (gate < -20, gate >= -20):
+        q = _silu_problem(mc, ref, [v for v, keep in zip(gates, part) if keep], 100)
+        mine = q.run()[0][: part.sum()]
+        largest = np.abs(want[part]).max()
+        assert (np.abs(mine - want[part]) <= 2.0 ** -8 * 1.01 * np.abs(want[part]) + 2.0 ** -46 * largest).all(), (mine, want[part])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", [(6, 1, 4), (4, 1.5, 4), (6, 2, 4)])
+def test_silu_of_one_very_negative_gate(mc, ref, gate):  # noqa: F811
+    """-112, -88 and -128: alone in its layer each keeps its bits."""
+    v = -(gate[0] + gate[1]) * 2.0 ** gate[2]
+    got = _silu_problem(mc, ref, [gate], 100).run()[0][0]
+    want = v / (1 + np.exp(-v)) * 2.0 ** 100
+    assert abs(got - want) <= 2.0 ** -8 * 1.01 * abs(want)
