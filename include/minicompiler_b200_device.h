@@ -357,7 +357,7 @@ MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
  *  y          [tokens, d], ldy; only these elements are written
  *  chosen     [tokens, top_k] int32, best first, and weights [tokens, top_k] f32: device, either may be NULL
  *  workspace  mcd_moe_workspace(...) bytes, 16-byte aligned; calls that may run at the same time need one each
- * The products accumulate in f32. x enters them with 11 significant bits, silu(..) * (..) with 22, after a power of two per
+ * The products accumulate in f32. x enters them with 11 significant bits, silu(..) * (..), an f32 number, with 22, after a power of two per
  * token, or per token and expert, that takes their largest magnitude below 2^15: nothing of a bf16 or f16 x is lost above
  * 2^-29 of the token's largest value. The experts' results are added in an order that the routing alone fixes: results do not
  * depend on scheduling. Nothing in it waits, so there is no status word; three or four launches. */

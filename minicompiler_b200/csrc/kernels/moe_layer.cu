@@ -933,8 +933,7 @@ struct DownWork {
         }
     }
     struct Side {
-        float back;    // undoes h's shift, times the expert's tensor scale
-        float weight;
+        TwoFactors weight;  // the expert's for the token, times its tensor scale, and undoes h's shift
         int token;
     };
     // A lane's two columns are the two of one slot.
@@ -943,8 +942,9 @@ struct DownWork {
         const int at = routing.start[pass.active] + pass.first + min(static_cast<int>(threadIdx.x & 3), here - 1);
         const int slot = routing.slots[at];
         Side side;
-        side.back = power(-shift_of(p.h_max[slot])) * scale;
-        side.weight = p.weights[slot];
+        const float back = power(-shift_of(p.h_max[slot]));
+        side.weight = scale < back ? two_factors(scale, back) : two_factors(back, scale);
+        side.weight.second *= p.weights[slot];  // the larger one, where there are two
         side.token = routing.tokens[at];
         return side;
     }
@@ -954,8 +954,8 @@ struct DownWork {
         if (t < here) {
             // this warp's 16 columns; nobody else adds to them
             float* sum = sums + side.token * S::kPitch + tile * 16;
-            sum[g] += side.weight * (fmaf(acc[1], 0x1p-11f, acc[0]) * side.back);
-            sum[g + 8] += side.weight * (fmaf(acc[3], 0x1p-11f, acc[2]) * side.back);
+            sum[g] += side.weight.times(fmaf(acc[1], 0x1p-11f, acc[0]));
+            sum[g + 8] += side.weight.times(fmaf(acc[3], 0x1p-11f, acc[2]));
         }
     }
 };

@@ -140,3 +140,27 @@ def test_silu_of_one_very_negative_gate(mc, ref, gate):  # noqa: F811
     got = _silu_problem(mc, ref, [gate], 100).run()[0][0]
     want = v / (1 + np.exp(-v)) * 2.0 ** 100
     assert abs(got - want) <= 2.0 ** -8 * 1.01 * abs(want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x_sigma, gate_up_scale, down_scale", [(2.0 ** -40, 1.37 * 2.0 ** -20, 1.37 * 2.0 ** -36), (2.0 ** -40, 1.37 * 2.0 ** -20, 1.9 * 2.0 ** -34),
+                                                               (1.0, 1.37 * 2.0 ** -55, 1.37 * 2.0 ** -37), (2.0 ** 10, 1.37 * 2.0 ** 10, 1.37 * 2.0 ** -100)])
+@pytest.mark.parametrize("tokens", (2, 40))
+def test_tensor_scales_beside_the_shifts(mc, ref, tokens, x_sigma, gate_up_scale, down_scale):  # noqa: F811
+    """A tensor scale times the power of two that undoes a shift may be subnormal where the result is an ordinary number."""
+    import torch
+
+    d, f, experts = 64, 48, 5
+    rng = np.random.default_rng(4)
+    router = rng.standard_normal((experts, d)) * d ** -0.5 / x_sigma
+    p = Tight(mc, ref, fmt="e4m3_16", dtype="bf16", tokens=tokens, experts=experts, top_k=2, d=d, f=f, sigma=x_sigma, router=router)
+    for i, scale in enumerate((gate_up_scale, down_scale)):
+        old = p.keep[i][2].double().cpu().numpy()
+        new = np.full(experts, np.float32(scale))
+        p.keep[i][2].copy_(torch.from_numpy(new))
+        p.values[i] = [v / o * float(n) for v, o, n in zip(p.values[i], old, new)]
+    got = p.run()
+    y, bound, _, _ = p.expected()
+    fine = np.abs(y) >= 2.0 ** -122
+    assert fine.mean() > 0.9
+    assert (np.abs(got - y) <= bound)[fine].all(), float((np.abs(got - y) / bound)[fine].max())
