@@ -345,7 +345,7 @@ MCD_API int mcd_fp4_gemm_launches(const mcd_fp4_gemm_args* args);
 
 /* ------------------------------------------------- mixture of experts, few tokens
  * A whole layer: for each of 1 .. MCD_MOE_MAX_TOKENS tokens
- *   l = R x (products of 16-bit values, exact in f32, summed to twice f32's precision), p = softmax(l) over all experts,
+ *   l = R x (exact products, whatever their exponents, summed to twice f32's precision), p = softmax(l) over all experts,
  *   the top_k experts by l, ties and NaN to the lowest index (a NaN counts as lower than every number),
  *   w_j = p of the j-th one (renormalize != 0: divided by their sum),
  *   y = sum_j w_j * D_j (silu(G_j x) * (U_j x)),   silu(v) = v / (1 + exp(-v)).

@@ -172,7 +172,7 @@ __device__ __forceinline__ void add_exactly(float& sum, float& c, float v) {
 __device__ __forceinline__ void add_products(float& sum, float& c, const uint4& a, const uint4& b, int type) {
     const unsigned aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // products of 16-bit values are exact in f32
+    for (int i = 0; i < 4; ++i) {  // products of 16-bit values are exact in f32, see far_logit for the range
         add_exactly(sum, c, value16(aw[i] & 0xffffu, type) * value16(bw[i] & 0xffffu, type));
         add_exactly(sum, c, value16(aw[i] >> 16, type) * value16(bw[i] >> 16, type));
     }
@@ -194,6 +194,23 @@ __device__ __forceinline__ double lanes_sum(const float (&sum)[2], const float (
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     return total;
+}
+
+// Products of bf16 numbers reach from 2^-266 to 2^256. Where a logit leaves f32 above, its sum in f32 is not finite. Below, a
+// product is off by 2^-150 at most and 2^24 of them by 2^-126: less than the 2^-48 of all the sum's terms that it is
+// good for, if it is 2^-60 or more. All other logits are taken again in 64 bits, which hold every product.
+__device__ __forceinline__ bool is_far(double logit) { return !(fabs(logit) >= 0x1p-60 && fabs(logit) <= 3.402823466e38); }
+
+__device__ __noinline__ double far_logit(const unsigned short* x, const unsigned short* r, int d) {
+    const int lane = threadIdx.x & 31;
+    double sum = 0.0;
+#pragma unroll 8
+    for (int k = lane; k < d; k += 32) {
+        sum = fma(static_cast<double>(value16(x[k], MCD_HALF_BF16)), static_cast<double>(value16(r[k], MCD_HALF_BF16)), sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
 }
 
 __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads) mc_moe_router(const MoeParams p) {
@@ -252,7 +269,9 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
                 largest = packed_max(largest, make_uint4(a[i], 0, 0, 0));
             }
         }
-        const double total = lanes_sum(sum, c);
+        double total = lanes_sum(sum, c);
+        // `largest` speaks for all of x from the first expert on; a token of zeros (padding) needs no second look
+        if (p.type == MCD_HALF_BF16 && is_far(total) && (total != 0.0 || __any_sync(0xffffffffu, largest != 0))) total = far_logit(x, r, p.d);
         if (!started) {  // the first CTA of the cluster runs before its shared memory is written
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             started = true;

@@ -164,3 +164,39 @@ def test_tensor_scales_beside_the_shifts(mc, ref, tokens, x_sigma, gate_up_scale
     fine = np.abs(y) >= 2.0 ** -122
     assert fine.mean() > 0.9
     assert (np.abs(got - y) <= bound)[fine].all(), float((np.abs(got - y) / bound)[fine].max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x_exponent, router_exponent", [(-80, -80), (-100, -30), (-130, -10), (70, 70), (100, 28), (-120, 120), (0, -130)])
+@pytest.mark.parametrize("d", (96, 97, 1100))
+def test_the_choice_of_experts_at_any_exponent(mc, ref, x_exponent, router_exponent, d):  # noqa: F811
+    """Products of two bf16 numbers reach from 2^-266 to 2^256, further than f32: the choice is that of 64 bits all the same."""
+    rng = np.random.default_rng(d)
+    tokens, experts, top_k = 6, 70, 5
+    x = rng.standard_normal((tokens, d)) * 2.0 ** x_exponent
+    router = rng.standard_normal((experts, d)) * 2.0 ** router_exponent
+    p = Problem(mc, ref, fmt="e8m0_32", dtype="bf16", tokens=tokens, experts=experts, top_k=top_k, d=d, f=32, x=x, router=router, renormalize=False)
+    p.run()
+    logits = p.x64 @ p.router64.T
+    chosen = np.argsort(-logits, axis=1, kind="stable")[:, :top_k]
+    assert np.array_equal(p.chosen.cpu().numpy(), chosen)
+    weights = np.exp(logits - logits.max(axis=1, keepdims=True))
+    weights = np.take_along_axis(weights / weights.sum(axis=1, keepdims=True), chosen, axis=1)
+    assert np.allclose(p.weights.double().cpu().numpy(), weights, rtol=64 * U, atol=2.0 ** -126)
+
+
+@pytest.mark.gpu
+def test_products_that_mix_exponents(mc, ref):  # noqa: F811
+    """Large values of x that meet zeros of the router: only the products' own size says whether f32 holds them."""
+    d, experts = 64, 40
+    rng = np.random.default_rng(2)
+    x = np.zeros((2, d))
+    x[:, :32] = 1.0
+    x[0, 32:] = rng.standard_normal(32) * 2.0 ** -80
+    x[1, 32:] = rng.standard_normal(32) * 2.0 ** 80
+    router = np.zeros((experts, d))
+    router[:, 32:] = rng.standard_normal((experts, 32)) * 2.0 ** -70
+    p = Problem(mc, ref, fmt="e8m0_32", dtype="bf16", tokens=2, experts=experts, top_k=4, d=d, f=32, x=x, router=router)
+    p.run()
+    logits = p.x64 @ p.router64.T
+    assert np.array_equal(p.chosen.cpu().numpy(), np.argsort(-logits, axis=1, kind="stable")[:, :4])
