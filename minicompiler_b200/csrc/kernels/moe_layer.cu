@@ -213,6 +213,15 @@ __device__ __noinline__ double far_logit(const unsigned short* x, const unsigned
     return sum;
 }
 
+// exp(d) for d <= 0. A difference of logits has more bits than f32: what is left of it counts as exp(rest) = 1 + rest. Below
+// -200 it is 0.
+__device__ __forceinline__ float exp_below(double d) {
+    d = d < -200.0 ? -200.0 : d;
+    const float near = static_cast<float>(d);
+    const float e = expf(near);
+    return fmaf(e, static_cast<float>(d - near), e);
+}
+
 __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads) mc_moe_router(const MoeParams p) {
     // used in the cluster's first CTA
     __shared__ double logits[MCD_MOE_MAX_EXPERTS];
@@ -320,7 +329,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     __syncthreads();
     const double top = logits[best[0]];
     float total = 0.0f;
-    for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) total += expf(static_cast<float>(logits[e] - top));
+    for (int e = threadIdx.x; e < p.experts; e += kRouterThreads) total += exp_below(logits[e] - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) warp_sum[warp] = total;
@@ -329,7 +338,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     total = 0.0f;
     for (int w = 0; w < kRouterThreads / 32; ++w) total += warp_sum[w];
     float weight = 0.0f, kept = 0.0f;
-    if (lane < p.top_k) weight = expf(static_cast<float>(logits[best[lane]] - top)) / total;
+    if (lane < p.top_k) weight = exp_below(logits[best[lane]] - top) / total;
     for (int j = 0; j < p.top_k; ++j) kept += __shfl_sync(0xffffffffu, weight, j);
     if (lane < p.top_k) {
         if (p.renormalize) weight /= kept;

@@ -200,3 +200,22 @@ def test_products_that_mix_exponents(mc, ref):  # noqa: F811
     p.run()
     logits = p.x64 @ p.router64.T
     assert np.array_equal(p.chosen.cpu().numpy(), np.argsort(-logits, axis=1, kind="stable")[:, :4])
+
+
+@pytest.mark.gpu
+def test_weights_of_experts_far_below_the_best(mc, ref):  # noqa: F811
+    """Weights of logits some 80 below the best: the difference has more bits than f32, and a rounding of it would be 2^-18 of the
+    weight. A weight is off by expf (2 steps of 2^-23), the part that f32 leaves of the difference, the sum and the division: 8 steps."""
+    d, experts, top_k = 64, 16, 16
+    router = np.zeros((experts, d))
+    router[:, 0] = -np.linspace(0, 84, experts)
+    router[:, 1] = 2.0 ** -18 * (1 + np.arange(experts) % 3)
+    router[:, 2] = 1.01
+    x = np.zeros((3, d))
+    x[:, :3] = [[1, 1, 0], [1, 1, 3], [0.9, 1.7, 0.3]]
+    for renormalize in (False, True):
+        p = Problem(mc, ref, fmt="e8m0_32", dtype="bf16", tokens=3, experts=experts, top_k=top_k, d=d, f=32, x=x, router=router, renormalize=renormalize)
+        p.run()
+        _, _, chosen, weights = p.expected()
+        assert np.array_equal(p.chosen.cpu().numpy(), chosen)
+        assert np.allclose(p.weights.double().cpu().numpy(), weights, rtol=8 * U, atol=0)
