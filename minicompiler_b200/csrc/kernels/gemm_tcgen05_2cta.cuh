@@ -36,8 +36,8 @@ __device__ __forceinline__ void mc_tma_load_2d_pair(unsigned smem_dst, const McT
         : "memory");
 }
 
-// TMA store of one box from shared memory; completion is tracked in the issuing thread's bulk groups. Rows and
-// columns of the box that lie outside the tensor are not written.
+// TMA store of one box from shared memory; completion is tracked in the issuing thread's bulk groups. Rows of the box
+// that lie outside the tensor are not written, nor are pieces of 16 bytes of a row that lie outside as a whole.
 __device__ __forceinline__ void mc_tma_store_2d(const McTensorMap* map, unsigned smem_src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((unsigned long long)map),
                  "r"(smem_src), "r"(c0), "r"(c1)
@@ -60,6 +60,12 @@ __device__ __forceinline__ void mc_st_shared_v4u(unsigned addr, unsigned a, unsi
 
 __device__ __forceinline__ void mc_st_shared_v4(unsigned addr, float a, float b, float c, float d) {
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+__device__ __forceinline__ unsigned short mc_ld_shared_u16(unsigned addr) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ void mc_umma_pair(unsigned tmem_d, unsigned long long desc_a, unsigned long long desc_b, unsigned idesc,
@@ -361,6 +367,7 @@ __device__ __forceinline__ void mc_gemm_tc2_body(const McTensorMap& map_a, const
         const bool vec16 = (p.ldc16 & 7) == 0 && (((unsigned long long)p.c16) & 15) == 0;
         // Staged stores need the aligned fast paths of both outputs; anything else takes the direct per-row stores.
         const bool staged = p.staged != 0 && (p.c == nullptr || vec4) && (p.c16 == nullptr || vec16);
+        const bool whole_pieces = (p.c == nullptr || (p.n & 3) == 0) && (p.c16 == nullptr || (p.n & 7) == 0);
         const unsigned stage_base = bars_base + MC_TC2_BARRIER_BYTES + (unsigned)(warp - 2) * MC_TC2_STAGING_PER_WARP;
         int acc = 0;
         unsigned full_phase = 0;  // bit r: parity of region r's tmem_full barrier
@@ -427,7 +434,11 @@ __device__ __forceinline__ void mc_gemm_tc2_body(const McTensorMap& map_a, const
                         // the data never passes through the load/store unit again. Plain vector stores from the
                         // 8 warps were measured to hold up the MMAs of the next tile by 1.5 us per 256 x 256 tile (the
                         // same kernel with the stores left out, or with the TMEM reads alone, ran at the MMA rate).
-                        // TMA writes only the part of the box that lies inside the tensor, so ragged edges need no care.
+                        // TMA leaves out rows behind the last one, and columns in whole pieces of 16 bytes: a box that reaches
+                        // over the last column of a C whose rows are no such pieces would overwrite up to 14 bytes behind
+                        // each row. The warp writes that one from the staging buffer, a row at a time (8192 x 8190 x 1024 to
+                        // f16: 120 us, 137 with every lane on a row of its own).
+                        const bool by_tma = whole_chunk || whole_pieces;
                         if (p.c != nullptr) {
                             // 128-byte rows of FP32 through the whole buffer, one box at a time (two boxes of 16 columns
                             // taking turns in its halves measured no faster: 8192^3 1536 against 1538 TFLOP/s on one box)
@@ -438,9 +449,14 @@ __device__ __forceinline__ void mc_gemm_tc2_body(const McTensorMap& map_a, const
                                 mc_st_shared_v4(stage_base + lane * 128 + ((j ^ (lane & 7)) << 4), f[4 * j], f[4 * j + 1], f[4 * j + 2],
                                                 f[4 * j + 3]);
                             }
-                            mc_fence_async_shared();
+                            if (by_tma) mc_fence_async_shared();
                             __syncwarp();
-                            if (lane == 0) {
+                            if (!by_tma) {
+                                float* out = p.c + (long long)row_base * p.ldc + col0 + lane;
+                                for (int r = 0; r < min(32, p.m - row_base) && col0 + lane < p.n; ++r, out += p.ldc) {
+                                    *out = mc_ld_shared_f32(stage_base + r * 128 + ((((unsigned)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                }
+                            } else if (lane == 0) {
                                 mc_tma_store_2d(&map_c, stage_base, col0, row_base);
                                 if (p.c16 != nullptr) mc_tma_store_wait_read();  // the 16-bit form goes through the same buffer next
                             }
@@ -460,10 +476,20 @@ __device__ __forceinline__ void mc_gemm_tc2_body(const McTensorMap& map_a, const
                                                  mc_to_half2(f[8 * j + 4], f[8 * j + 5], p.c16_kind),
                                                  mc_to_half2(f[8 * j + 6], f[8 * j + 7], p.c16_kind));
                             }
-                            mc_fence_async_shared();
-                            __syncwarp();
-                            if (lane == 0) mc_tma_store_2d(&map_c16, half_buf, col0, row_base);
-                            ++buffer_turn;
+                            if (by_tma) {
+                                mc_fence_async_shared();
+                                __syncwarp();
+                                if (lane == 0) mc_tma_store_2d(&map_c16, half_buf, col0, row_base);
+                                ++buffer_turn;
+                            } else {
+                                // the next box takes this half again: the other one may still be on its way
+                                __syncwarp();
+                                unsigned short* out16 = p.c16 + (long long)row_base * p.ldc16 + col0 + lane;
+                                for (int r = 0; r < min(32, p.m - row_base) && col0 + lane < p.n; ++r, out16 += p.ldc16) {
+                                    *out16 = mc_ld_shared_u16(half_buf + r * 64 + ((((unsigned)lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+                                }
+                                __syncwarp();
+                            }
                         }
                     } else if (row < p.m) {
                         if (p.c != nullptr) {
