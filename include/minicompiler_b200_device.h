@@ -384,6 +384,7 @@ typedef struct mcd_moe_args {
     size_t workspace_bytes;
 } mcd_moe_args;
 
+/* 0 for sizes that mcd_moe_layer refuses: besides the limits above, top_k beyond experts and d or f beyond 2^24. */
 MCD_API size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f);
 MCD_API int mcd_moe_layer(const mcd_moe_args* args, void* stream);
 

@@ -1106,6 +1106,8 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     return p.tokens <= 32 ? launch_down<kFormat, 2, 3>(p, reached, s) : launch_down<kFormat, 2, 2>(p, reached, s);
 }
 
+constexpr long long kMaxWidth = 1 << 24;  // d and f
+
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 size_t in_eights(long long n) { return static_cast<size_t>((n + 7) / 8 * 8); }
@@ -1129,7 +1131,10 @@ Matrix4 matrix_of(const mcd_fp4_tensor& t) {
 }  // namespace
 
 extern "C" size_t mcd_moe_workspace(int tokens, int experts, int top_k, long long d, long long f) {
-    if (tokens < 1 || tokens > MCD_MOE_MAX_TOKENS || experts < 1 || top_k < 1 || top_k > MCD_MOE_MAX_TOP_K || d < 1 || f < 1) return 0;
+    if (tokens < 1 || tokens > MCD_MOE_MAX_TOKENS || experts < 1 || experts > MCD_MOE_MAX_EXPERTS || top_k < 1 || top_k > MCD_MOE_MAX_TOP_K ||
+        top_k > experts || d < 1 || d > kMaxWidth || f < 1 || f > kMaxWidth) {
+        return 0;
+    }
     const size_t slots = static_cast<size_t>(tokens) * static_cast<size_t>(top_k);
     return 3 * rounded(slots * 4) + rounded(static_cast<size_t>(tokens) * 4) + slots * in_eights(f) * 4 +
            rounded(static_cast<size_t>(tokens) * in_eights(d) * 2);
@@ -1151,7 +1156,7 @@ extern "C" int mcd_moe_layer(const mcd_moe_args* args, void* stream) {
     if (gu.format != dn.format) return fail("mcd_moe_layer: gate_up and down differ in format");
     if (gu.rows % 2 != 0 || gu.rows / 2 != dn.cols) return fail("mcd_moe_layer: gate_up has 2f rows where down has f columns");
     if (gu.cols != dn.rows) return fail("mcd_moe_layer: gate_up's columns are down's rows (d)");
-    if (gu.cols > (1 << 24) || dn.cols > (1 << 24)) return fail("mcd_moe_layer: d and f are at most 2^24");
+    if (gu.cols > kMaxWidth || dn.cols > kMaxWidth) return fail("mcd_moe_layer: d and f are at most 2^24");
     if (args->top_k < 1 || args->top_k > MCD_MOE_MAX_TOP_K || args->top_k > experts) {
         return fail("mcd_moe_layer: top_k is 1 to " + std::to_string(std::min(MCD_MOE_MAX_TOP_K, experts)) + ", got " + std::to_string(args->top_k));
     }

@@ -71,6 +71,18 @@ def test_null_arguments_and_workspace_of_refused_sizes(mc):
         assert mc.moe_workspace_bytes(*sizes) == 0
 
 
+def test_the_workspace_of_every_size_that_the_layer_refuses_is_nothing(mc):
+    """The layer's limits are those of its workspace: just inside there is one, just outside there is none."""
+    widest = 1 << 24
+    for inside, outside in [((1, 512, 2, 64, 64), (1, 513, 2, 64, 64)), ((1, 3, 3, 64, 64), (1, 3, 4, 64, 64)),
+                            ((1, 8, 2, widest, 64), (1, 8, 2, widest + 1, 64)), ((1, 8, 2, 64, widest), (1, 8, 2, 64, widest + 1)),
+                            ((64, 512, 16, widest, widest), (64, 512, 16, 1 << 62, 1 << 62))]:
+        assert mc.moe_workspace_bytes(*inside) > 0 and mc.moe_workspace_bytes(*outside) == 0
+    for change, message in [(dict(experts=513), "at most 512 experts"), (dict(experts=3, top_k=4), "top_k is 1 to 3"), (dict(d=widest + 1), "at most 2\\^24")]:
+        with pytest.raises(mc.McError, match=message):
+            _layer(mc, **change).enqueue()
+
+
 # ------------------------------------------------------------------------------------------------------ on a GPU
 
 
