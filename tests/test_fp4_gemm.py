@@ -344,3 +344,23 @@ def test_tensor_scales_whose_product_is_subnormal(mc, ref, m, n, k, ga, gb, byte
     want = a.values @ b.values.T
     got, _ = _product(mc, a, b, "f32")
     assert (np.abs(got - want) <= 2.01 * 2.0 ** -24 * np.abs(want) + 2.0 ** -149).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k, launches", [(5, 40, 200, 1), (3, 256, 8192, 1), (3, 256, 70000, 2), (300, 513, 321, 1), (300, 501, 6400, 1)])
+def test_the_launches_that_the_plan_says(mc, ref, m, n, k, launches):
+    """Whole, in clusters, through the workspace, pairs, pairs in slices: what is said beforehand is what was counted."""
+    import torch
+
+    rng = np.random.default_rng(3)
+    a, b = _exact_operand(mc, ref, rng, m, k, "e8m0_32"), _exact_operand(mc, ref, rng, n, k, "e8m0_32")
+    need = mc.fp4_gemm_workspace_bytes("e8m0_32", m, n, k)
+    assert (need > 0) == (launches == 2)
+    ws, c = torch.empty(max(16, need), dtype=torch.uint8, device="cuda"), torch.empty(m, n, device="cuda")
+    plan = mc.Fp4Gemm(a.m, b.m, c.data_ptr(), "f32", workspace=ws.data_ptr(), workspace_bytes=need)
+    torch.cuda.synchronize()
+    before = mc.lib().mcd_launch_count()
+    plan.enqueue()
+    counted = mc.lib().mcd_launch_count() - before
+    torch.cuda.synchronize()
+    assert plan.launches == launches == counted

@@ -384,3 +384,18 @@ def test_host_memory_is_refused(mc, ref):
     p.plan._args.x = host.ctypes.data
     with pytest.raises(mc.McError, match="not device memory"):
         p.plan.enqueue()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens, experts, top_k, d, launches", [(1, 8, 2, 64, 3), (16, 8, 2, 64, 3), (17, 8, 2, 64, 4), (6, 30, 5, 1024, 4), (6, 30, 5, 1025, 3), (64, 40, 8, 64, 4)])
+def test_three_launches_or_four(mc, ref, tokens, experts, top_k, d, launches):
+    """Three for up to 32 slots; a fourth levels h where there are more, or where few rows of y meet 24 experts."""
+    import torch
+
+    p = Problem(mc, ref, fmt="e8m0_32", dtype="bf16", tokens=tokens, experts=experts, top_k=top_k, d=d, f=32)
+    torch.cuda.synchronize()
+    before = mc.lib().mcd_launch_count()
+    p.plan.enqueue()
+    counted = mc.lib().mcd_launch_count() - before
+    torch.cuda.synchronize()
+    assert counted == launches
