@@ -302,8 +302,8 @@ mc_fp4_gemm(const __grid_constant__ McTensorMap map_rows, const __grid_constant_
                         for (int t = 0; t < Tile::kScaleTiles; ++t) {
                             const int tile = i * Tile::kScaleTiles + t;
                             if (t * (kFp4BlockK / kFp4MmaK / Tile::kScaleTiles) < steps) {
-                                fp4_scales_to_tmem<1>(scale_r + 4 * tile, fp4_scale_desc(scales_src + tile * kFp4TileBytes));
-                                fp4_scales_to_tmem<1>(scale_c + 4 * tile,
+                                fp4_scales_to_tmem(scale_r + 4 * tile, fp4_scale_desc(scales_src + tile * kFp4TileBytes));
+                                fp4_scales_to_tmem(scale_c + 4 * tile,
                                                       fp4_scale_desc(scales_src + (Tile::kBlocks * Tile::kScaleTiles + tile) * kFp4TileBytes));
                             }
                         }
@@ -618,7 +618,7 @@ struct Fp4PairParams {
     unsigned* status;
     long long ldc;
     int c_type;
-    int m, n, k, k_blocks;
+    int m, n, k_blocks;
     int splits, k_blocks_per_split;
     int by_tma;  // C leaves as TMA boxes; otherwise (alignment) row by row
 };
@@ -1226,8 +1226,7 @@ int launch_pairs(const mcd_fp4_gemm_args* args, const Plan& plan, cudaStream_t s
     p.c_type = args->c_type;
     p.m = static_cast<int>(args->a.rows);
     p.n = static_cast<int>(args->b.rows);
-    p.k = static_cast<int>(args->a.cols);
-    p.k_blocks = (p.k + kFp4BlockK - 1) / kFp4BlockK;
+    p.k_blocks = plan.k_blocks;
     p.splits = plan.splits;
     p.k_blocks_per_split = plan.per_split;
     p.by_tma = is_aligned(args->c, 16) && args->ldc % (args->c_type == MCD_TYPE_F32 ? 4 : 8) == 0;

@@ -32,13 +32,8 @@ constexpr unsigned fp4_instruction(int m, int n) {
 constexpr unsigned kFp4UpperScales = (2u << 4) | (2u << 29);
 
 // One scale tile into four TMEM columns, repeated for the four groups of 32 lanes.
-template <int kGroup>
 __device__ __forceinline__ void fp4_scales_to_tmem(unsigned taddr, unsigned long long desc) {
-    if constexpr (kGroup == 1) {
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    } else {
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    }
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 template <int kFormat, int kGroup>
