@@ -65,16 +65,17 @@ constexpr int kMaxSlots = MCD_MOE_MAX_TOKENS * MCD_MOE_MAX_TOP_K;
 // beside its multiplies (as many instructions as they have, for 1024 columns) is spread over twice the columns. Groups of
 // four or of two warps go through passes of their own, each with its barrier: the down projection's form of that, whose
 // CTAs must not grow beyond 64 rows.
-template <int kHalves, int kGroups>
+template <int kHalves, int kGroups, int kColumnTiles = 1>
 struct Shape {
     static constexpr int kGroupWarps = kWarps / kGroups;
     static constexpr int kGroupThreads = kGroupWarps * 32;
     static constexpr int kTiles = kGroupWarps / kHalves;
-    static constexpr int kRoundSteps = kHalves * kGroups == 1 ? 4 : kGroups == 4 ? 1 : 2;  // per warp
+    static constexpr int kColumns = kTokenTile * kColumnTiles;
+    static constexpr int kRoundSteps = kHalves * kGroups == 1 ? 4 : kGroups == 4 || kColumnTiles == 2 ? 1 : 2;  // per warp
     static constexpr int kRoundK = kStageK * kRoundSteps * kHalves;
     static constexpr int kValuePitch = 2 * (kRoundK + 32);  // bytes; 16 words past a multiple of 32: the four lanes of two tokens cover all banks
-    static constexpr int kValueBytes = kTokenTile * kValuePitch;
-    static constexpr int kPieces = kTokenTile * kRoundK / 8 / kGroupThreads;  // of 8 values of a column, per thread and round
+    static constexpr int kValueBytes = kColumns * kValuePitch;
+    static constexpr int kPieces = kColumns * kRoundK / 8 / kGroupThreads;  // of 8 values of a column, per thread and round
 };
 
 constexpr int kRouterCluster = 8;
@@ -451,7 +452,7 @@ __device__ __forceinline__ void load_routing(Routing& r, int* scratch, const Moe
     __syncthreads();
 }
 
-// What a CTA works through: rows of an expert against up to 8 (up) or 4 (down, two columns each) of its slots.
+// What a CTA works through: rows of an expert against up to 8 of its slots, or 4 (down, two columns each, in one tile of them).
 struct Pass {
     int active;  // which of the active experts
     int group;   // of rows (up only)
@@ -538,9 +539,9 @@ __device__ __forceinline__ int value_piece(int k) {
     return kFormat == MCD_FP4_E8M0_32 ? i : (i & ~15) | (i & 3) << 2 | (i >> 2 & 3);
 }
 
-// One step: 16 rows x 256 codes at `base` times the values at `values` (f16, token rows kValuePitch apart).
-template <int kFormat, int kValuePitch>
-__device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[2][4]) {
+// One step: 16 rows x 256 codes at `base` times the values at `values` (f16, columns kValuePitch apart).
+template <int kFormat, int kValuePitch, int kColumnTiles>
+__device__ __forceinline__ void multiply_step(const unsigned char* base, const unsigned char* values, float (&acc)[kColumnTiles][2][4]) {
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const unsigned char* v_at = values + g * kValuePitch + t * 16;
@@ -552,7 +553,6 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
         for (int b = 0; b < kStageK / 32; ++b) {
             const unsigned lo = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4));
             const unsigned hi = *reinterpret_cast<const unsigned*>(c_at + ((b ^ g) << 4) + 8 * 128);
-            const uint4 v = *reinterpret_cast<const uint4*>(v_at + b * 64);
             if ((b & 3) == 0) {
                 e8m0x4(*reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64), scale_lo);
                 e8m0x4(*reinterpret_cast<const unsigned*>(scales + (b >> 2) * 64 + 32), scale_hi);
@@ -560,13 +560,17 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
             unsigned a[4], c[4];
             fp4_decode8(lo, a);
             fp4_decode8(hi, c);
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(s, a[0], c[0], a[1], c[1], v.x, v.y);
-            mma16816(s, a[2], c[2], a[3], c[3], v.z, v.w);
-            acc[b & 1][0] = fmaf(s[0], scale_lo[b & 3], acc[b & 1][0]);
-            acc[b & 1][1] = fmaf(s[1], scale_lo[b & 3], acc[b & 1][1]);
-            acc[b & 1][2] = fmaf(s[2], scale_hi[b & 3], acc[b & 1][2]);
-            acc[b & 1][3] = fmaf(s[3], scale_hi[b & 3], acc[b & 1][3]);
+#pragma unroll
+            for (int n = 0; n < kColumnTiles; ++n) {
+                const uint4 v = *reinterpret_cast<const uint4*>(v_at + n * kTokenTile * kValuePitch + b * 64);
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma16816(s, a[0], c[0], a[1], c[1], v.x, v.y);
+                mma16816(s, a[2], c[2], a[3], c[3], v.z, v.w);
+                acc[n][b & 1][0] = fmaf(s[0], scale_lo[b & 3], acc[n][b & 1][0]);
+                acc[n][b & 1][1] = fmaf(s[1], scale_lo[b & 3], acc[n][b & 1][1]);
+                acc[n][b & 1][2] = fmaf(s[2], scale_hi[b & 3], acc[n][b & 1][2]);
+                acc[n][b & 1][3] = fmaf(s[3], scale_hi[b & 3], acc[n][b & 1][3]);
+            }
         }
     } else {
         // lane t: pieces t and t + 4 of a row, each two blocks of 16; their scales are one half of word (t + 4 q) / 2
@@ -583,14 +587,17 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
             const unsigned lo_w[4] = {lo.x, lo.y, lo.z, lo.w}, hi_w[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(v_at + q * 256 + i * 64);
                 unsigned a[4], c[4];
                 fp4_decode8(lo_w[i], a);
                 fp4_decode8(hi_w[i], c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) a[j] = mul_f16x2(a[j], s_lo[i >> 1]), c[j] = mul_f16x2(c[j], s_hi[i >> 1]);
-                mma16816(acc[0], a[0], c[0], a[1], c[1], v.x, v.y);
-                mma16816(acc[1], a[2], c[2], a[3], c[3], v.z, v.w);
+#pragma unroll
+                for (int n = 0; n < kColumnTiles; ++n) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(v_at + n * kTokenTile * kValuePitch + q * 256 + i * 64);
+                    mma16816(acc[n][0], a[0], c[0], a[1], c[1], v.x, v.y);
+                    mma16816(acc[n][1], a[2], c[2], a[3], c[3], v.z, v.w);
+                }
             }
         }
     }
@@ -604,10 +611,11 @@ __device__ __forceinline__ void multiply_step(const unsigned char* base, const u
 //   finish(piece, columns)    the same in f16, for each of its columns
 //   look(pass, here)          what a lane will need of its two columns, read before the multiplies
 //   done(pass, here, tile, side, acc)  a warp's sums, both halves of k
-template <int kFormat, int kHalves, int kGroups, int kStages, typename Work>
+template <int kFormat, int kHalves, int kGroups, int kColumnTiles, int kStages, typename Work>
 __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const Routing& routing, unsigned char* values, unsigned char* rings,
                                            float4* halves) {
-    using S = Shape<kHalves, kGroups>;
+    using S = Shape<kHalves, kGroups, kColumnTiles>;
+    static_assert(kHalves == 1 || kColumnTiles == 1, "halves meet in one tile of columns");
     constexpr int kTiles = S::kTiles, kRoundSteps = S::kRoundSteps, kRoundK = S::kRoundK, kValuePitch = S::kValuePitch;
     constexpr int kParts = Work::kParts, kPieces = S::kPieces / kParts;
     const int lane = threadIdx.x & 31, group = threadIdx.x / S::kGroupThreads;
@@ -690,7 +698,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
         }
     };
     int buffer = 1, slot = 0, round = -1;  // round -1: the first values only
-    float sums[2][4] = {};                 // two chains
+    float sums[kColumnTiles][2][4] = {};   // two chains
     while (more) {
         const typename Work::Side side = work.look(at, slots_of(at));
 #pragma unroll 1
@@ -705,7 +713,7 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
                     copy_next();  // into the slot of the step before, which all lanes have left
                     const int s = round * (kRoundSteps * kHalves) + half * kRoundSteps + j;
                     if (s < m.stages) {
-                        multiply_step<kFormat, kValuePitch>(ring + slot * Stage<kFormat>::kBytes,
+                        multiply_step<kFormat, kValuePitch, kColumnTiles>(ring + slot * Stage<kFormat>::kBytes,
                                                             values + buffer * S::kValueBytes + (half * kRoundSteps + j) * (kStageK * 2), sums);
                     }
                     copies_end();
@@ -716,15 +724,18 @@ __device__ __forceinline__ void run_passes(Work& work, const Matrix4& m, const R
             store_values(values + buffer * S::kValueBytes);
         }
         round = 0;
-        float acc[4];
+        float acc[kColumnTiles][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = sums[0][i] + sums[1][i], sums[0][i] = sums[1][i] = 0.0f;
+        for (int n = 0; n < kColumnTiles; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = sums[n][0][i] + sums[n][1][i], sums[n][0][i] = sums[n][1][i] = 0.0f;
+        }
         if constexpr (kHalves == 2) {
-            if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (half == 1) halves[tile * 32 + lane] = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
             sync();
             if (half == 0) {
                 const float4 other = halves[tile * 32 + lane];
-                acc[0] += other.x, acc[1] += other.y, acc[2] += other.z, acc[3] += other.w;
+                acc[0][0] += other.x, acc[0][1] += other.y, acc[0][2] += other.z, acc[0][3] += other.w;
             }
         }
         if (half == 0) work.done(at, slots_of(at), tile, side, acc);
@@ -811,7 +822,7 @@ struct UpWork {
         }
         return side;
     }
-    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[4]) const {
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[1][4]) const {
         const int lane = threadIdx.x & 31;
         const int g = lane >> 2, t = lane & 3;
         const int r = row_in_f(pass, tile, g);
@@ -821,7 +832,7 @@ struct UpWork {
             const int slot = side.slot[j];
             float h = 0.0f;
             if (n < here && r < p.f) {
-                const float gate = acc[j] * side.back[j], up = acc[2 + j] * side.back[j];
+                const float gate = acc[0][j] * side.back[j], up = acc[0][2 + j] * side.back[j];
                 h = silu_times(gate, up);
             }
             int e = static_cast<int>((__float_as_uint(h) >> 23) & 0xffu);
@@ -844,16 +855,20 @@ constexpr int kUpSmem = 2 * Shape<kHalves, 1>::kValueBytes + ring_bytes<kFormat>
 // experts of 2048 x 768: 40 us against 45), rings as deep as the sums beside them allow. Four, of two warps and 32 rows of y,
 // for few rows of y, which leave SMs without work otherwise (the layer, 64 tokens, 8 of 64 experts of 1024 x 1024: 86 us
 // against 101; 32 tokens, 1024 x 512: 44 against 48; 4 tokens, 1024 x 1024: 37 against 40). Eight of one warp were slower
-// throughout: nothing is shared among rows then.
-template <int kGroups>
-struct DownShape : Shape<kGroups == 1 ? 2 : 1, kGroups> {
+// throughout: nothing is shared among rows then. Two groups may take two tiles of columns, eight slots, in one pass: the codes
+// are decoded once for both, in rounds half as long (64 tokens, 8 of 64 experts of 2048 x 768: 139 us against 160; 8 of
+// 128: 143 against 156; 32 tokens, two slots per expert: 109 both ways; 64 tokens, 8 of 64 experts of 1024 x 1024: 109, 139
+// in four groups of one tile).
+template <int kGroups, int kColumnTiles>
+struct DownShape : Shape<kGroups == 1 ? 2 : 1, kGroups, kColumnTiles> {
     static constexpr int kRows = DownShape::kTiles * 16;
     static constexpr int kRowGroups = 128 / kRows;  // in 128 rows of y
     static constexpr int kPitch = kRows + 4;
 };
-template <int kFormat, int kGroups, int kStages>
+template <int kFormat, int kGroups, int kColumnTiles, int kStages>
 constexpr int down_smem(int tokens) {
-    return kGroups * (tokens * DownShape<kGroups>::kPitch * 4 + 2 * DownShape<kGroups>::kValueBytes) + ring_bytes<kFormat>(kStages);
+    using S = DownShape<kGroups, kColumnTiles>;
+    return kGroups * (tokens * S::kPitch * 4 + 2 * S::kValueBytes) + ring_bytes<kFormat>(kStages);
 }
 
 template <int kFormat, int kHalves>
@@ -864,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_up(const MoeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     load_routing(routing, reinterpret_cast<int*>(smem), p);
     UpWork<kHalves> work(p, routing);
-    run_passes<kFormat, kHalves, 1, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves, 1>::kValueBytes, halves);
+    run_passes<kFormat, kHalves, 1, 1, kUpStages>(work, p.gate_up, routing, smem, smem + 2 * Shape<kHalves, 1>::kValueBytes, halves);
 }
 
 // Eight values of h after the power of two of their slot's largest: hi, the nearest f16, and lo, 2^11 times what hi leaves, at
@@ -900,11 +915,11 @@ __global__ void __launch_bounds__(128) mc_moe_level(const MoeParams p) {
 }
 
 // One group: h lies as mc_moe_up left it, in f32; several: as mc_moe_level did, as the two f16 numbers.
-template <int kGroups>
+template <int kGroups, int kColumnTiles>
 struct DownWork {
-    using S = DownShape<kGroups>;
+    using S = DownShape<kGroups, kColumnTiles>;
     static constexpr bool kLevel = kGroups > 1;
-    static constexpr int kParts = 2, kSlots = kTokenTile / 2;
+    static constexpr int kParts = 2, kSlots = S::kColumns / 2;
     struct Piece {
         uint4 raw[2];
         int largest;
@@ -961,39 +976,46 @@ struct DownWork {
         }
     }
     struct Side {
-        TwoFactors weight;  // the expert's for the token, times its tensor scale, and undoes h's shift
-        int token;
+        TwoFactors weight[kColumnTiles];  // the expert's for the token, times its tensor scale, and undoes h's shift
+        int token[kColumnTiles];
     };
-    // A lane's two columns are the two of one slot.
+    // A lane's two columns of a tile are the two of one slot.
     __device__ __forceinline__ Side look(const Pass& pass, int here) const {
         const float scale = p.down.tensor_scale != nullptr ? p.down.tensor_scale[routing.active[pass.active]] : 1.0f;
-        const int at = routing.start[pass.active] + pass.first + min(static_cast<int>(threadIdx.x & 3), here - 1);
-        const int slot = routing.slots[at];
+        const int first_slot = routing.start[pass.active] + pass.first;
         Side side;
-        const float back = power(-shift_of(p.h_max[slot]));
-        side.weight = scale < back ? two_factors(scale, back) : two_factors(back, scale);
-        side.weight.second *= p.weights[slot];  // the larger one, where there are two
-        side.token = routing.tokens[at];
+#pragma unroll
+        for (int n = 0; n < kColumnTiles; ++n) {
+            const int at = first_slot + min(n * 4 + static_cast<int>(threadIdx.x & 3), here - 1);
+            const int slot = routing.slots[at];
+            const float back = power(-shift_of(p.h_max[slot]));
+            side.weight[n] = scale < back ? two_factors(scale, back) : two_factors(back, scale);
+            side.weight[n].second *= p.weights[slot];  // the larger one, where there are two
+            side.token[n] = routing.tokens[at];
+        }
         return side;
     }
-    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[4]) const {
+    __device__ __forceinline__ void done(const Pass& pass, int here, int tile, const Side& side, const float (&acc)[kColumnTiles][4]) const {
         const int lane = threadIdx.x & 31;
         const int g = lane >> 2, t = lane & 3;
-        if (t < here) {
-            // this warp's 16 columns; nobody else adds to them
-            float* sum = sums + side.token * S::kPitch + tile * 16;
-            sum[g] += side.weight.times(fmaf(acc[1], 0x1p-11f, acc[0]));
-            sum[g + 8] += side.weight.times(fmaf(acc[3], 0x1p-11f, acc[2]));
+#pragma unroll
+        for (int n = 0; n < kColumnTiles; ++n) {
+            if (n * 4 + t < here) {
+                // this warp's 16 columns; nobody else adds to them
+                float* sum = sums + side.token[n] * S::kPitch + tile * 16;
+                sum[g] += side.weight[n].times(fmaf(acc[n][1], 0x1p-11f, acc[n][0]));
+                sum[g + 8] += side.weight[n].times(fmaf(acc[n][3], 0x1p-11f, acc[n][2]));
+            }
         }
     }
 };
 
-template <int kFormat, int groups, int kStages>
+template <int kFormat, int groups, int kColumnTiles, int kStages>
 __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, int cluster) {
-    using S = DownShape<groups>;
+    using S = DownShape<groups, kColumnTiles>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Routing routing;
-    __shared__ float4 halves[kWarps / 2 * 32];
+    __shared__ float4 halves[groups == 1 ? kWarps / 2 * 32 : 1];
     unsigned char* values = smem;
     unsigned char* rings = values + groups * 2 * S::kValueBytes;
     float* sums = reinterpret_cast<float*>(rings + ring_bytes<kFormat>(kStages));  // [groups][tokens][kPitch]
@@ -1003,8 +1025,8 @@ __global__ void __launch_bounds__(kThreads, 2) mc_moe_down(const MoeParams p, in
     const int mine = threadIdx.x / S::kGroupThreads;
     for (int i = threadIdx.x; i < groups * group_sums; i += kThreads) sums[i] = 0.0f;
     load_routing(routing, reinterpret_cast<int*>(values), p);
-    DownWork<groups> work{p, routing, sums + mine * group_sums, rows, rank * groups + mine, cluster * groups};
-    run_passes<kFormat, groups == 1 ? 2 : 1, groups, kStages>(work, p.down, routing, values, rings, halves);
+    DownWork<groups, kColumnTiles> work{p, routing, sums + mine * group_sums, rows, rank * groups + mine, cluster * groups};
+    run_passes<kFormat, groups == 1 ? 2 : 1, groups, kColumnTiles, kStages>(work, p.down, routing, values, rings, halves);
     __syncthreads();
     if (cluster > 1) cluster_sync_all();
     // Every CTA of the cluster finishes its share of the elements: the partial sums in the order of ranks and groups.
@@ -1076,17 +1098,17 @@ int launch_up(MoeParams p, int reached, cudaStream_t s) {
     return launch(mc_moe_up<kFormat, kHalves>, grid, 1, kThreads, kUpSmem<kFormat, kHalves>, s, "mc_moe_up", p);
 }
 
-template <int kFormat, int kGroups, int kStages>
+template <int kFormat, int kGroups, int kColumnTiles, int kStages>
 int launch_down(MoeParams p, int reached, cudaStream_t s) {
-    using S = DownShape<kGroups>;
-    static_assert(down_smem<kFormat, kGroups, kStages>(MCD_MOE_MAX_TOKENS) + 10 * 1024 <= 227 * 1024, "shared memory");
+    using S = DownShape<kGroups, kColumnTiles>;
+    static_assert(down_smem<kFormat, kGroups, kColumnTiles, kStages>(MCD_MOE_MAX_TOKENS) + 10 * 1024 <= 227 * 1024, "shared memory");
     static SharedMemoryOnce once;
-    if (int rc = once.allow(mc_moe_down<kFormat, kGroups, kStages>, down_smem<kFormat, kGroups, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
+    if (int rc = once.allow(mc_moe_down<kFormat, kGroups, kColumnTiles, kStages>, down_smem<kFormat, kGroups, kColumnTiles, kStages>(MCD_MOE_MAX_TOKENS))) return rc;
     p.down.rounds = (p.f + S::kRoundK - 1) / S::kRoundK;
     int cluster = 8;
     while (cluster > reached) cluster /= 2;
     const auto grid = static_cast<unsigned>((p.d + 127) / 128 * S::kRowGroups * cluster);
-    return launch(mc_moe_down<kFormat, kGroups, kStages>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat, kGroups, kStages>(p.tokens), s,
+    return launch(mc_moe_down<kFormat, kGroups, kColumnTiles, kStages>, grid, static_cast<unsigned>(cluster), kThreads, down_smem<kFormat, kGroups, kColumnTiles, kStages>(p.tokens), s,
                   "mc_moe_down", p, cluster);
 }
 
@@ -1100,10 +1122,13 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     // Four groups per CTA where their clusters find SMs all at once, two CTAs on each, and there are experts for the groups.
     const bool spread = p.d <= 1024 && reached >= 24;
     // A launch of its own for h pays where many CTAs would each level the same rows of it: 32 row groups for every 2048 of d.
-    if (p.tokens * p.top_k <= 32 && !spread) return launch_down<kFormat, 1, 3>(p, reached, s);
+    if (p.tokens * p.top_k <= 32 && !spread) return launch_down<kFormat, 1, 1, 3>(p, reached, s);
     if (int rc = launch(mc_moe_level, static_cast<unsigned>(p.tokens * p.top_k), 1, 128, 0, s, "mc_moe_level", p)) return rc;
-    if (spread) return p.tokens <= 32 ? launch_down<kFormat, 4, 3>(p, reached, s) : launch_down<kFormat, 4, 2>(p, reached, s);
-    return p.tokens <= 32 ? launch_down<kFormat, 2, 3>(p, reached, s) : launch_down<kFormat, 2, 2>(p, reached, s);
+    // Two tiles of columns where most experts have more slots than the four of one.
+    const bool crowded = p.tokens * p.top_k > 3 * reached;
+    if (crowded) return p.tokens <= 32 ? launch_down<kFormat, 2, 2, 3>(p, reached, s) : launch_down<kFormat, 2, 2, 2>(p, reached, s);
+    if (spread) return p.tokens <= 32 ? launch_down<kFormat, 4, 1, 3>(p, reached, s) : launch_down<kFormat, 4, 1, 2>(p, reached, s);
+    return p.tokens <= 32 ? launch_down<kFormat, 2, 1, 3>(p, reached, s) : launch_down<kFormat, 2, 1, 2>(p, reached, s);
 }
 
 constexpr long long kMaxWidth = 1 << 24;  // d and f
