@@ -325,7 +325,8 @@ MCD_API int mcd_fp4_dequantize(const mcd_fp4_tensor* src, int type, void* dst, l
  *             written.
  *  workspace  mcd_fp4_gemm_workspace(args) bytes of device memory, 16-byte aligned, or NULL where that is 0. Calls that
  *             may run at the same time (two streams, two captured graphs) need one each.
- *  status     device word, may be NULL: a kernel that gives up a bounded wait ORs an error code in (as in mcd_gemm).
+ *  status     device word, may be NULL: a kernel that gives up a bounded wait (2 s) ORs an error code in (as in mcd_gemm).
+ *             c is unfinished then, and without the word nothing says so.
  * Results do not depend on scheduling: K slices are added in a fixed order. */
 typedef struct mcd_fp4_gemm_args {
     mcd_fp4_tensor a;

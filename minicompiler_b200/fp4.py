@@ -85,7 +85,10 @@ def fp4_gemm_workspace_bytes(fmt: str, m: int, n: int, k: int) -> int:
 
 
 class Fp4Gemm:
-    """mcd_fp4_gemm: c[m, n] = a[m, k] * b[n, k]^T, kept for any number of enqueue() calls."""
+    """mcd_fp4_gemm: c[m, n] = a[m, k] * b[n, k]^T, kept for any number of enqueue() calls.
+
+    `status`, a device word that is 0 at first, is where a kernel says that it gave up a wait of two seconds and left c
+    unfinished. Without one that shows nowhere: a program that has to know gives a word and looks at it where it reads c."""
 
     def __init__(self, a: Fp4Matrix, b: Fp4Matrix, c: int, c_dtype: str, ldc: int = 0, workspace: int = 0, workspace_bytes: int = 0,
                  status: int = 0):
