@@ -850,15 +850,14 @@ template <int kFormat>
 constexpr int ring_bytes(int stages) { return kWarps * stages * Stage<kFormat>::kBytes; }
 template <int kFormat, int kHalves>
 constexpr int kUpSmem = 2 * Shape<kHalves, 1>::kValueBytes + ring_bytes<kFormat>(kUpStages);
-// The down projection in one of three forms, by groups of warps. One group: the halves of a round, all warps on one expert after the
-// other, h as mc_moe_up left it. Two groups on experts of their own, h levelled before by mc_moe_level (32 tokens of 128
-// experts of 2048 x 768: 40 us against 45), rings as deep as the sums beside them allow. Four, of two warps and 32 rows of y,
-// for few rows of y, which leave SMs without work otherwise (the layer, 64 tokens, 8 of 64 experts of 1024 x 1024: 86 us
-// against 101; 32 tokens, 1024 x 512: 44 against 48; 4 tokens, 1024 x 1024: 37 against 40). Eight of one warp were slower
-// throughout: nothing is shared among rows then. Two groups may take two tiles of columns, eight slots, in one pass: the codes
-// are decoded once for both, in rounds half as long (64 tokens, 8 of 64 experts of 2048 x 768: 139 us against 160; 8 of
-// 128: 143 against 156; 32 tokens, two slots per expert: 109 both ways; 64 tokens, 8 of 64 experts of 1024 x 1024: 109, 139
-// in four groups of one tile).
+// The down projection in one of four forms. One group: the halves of a round, all warps on one expert after the other, h as
+// mc_moe_up left it. Two groups on experts of their own, h levelled before by mc_moe_level. Four, of two warps and 32 rows
+// of y, for few rows of y, which leave SMs without work otherwise (the layer, 4 tokens, 8 of 64 experts of 1024 x 1024: 36
+// us against 39 in two groups; 40 tokens, 8 of 160 of 1024 x 512: 71 against 78; 16 tokens, 8 of 64 of 512 x 512: 31 against
+// 32). And two groups with two tiles of columns, eight slots, in one pass: the codes are decoded once for both, in rounds
+// half as long (64 tokens, 8 of 64 experts of 2048 x 768: 139 us against 160; 8 of 128: 143 against 156; 32 tokens, two slots
+// per expert: 109 both ways; 64 tokens, 8 of 64 experts of 1024 x 1024: 109, 139 in four groups of one tile). Two CTAs have
+// to fit on an SM: with room for one, 32 tokens, 8 of 128 experts of 1024 x 512 took 81 us instead of 59.
 template <int kGroups, int kColumnTiles>
 struct DownShape : Shape<kGroups == 1 ? 2 : 1, kGroups, kColumnTiles> {
     static constexpr int kRows = DownShape::kTiles * 16;
@@ -1112,6 +1111,20 @@ int launch_down(MoeParams p, int reached, cudaStream_t s) {
                   "mc_moe_down", p, cluster);
 }
 
+// Whether two CTAs of the down projection have room on an SM (228 KB, of which a CTA takes one for itself).
+template <int kFormat, int kGroups, int kColumnTiles, int kStages>
+bool two_fit(int tokens) {
+    constexpr int kStatic = sizeof(Routing) + (kGroups == 1 ? kWarps / 2 * 32 : 1) * sizeof(float4) + 128;
+    return down_smem<kFormat, kGroups, kColumnTiles, kStages>(tokens) + kStatic + 1024 <= 114 * 1024;
+}
+
+// Rings as deep as the sums beside them allow.
+template <int kFormat, int kGroups, int kColumnTiles>
+int launch_levelled(const MoeParams& p, int reached, cudaStream_t s) {
+    return two_fit<kFormat, kGroups, kColumnTiles, 3>(p.tokens) ? launch_down<kFormat, kGroups, kColumnTiles, 3>(p, reached, s)
+                                                                 : launch_down<kFormat, kGroups, kColumnTiles, 2>(p, reached, s);
+}
+
 template <int kFormat>
 int launch_layer(const MoeParams& p, cudaStream_t s) {
     // The router's clusters are declared with the kernel.
@@ -1120,15 +1133,14 @@ int launch_layer(const MoeParams& p, cudaStream_t s) {
     const bool many = static_cast<long long>(reached) * (p.f_groups / Shape<2, 1>::kTiles) > 4LL * sm_count();
     if (int rc = many ? launch_up<kFormat, 1>(p, reached, s) : launch_up<kFormat, 2>(p, reached, s)) return rc;
     // Four groups per CTA where their clusters find SMs all at once, two CTAs on each, and there are experts for the groups.
-    const bool spread = p.d <= 1024 && reached >= 24;
+    const bool spread = p.d <= 1024 && reached >= 24 && two_fit<kFormat, 4, 1, 2>(p.tokens);
     // A launch of its own for h pays where many CTAs would each level the same rows of it: 32 row groups for every 2048 of d.
     if (p.tokens * p.top_k <= 32 && !spread) return launch_down<kFormat, 1, 1, 3>(p, reached, s);
     if (int rc = launch(mc_moe_level, static_cast<unsigned>(p.tokens * p.top_k), 1, 128, 0, s, "mc_moe_level", p)) return rc;
     // Two tiles of columns where most experts have more slots than the four of one.
     const bool crowded = p.tokens * p.top_k > 3 * reached;
-    if (crowded) return p.tokens <= 32 ? launch_down<kFormat, 2, 2, 3>(p, reached, s) : launch_down<kFormat, 2, 2, 2>(p, reached, s);
-    if (spread) return p.tokens <= 32 ? launch_down<kFormat, 4, 1, 3>(p, reached, s) : launch_down<kFormat, 4, 1, 2>(p, reached, s);
-    return p.tokens <= 32 ? launch_down<kFormat, 2, 1, 3>(p, reached, s) : launch_down<kFormat, 2, 1, 2>(p, reached, s);
+    if (crowded) return launch_levelled<kFormat, 2, 2>(p, reached, s);
+    return spread ? launch_levelled<kFormat, 4, 1>(p, reached, s) : launch_levelled<kFormat, 2, 1>(p, reached, s);
 }
 
 constexpr long long kMaxWidth = 1 << 24;  // d and f
