@@ -1057,7 +1057,7 @@ struct Plan {
 // the 128 lanes and is read once. Anything larger: SM pairs, however few their tiles (256 x 8192 x 8192 unsplit: 18 us, 36 in
 // tiles of 128 x 128; 1024^3: 12 against 23).
 //
-// K is split where the tiles leave half of the SMs without work: an SM draws some 70 GB/s at most. The slices of a tile are
+// K is split where the tiles leave half of the SMs without work, and their loads out of those in flight. The slices of a tile are
 // CTAs, or pairs, of one cluster, which adds them up from shared memory, as many as find SMs all at once: eight CTAs for 14
 // tiles, four for 32, three for 42.
 //   One CTA per slice: one token, 8192 x 8192: 11 us, 14 whole; 128 tokens: 14, 18 through a workspace and a second launch;

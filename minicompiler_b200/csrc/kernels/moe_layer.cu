@@ -12,11 +12,11 @@
 //   mc_moe_level   (where many CTAs read it) h to the two f16 numbers that the down projection multiplies
 //   mc_moe_down    a cluster of up to 8 CTAs takes 64 or 32 rows of y, its CTAs share the experts and add up what they found
 //
-// Where the time goes: for one token and 8 of 64 experts (26.7 MB of weights, 4 us to read) 25 us are the latencies of
+// Where the time goes: for one token and 8 of 64 experts (26.7 MB of weights, 4 us to read) 24 us are the latencies of
 // three dependent launches - routing, first copies, one round of multiplies, joining, each a microsecond or two. For 32
-// tokens and 128 experts of 2048 x 768 (294 MB, 46 us) 105 us: 49 up, 40 down. The SMs then issue instructions on 2.3 of 4
-// slots; half of them are the multiplies' (22 per 512 codes and warp), the rest what every pass of an expert's rows over
-// its 2 tokens costs beside.
+// tokens and 128 experts of 2048 x 768 (294 MB, 46 us) 106 to 110 us: 49 up, 44 down. Nothing is full then: instructions are
+// issued on 2.3 and 1.8 of 4 slots, DRAM is at 47 and 26 %, the tensor pipe at 20 and 11 %. What is left is latency that 16
+// warps per SM, a barrier per round and the chain of load, decode and multiply of a step do not cover.
 //
 // The products: codes are small numbers that f16 holds exactly, so a warp turns 16 rows of codes into f16 fragments
 // (one conversion for two codes) and multiplies them with 8 tokens' values by mma.sync m16n8k16, f32 sums. That
