@@ -364,3 +364,13 @@ def test_the_launches_that_the_plan_says(mc, ref, m, n, k, launches):
     counted = mc.lib().mcd_launch_count() - before
     torch.cuda.synchronize()
     assert plan.launches == launches == counted
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", FORMS)
+def test_a_nan_tensor_scale_makes_all_of_c_nan(mc, ref, m, n, k):
+    rng = np.random.default_rng(1)
+    for scales in ((float("nan"), 2.0 ** 5), (2.0 ** -100, float("nan"))):
+        a, b = (_far_operand(mc, ref, rng, rows, k, 0x38, g) for rows, g in zip((m, n), scales))
+        got, around = _product(mc, a, b, "bf16")
+        assert around and np.isnan(got).all()

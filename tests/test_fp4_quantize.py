@@ -401,3 +401,33 @@ def test_values_read_back_are_rounded_once(mc, ref, dtype, cols):
         twice = np.stack([_rounded_once(_rounded_once(ref.values(code, scale, "e4m3_16", float(v))[0], "f32"), dtype) for v in g])
         assert (twice != want).sum() > 200  # what two roundings would give is told apart
     assert np.array_equal(got, want), int((got != want).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("g", [None, 1.0, -0.37, float("nan"), float("inf"), 0.0, 2.0 ** -149, -(2.0 ** 120)])
+def test_reading_back_with_any_tensor_scale_and_nan_blocks(mc, ref, dtype, g):
+    """The signs of codes and of g multiply, a NaN scale makes its 16 values NaN, zeros of a block under an infinite g are NaN."""
+    import torch
+
+    rng = np.random.default_rng(12)
+    rows, cols = 5, 200
+    code = rng.integers(0, 16, size=(rows, cols)).astype(np.uint8)
+    scale = rng.integers(0, 0x7F, size=(rows, -(-cols // 16))).astype(np.uint8)
+    scale[2, 4] = 0x7F
+    scale[3, 1] = 0
+    codes, tiles = (torch.from_numpy(v).cuda() for v in ref.pack(code, scale, "e4m3_16"))
+    tg = torch.tensor([1.0 if g is None else g], dtype=torch.float32, device="cuda")
+    m = mc.Fp4Matrix("e4m3_16", rows, cols, codes.data_ptr(), tiles.data_ptr(), 0 if g is None else tg.data_ptr())
+    out = torch.empty(rows, cols, dtype=_torch_dtype(dtype), device="cuda")
+    torch.cuda.synchronize()
+    mc.fp4_dequantize(m, out.data_ptr(), dtype)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        values = ref.values(code, scale, "e4m3_16", float(tg.item()))
+        fine = np.isfinite(values)
+        want = values.copy()
+        want[fine] = _rounded_once(values[fine], dtype)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~np.isnan(want)], want[~np.isnan(want)])

@@ -219,3 +219,57 @@ def test_weights_of_experts_far_below_the_best(mc, ref):  # noqa: F811
         _, _, chosen, weights = p.expected()
         assert np.array_equal(p.chosen.cpu().numpy(), chosen)
         assert np.allclose(p.weights.double().cpu().numpy(), weights, rtol=8 * U, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens, experts, top_k, d, f", [(64, 1, 1, 33, 17), (33, 1, 1, 1025, 256), (40, 3, 2, 300, 1300), (34, 5, 4, 1100, 520), (64, 17, 16, 97, 257),
+                                                          (63, 30, 3, 200, 300), (64, 30, 3, 200, 300), (31, 60, 4, 130, 700), (32, 60, 4, 130, 700), (37, 40, 3, 1030, 90),
+                                                          (38, 40, 3, 1030, 90)])
+def test_every_form_of_the_down_projection(mc, ref, fmt, tokens, experts, top_k, d, f):  # noqa: F811
+    """Experts with many slots, on both sides of where the form or the depth of its rings changes."""
+    p = Tight(mc, ref, fmt=fmt, dtype="f16", tokens=tokens, experts=experts, top_k=top_k, d=d, f=f, seed=d + f)
+    got = p.run()
+    y, bound, chosen, _ = p.expected()
+    assert np.array_equal(p.chosen.cpu().numpy(), chosen)
+    assert (np.abs(got - y) <= bound).all(), float((np.abs(got - y) / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens, experts, top_k, d, f", [(40, 160, 3, 256, 192), (33, 40, 2, 1100, 100), (64, 6, 5, 1100, 300), (8, 20, 4, 1100, 300)])
+def test_the_same_bits_in_every_form(mc, ref, tokens, experts, top_k, d, f):  # noqa: F811
+    import torch
+
+    p = Problem(mc, ref, fmt="e4m3_16", dtype="bf16", tokens=tokens, experts=experts, top_k=top_k, d=d, f=f)
+    first = p.run()
+    for _ in range(10):
+        p.y_view[: tokens * d].fill_(float("nan"))
+        p.ws[: p.need].fill_(0xFF)
+        torch.cuda.synchronize()
+        assert np.array_equal(p.run(), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+def test_tokens_of_zeros_and_an_expert_that_is_not_a_number(mc, ref, dtype):  # noqa: F811
+    """A batch padded with zeros: these tokens choose the first experts, with equal weights, and get zeros. A router's row with a NaN
+    comes behind every number; the softmax over all experts is NaN then, and so are y and the weights, but not the choice."""
+    rng = np.random.default_rng(3)
+    tokens, experts, d = 12, 20, 72
+    x = rng.standard_normal((tokens, d))
+    x[5:] = 0.0
+    router = rng.standard_normal((experts, d)) * d ** -0.5
+    p = Problem(mc, ref, fmt="e8m0_32", dtype=dtype, tokens=tokens, experts=experts, top_k=3, d=d, f=48, x=x, router=router)
+    got = p.run()
+    y, bound, chosen, _ = p.expected()
+    assert np.array_equal(p.chosen.cpu().numpy(), chosen) and (chosen[5:] == [0, 1, 2]).all()
+    assert (np.abs(got - y) <= bound).all() and (got[5:] == 0).all()
+    assert (p.weights[5:] == p.weights[5, 0]).all()
+    router[7, 3] = np.nan
+    p = Problem(mc, ref, fmt="e8m0_32", dtype=dtype, tokens=tokens, experts=experts, top_k=experts - 4, d=d, f=48, x=x, router=router)
+    got = p.run()
+    logits = p.x64 @ p.router64.T
+    logits[:, 7] = -np.inf
+    want = np.argsort(-logits, axis=1, kind="stable")[:, : experts - 4]
+    assert np.array_equal(p.chosen.cpu().numpy(), want) and not (want == 7).any()
+    assert np.isnan(got).all() and np.isnan(p.weights.cpu().numpy()).all()
